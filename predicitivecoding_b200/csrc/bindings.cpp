@@ -23,6 +23,7 @@
 
 #include "gemm_api.h"
 #include "skinny_api.h"
+#include "vocab_api.h"
 
 // launchers defined in the .cu files
 int pcb_embed_fwd(const int* tok, const void* W, float* x, int M, int D, int V, cudaStream_t s);
@@ -348,6 +349,150 @@ void skinny_qkv_rope(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
   check(pcb_skinny_gemm(x.data_ptr(), row_stride(x, "x"), w.data_ptr(), row_stride(w, "w"), qo.data_ptr(), 0, 0, M,
                         N, K, splits, nullptr, nullptr, 0, &r, cur_stream()),
         "skinny_qkv_rope");
+}
+
+// ---------------------------------------------------------------- the vocabulary ends of a decoder
+int is64(const at::Tensor& t, const char* name) {
+  PCB_CHECK(t.is_cuda() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), name,
+            " must be an int32 or int64 CUDA tensor");
+  return t.scalar_type() == at::kLong ? 1 : 0;
+}
+int is_bf16(const at::Tensor& t, const char* name) {
+  PCB_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat), name,
+            " must be a bf16 or fp32 CUDA tensor");
+  return t.scalar_type() == at::kBFloat16 ? 1 : 0;
+}
+
+// Loss of the vocabulary head.  x [N, D], w [V, D] bf16; either tgt [N] or ids, logits [N, K].  Allocates and returns
+// (row losses [N], scalars [2], the forward's buffer, w as the GEMMs read it: w itself, or a copy with 16-byte rows).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> vocab_fwd(
+    const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& tgt, int64_t ignore,
+    const c10::optional<at::Tensor>& ids, const c10::optional<at::Tensor>& logits, double temperature, bool mean) {
+  req(x, at::kBFloat16, "x");
+  req(w, at::kBFloat16, "w");
+  pcb::VocabHeadArgs a{};
+  a.ldx = row_stride(x, "x");
+  a.ldw = row_stride(w, "w");
+  a.N = x.size(0);
+  a.D = x.size(1);
+  a.V = w.size(0);
+  PCB_CHECK(w.size(1) == a.D, "vocab_fwd: w must be [V, D]");
+  PCB_CHECK(a.N >= 1 && a.V >= 1 && a.D >= 1, "vocab_fwd: empty operand");
+  a.K = 1;
+  a.temperature = 1.f;
+  if (tgt) {
+    a.tgt64 = is64(*tgt, "targets");
+    PCB_CHECK(tgt->is_contiguous() && tgt->numel() == a.N, "vocab_fwd: targets must be [N] contiguous");
+    a.tgt = tgt->data_ptr();
+    a.ignore = ignore;
+  } else {
+    PCB_CHECK(ids && logits && ids->dim() == 2 && ids->sizes() == logits->sizes() && ids->size(0) == a.N,
+              "vocab_fwd: ids and logits must be [N, K]");
+    a.ids64 = is64(*ids, "ids");
+    a.logits_bf16 = is_bf16(*logits, "logits");
+    a.ld_ids = row_stride(*ids, "ids");
+    a.ld_logits = row_stride(*logits, "logits");
+    a.ids = ids->data_ptr();
+    a.logits = logits->data_ptr();
+    a.K = ids->size(1);
+    a.temperature = (float)temperature;
+  }
+  const at::cuda::CUDAGuard guard(x.device());
+  at::Tensor wr = w;
+  if (a.ldw % 8 != 0 || a.ldw < a.D || (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) != 0) {
+    const int64_t ld = (a.D + 7) / 8 * 8;
+    wr = at::empty({a.V, ld}, w.options());
+    check(pcb_vocab_pad_rows(w.data_ptr(), a.ldw, wr.data_ptr(), ld, a.V, a.D, cur_stream()), "vocab_pad_rows");
+    a.ldw = ld;
+  }
+  a.x = x.data_ptr();
+  a.w = wr.data_ptr();
+  const pcb::VocabLayout l = pcb::vocab_layout(a.N, a.V, a.D, a.K, !tgt);
+  at::Tensor saved = at::empty({l.bytes}, x.options().dtype(at::kByte));
+  at::Tensor part = at::empty({(int64_t)l.granules * a.N * 2}, x.options().dtype(at::kFloat));
+  at::Tensor loss = at::empty({a.N}, x.options().dtype(at::kFloat));
+  at::Tensor scalars = at::empty({2}, x.options().dtype(at::kFloat));
+  a.loss = loss.data_ptr<float>();
+  a.scalars = scalars.data_ptr<float>();
+  check(pcb_vocab_fwd(a, saved.data_ptr(), part.data_ptr(), mean ? 1 : 0, num_sms(), cur_stream()), "vocab_fwd",
+        tgt ? 4 : 5);
+  return {loss, scalars, saved, wr};
+}
+
+// Gradients of vocab_fwd's loss into dx [N, D] and dw [V, D] (either may be absent).  Allocates its workspaces.
+void vocab_bwd(const at::Tensor& saved, const at::Tensor& scalars, const at::Tensor& w, int64_t N, int64_t V, int64_t D,
+               int64_t K, bool distill, double temperature, bool mean, double gout,
+               const c10::optional<at::Tensor>& gout_dev, const c10::optional<at::Tensor>& dx,
+               const c10::optional<at::Tensor>& dw, bool dw_add, int64_t piece) {
+  pcb::VocabGradArgs a{};
+  a.w = w.data_ptr();
+  a.ldw = row_stride(w, "w");
+  a.N = N;
+  a.V = V;
+  a.D = D;
+  a.K = K;
+  a.distill = distill;
+  a.temperature = (float)temperature;
+  PCB_CHECK(saved.numel() == pcb::vocab_layout(N, V, D, K, distill).bytes, "vocab_bwd: saved is of another loss");
+  a.saved = saved.data_ptr();
+  a.scalars = scalars.data_ptr<float>();
+  a.gout = (float)gout;
+  if (gout_dev) {
+    req(*gout_dev, at::kFloat, "gout");
+    PCB_CHECK(gout_dev->numel() == 1, "vocab_bwd: gout must hold one value");
+    a.gout_dev = gout_dev->data_ptr<float>();
+  }
+  a.mean = mean;
+  if (dx) {
+    a.dx_f32 = !is_bf16(*dx, "dx");
+    PCB_CHECK(dx->dim() == 2 && dx->size(0) == N && dx->size(1) == D, "vocab_bwd: dx must be [N, D]");
+    a.dx = dx->data_ptr();
+    a.lddx = row_stride(*dx, "dx");
+  }
+  if (dw) {
+    a.dw_f32 = !is_bf16(*dw, "dw");
+    PCB_CHECK(dw->dim() == 2 && dw->size(0) == V && dw->size(1) == D, "vocab_bwd: dw must be [V, D]");
+    a.dw = dw->data_ptr();
+    a.lddw = row_stride(*dw, "dw");
+  }
+  a.dw_add = dw_add;
+  const at::cuda::CUDAGuard guard(w.device());
+  pcb::vocab_plan(N, V, D, (int)piece, num_sms(), &a.piece, &a.splits);
+  const int pieces = (V + a.piece - 1) / a.piece;
+  a.ld_slab = (D + 3) / 4 * 4;
+  at::Tensor g = at::empty({N * a.piece}, w.options().dtype(at::kBFloat16));
+  at::Tensor slab;
+  a.g = g.data_ptr();
+  if (dx) {
+    slab = at::empty({a.splits * N * a.ld_slab}, w.options().dtype(at::kFloat));
+    a.slab = slab.data_ptr<float>();
+  }
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "vocab_bwd", pieces * (1 + (dx ? 1 : 0) + (dw ? 1 : 0)) + (dx ? 1 : 0));
+}
+
+void vocab_embed_fwd(const at::Tensor& tok, const at::Tensor& w, double scale, at::Tensor& x) {
+  const int t64 = is64(tok, "tok"), wb = is_bf16(w, "w"), xb = is_bf16(x, "x");
+  const int64_t N = tok.numel(), V = w.size(0), D = w.size(1);
+  PCB_CHECK(tok.is_contiguous() && x.is_contiguous() && x.numel() == N * D, "embed_fwd: x must be [N, D] contiguous");
+  PCB_CHECK(N >= 1 && V >= 1 && D >= 1, "embed_fwd: empty operand");
+  const at::cuda::CUDAGuard guard(w.device());
+  check(pcb_vocab_embed_fwd(tok.data_ptr(), t64, w.data_ptr(), wb, row_stride(w, "w"), x.data_ptr(), xb, N, V, D,
+                            (float)scale, cur_stream()),
+        "vocab_embed_fwd");
+}
+
+// Allocates its workspace.
+void vocab_embed_bwd(const at::Tensor& tok, const at::Tensor& dx, double scale, at::Tensor& dw, bool add) {
+  const int t64 = is64(tok, "tok"), wb = is_bf16(dw, "dw"), xb = is_bf16(dx, "dx");
+  const int64_t N = tok.numel(), V = dw.size(0), D = dw.size(1);
+  PCB_CHECK(tok.is_contiguous() && dw.is_contiguous(), "embed_bwd: tok and dw must be contiguous");
+  PCB_CHECK(dx.dim() == 2 && dx.size(0) == N && dx.size(1) == D, "embed_bwd: dx must be [N, D]");
+  PCB_CHECK(N >= 1 && V >= 1 && D >= 1, "embed_bwd: empty operand");
+  const at::cuda::CUDAGuard guard(dw.device());
+  at::Tensor ws = at::empty({pcb_vocab_embed_bwd_bytes(N, V, D)}, dw.options().dtype(at::kByte));
+  check(pcb_vocab_embed_bwd(tok.data_ptr(), t64, dx.data_ptr(), xb, row_stride(dx, "dx"), dw.data_ptr(), wb, N, V, D,
+                            (float)scale, add ? 1 : 0, ws.data_ptr(), num_sms(), cur_stream()),
+        "vocab_embed_bwd", 8);
 }
 
 // ---------------------------------------------------------------- mixture of experts
@@ -974,6 +1119,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("skinny_gemm", &skinny_gemm, py::arg("x"), py::arg("w"), py::arg("y"), py::arg("err") = py::none(),
         py::arg("trace") = py::none(), py::arg("swiglu") = false);
   m.def("skinny_qkv_rope", &skinny_qkv_rope);
+  m.def("vocab_fwd", &vocab_fwd);
+  m.def("vocab_bwd", &vocab_bwd);
+  m.def("vocab_embed_fwd", &vocab_embed_fwd);
+  m.def("vocab_embed_bwd", &vocab_embed_bwd);
   m.def("moe_route", &moe_route);
   m.def("moe_dispatch", &moe_dispatch);
   m.def("moe_gather", &moe_gather);

@@ -1,0 +1,843 @@
+// The two ends of a decoder over its vocabulary: embedding lookup and its gradient, and the vocabulary head's losses
+// (softmax cross entropy; distillation from a teacher's top logits) with their gradients.
+//
+// Head.  With x [N, D], w [V, D], logits l = x w^T and a target distribution per row (one id of weight 1, or the
+// softmax q of K teacher logits at temperature T):
+//     loss_n = T^2 sum_k q_k (log q_k - log p_k),  p = softmax(l / T)   (T = 1, one target: lse(l) - l_t)
+//     d loss_n / d l = T (p - q),   dx = c (p - q) w,   dw = c (p - q)^T x,   c = T gout / counted rows
+// The logits [N, V] are never kept.  The forward's GEMM epilogue reduces each row's 128 columns to (max, sum) and picks
+// the logits at the targets; the backward makes the logits again, a piece of the vocabulary at a time, and its
+// epilogue turns them into bf16 p - q, which two more GEMMs read: dw of the piece is finished there, dx is
+// accumulated over the pieces in fp32.  8 N V D operations instead of 6, for N * piece * 2 bytes of workspace.
+// Rows without a target (masked prompts, padding) are taken out first: the counted rows are packed in order,
+// every GEMM runs over their number, known on the device only, and what stands in the other rows (NaN too) is
+// never read.
+#include <algorithm>
+#include <cstdio>
+
+#include "common.cuh"
+#include "gemm_api.h"
+#include "vocab_api.h"
+
+namespace pcb {
+namespace vocab {
+
+constexpr int kThreads = 256;
+constexpr int kMaxK = 256;   // teacher entries per row
+
+PCB_DEVICE long long load_id(const void* p, int is64, long long i) {
+  return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+// Exclusive prefix sum of one int per thread over the block (blockDim a multiple of 32, at most 1024); total in *sum.
+PCB_DEVICE int block_scan(int v, int* warp_sums, int* sum) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();   // the sums of the previous call have been read
+  if (lane == 31) warp_sums[w] = inc;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int i = 0; i < nw; ++i) {
+    if (i < w) before += warp_sums[i];
+    total += warp_sums[i];
+  }
+  *sum = total;
+  return before + inc - v;
+}
+
+// ---------------------------------------------------------------- packing
+// Packs the counted rows in order.  Block b owns rows [b R, (b + 1) R) and counts the rows before them by itself, so
+// that one launch does it without a scan over the blocks (8 bytes a row from L2, against 2 D a row copied).
+__global__ void __launch_bounds__(kThreads)
+    pack_rows_kernel(const void* __restrict__ tgt, int tgt64, long long ignore, const int* __restrict__ len, int V,
+                     const __nv_bfloat16* __restrict__ x, long long ldx, int N, int D, int R, int vec,
+                     __nv_bfloat16* __restrict__ xc, long long ldxc, int* __restrict__ row, int* __restrict__ pos,
+                     int* __restrict__ tgt32, int* __restrict__ count) {
+  __shared__ int sums[kThreads / 32];
+  __shared__ int src[kThreads];
+  auto counted = [&](int n) -> bool {
+    if (len != nullptr) return len[n] > 0;
+    const long long t = load_id(tgt, tgt64, n);
+    return t >= 0 && t < V && t != ignore;
+  };
+  auto zero_or_copy = [&](int n, long long j) {   // one warp: packed row j from row n, or zeros (n < 0)
+    const int lane = threadIdx.x & 31;
+    __nv_bfloat16* d = xc + j * ldxc;
+    if (vec) {
+      const uint4* s = reinterpret_cast<const uint4*>(x + (long long)max(n, 0) * ldx);
+      for (int i = lane; i < (int)(ldxc / 8); i += 32)
+        reinterpret_cast<uint4*>(d)[i] = n < 0 ? make_uint4(0, 0, 0, 0) : s[i];
+    } else {
+      const __nv_bfloat16* s = x + (long long)max(n, 0) * ldx;
+      for (int i = lane; i < (int)ldxc; i += 32) d[i] = n >= 0 && i < D ? s[i] : __float2bfloat16_rn(0.f);
+    }
+  };
+  const int r0 = (int)min((long long)N, (long long)blockIdx.x * R), r1 = (int)min((long long)N, (long long)r0 + R);
+  int before = 0;
+  for (int n = threadIdx.x; n < r0; n += kThreads) before += counted(n) ? 1 : 0;
+  int base;
+  block_scan(before, sums, &base);
+  for (int t0 = r0; t0 < r1; t0 += kThreads) {
+    const int n = t0 + threadIdx.x;
+    const bool c = n < r1 && counted(n);
+    int total;
+    const int k = block_scan(c ? 1 : 0, sums, &total);
+    if (n < r1) {
+      pos[n] = c ? base + k : -1;
+      if (tgt32 != nullptr) tgt32[n] = c ? (int)load_id(tgt, tgt64, n) : -1;
+    }
+    if (c) {
+      row[base + k] = n;
+      src[k] = n;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < total; i += kThreads / 32) zero_or_copy(src[i], base + i);
+    base += total;
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x == 0) *count = base;
+    const int end = min(N, (max(base, 1) + 63) / 64 * 64);
+    for (int j = base + (threadIdx.x >> 5); j < end; j += kThreads / 32) zero_or_copy(-1, j);
+  }
+}
+
+__global__ void pad_rows_kernel(const __nv_bfloat16* __restrict__ src, long long ld, __nv_bfloat16* __restrict__ dst,
+                                long long ldd, long long total, int D) {
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const long long r = i / ldd;
+    const int c = (int)(i - r * ldd);
+    dst[i] = c < D ? src[r * ld + c] : __float2bfloat16_rn(0.f);
+  }
+}
+
+// ---------------------------------------------------------------- the teacher's lists
+// One warp per row: the softmax of the entries present, and the entries in ascending id (rank = number of smaller
+// ids, ties by place), so that a thread of the GEMM's epilogue meets its row's targets in column order.
+__global__ void __launch_bounds__(kThreads)
+    sort_targets_kernel(const void* __restrict__ ids, int ids64, long long ld_ids, const void* __restrict__ logits,
+                        int bf16, long long ld_logits, int N, int V, int K, float c, int* __restrict__ out_ids,
+                        float* __restrict__ out_q, float* __restrict__ out_lq, int* __restrict__ out_len,
+                        unsigned short* __restrict__ start, int granules) {
+  __shared__ int s_id[kThreads / 32][kMaxK];
+  __shared__ int s_sorted[kThreads / 32][kMaxK];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = blockIdx.x * (kThreads / 32) + w;
+  if (n >= N) return;   // whole warps
+  int id[kMaxK / 32];
+  float y[kMaxK / 32];
+  float mx = -INFINITY;
+  int mine = 0;
+#pragma unroll
+  for (int r = 0; r < kMaxK / 32; ++r) {
+    const int k = lane + 32 * r;
+    id[r] = -1;
+    y[r] = -INFINITY;
+    if (k < K) {
+      const long long t = load_id(ids, ids64, n * ld_ids + k);
+      const long long at = n * ld_logits + k;
+      const float l = bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(logits)[at])
+                           : reinterpret_cast<const float*>(logits)[at];
+      if (t >= 0 && t < V && l != -INFINITY) {
+        id[r] = (int)t;
+        y[r] = l * c;
+        ++mine;
+      }
+      s_id[w][k] = id[r];
+    }
+    mx = fmaxf(mx, y[r]);
+  }
+  mx = warp_max(mx);
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < kMaxK / 32; ++r)
+    if (id[r] >= 0) sum += exp2f(y[r] - mx);
+  sum = warp_sum(sum);
+  const int present = __reduce_add_sync(0xffffffffu, mine);
+  const float ls = log2f(sum);
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < kMaxK / 32; ++r) {
+    if (id[r] < 0) continue;
+    const int k = lane + 32 * r;
+    int rank = 0;
+    for (int i = 0; i < K; ++i) {
+      const int o = s_id[w][i];
+      rank += o >= 0 && (o < id[r] || (o == id[r] && i < k)) ? 1 : 0;
+    }
+    s_sorted[w][rank] = id[r];
+    const long long at = (long long)n * K + rank;
+    out_ids[at] = id[r];
+    out_q[at] = exp2f(y[r] - mx) / sum;
+    out_lq[at] = y[r] - mx - ls;
+  }
+  __syncwarp();
+  if (lane == 0) out_len[n] = present;
+  for (int g = lane; g <= granules; g += 32) {   // entries with an id below 128 g
+    int lo = 0, hi = present;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_sorted[w][mid] < g * 128LL) lo = mid + 1;
+      else hi = mid;
+    }
+    start[(long long)g * N + n] = (unsigned short)lo;
+  }
+}
+
+// ---------------------------------------------------------------- row losses
+// 32 rows a block, 8 threads a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.
+__global__ void __launch_bounds__(256)
+    row_loss_kernel(const float2* __restrict__ part, int granules, long long ld_part, const int* __restrict__ pos,
+                    const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
+                    const int* __restrict__ len, int N, int K, float c, float factor, float* __restrict__ lse_out,
+                    float* __restrict__ loss) {
+  __shared__ float sm[8][33], ss[8][33], sl[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = blockIdx.x * 32 + tx;
+  const int j = n < N ? pos[n] : -1;
+  float m = -INFINITY, s = 0.f;
+  if (j >= 0) {
+#pragma unroll 4
+    for (int g = ty; g < granules; g += 8) {
+      const float2 p = part[g * ld_part + j];
+      const float nm = fmaxf(m, p.x);
+      const float ref = nm == -INFINITY ? 0.f : nm;
+      s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+      m = nm;
+    }
+  }
+  sm[ty][tx] = m;
+  ss[ty][tx] = s;
+  __syncthreads();
+  float mm = -INFINITY, tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mm = fmaxf(mm, sm[i][tx]);
+  const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) tot += ss[i][tx] * exp2f(sm[i][tx] - ref);
+  const float lse = ref + log2f(tot);
+  // sum_k q_k (log2 q_k + lse - c z_k), term by term: each is a difference of logarithms of the same size
+  float l = 0.f;
+  if (j >= 0) {
+    const long long at = (long long)n * K;
+    const int e = len != nullptr ? len[n] : 1;
+    for (int k = ty; k < e; k += 8) {
+      const float d = fmaf(-c, z[at + k], lse);
+      if (q == nullptr) l += d;
+      else if (q[at + k] != 0.f) l += q[at + k] * (lq[at + k] + d);   // 0 log 0 = 0
+    }
+  }
+  sl[ty][tx] = l;
+  __syncthreads();
+  if (ty == 0 && n < N) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += sl[i][tx];
+    loss[n] = j >= 0 ? sum * factor : 0.f;
+    if (j >= 0) lse_out[n] = lse;
+  }
+}
+
+// scalars[0] = sum or mean of the row losses, scalars[1] = 1 / counted rows (0 when there are none); one block,
+// a fixed order, sums in 64 bits
+__global__ void __launch_bounds__(1024)
+    reduce_loss_kernel(const float* __restrict__ loss, int N, const int* __restrict__ count, int mean,
+                       float* __restrict__ scalars) {
+  __shared__ double part[32];
+  double s = 0.0;
+  for (int n = threadIdx.x; n < N; n += 1024) s += loss[n];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = part[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) {
+      const int c = *count;
+      scalars[0] = (float)(mean ? (c > 0 ? s / c : 0.0) : s);
+      scalars[1] = c > 0 ? 1.f / (float)c : 0.f;
+    }
+  }
+}
+
+// dx of every row from the packed slabs: their sum in slab order, times the gradient's factor; zero where the row
+// is not counted
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads)
+    finish_dx_kernel(const float* __restrict__ slab, long long slab_stride, int slabs, long long ld,
+                     const int* __restrict__ pos, T* __restrict__ dx, long long lddx, int N, int D, float alpha,
+                     const float* __restrict__ scale, const float* __restrict__ scale2) {
+  const int per_row = (D + VEC - 1) / VEC;
+  const long long total = (long long)N * per_row;
+  float a = alpha;
+  if (scale != nullptr) a *= *scale;
+  if (scale2 != nullptr) a *= *scale2;
+  for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
+    const int n = (int)(i / per_row);
+    const int d0 = (int)(i - (long long)n * per_row) * VEC;
+    const int j = pos[n];
+    float v[VEC] = {};
+    if (j >= 0) {
+      const float* s = slab + (long long)j * ld + d0;
+      for (int k = 0; k < slabs; ++k, s += slab_stride) {
+        if constexpr (VEC == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(s);
+          v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+        } else {
+          v[0] += *s;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] *= a;
+    }
+    T* o = dx + n * lddx + d0;
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (VEC == 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+      else *o = v[0];
+    } else {
+      if constexpr (VEC == 4) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      else *o = __float2bfloat16_rn(v[0]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- embedding
+template <typename T> PCB_DEVICE float to_f32(T v);
+template <> PCB_DEVICE float to_f32<float>(float v) { return v; }
+template <> PCB_DEVICE float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> PCB_DEVICE T from_f32(float v);
+template <> PCB_DEVICE float from_f32<float>(float v) { return v; }
+template <> PCB_DEVICE __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int VEC>
+PCB_DEVICE void load_vec(const T* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32<T>(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    static_assert(VEC % 4 == 0, "16-byte vectors");
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 f = reinterpret_cast<const float4*>(p)[i];
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+  } else if constexpr (VEC == 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
+    v[4] = bf16_lo(u.z); v[5] = bf16_hi(u.z); v[6] = bf16_lo(u.w); v[7] = bf16_hi(u.w);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
+  }
+}
+template <typename T, int VEC>
+PCB_DEVICE void store_vec(T* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else if constexpr (VEC == 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  }
+}
+
+// one vector of VEC columns per thread
+template <typename TW, typename TX, int VEC>
+__global__ void __launch_bounds__(kThreads)
+    lookup_kernel(const void* __restrict__ tok, int tok64, const TW* __restrict__ w, long long ldw, TX* __restrict__ x,
+                  long long total, int per_row, int V, int D, float scale) {
+  const long long i = blockIdx.x * (long long)kThreads + threadIdx.x;
+  if (i >= total) return;
+  const long long n = i / per_row;
+  const int d0 = (int)(i - n * per_row) * VEC;
+  const long long t = load_id(tok, tok64, n);
+  float v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = 0.f;
+  if (t >= 0 && t < V) {
+    load_vec<TW, VEC>(w + t * ldw + d0, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] *= scale;
+  }
+  store_vec<TX, VEC>(x + n * D + d0, v);
+}
+
+// ---- stable sort of (token, place) by token: least significant digit first, 8 bits a pass.  Tokens outside
+// [0, V) take the key V and end up behind all others.
+constexpr int kSortTile = 2048;   // keys per block
+constexpr int kSortWarps = kThreads / 32;
+constexpr int kPerWarp = kSortTile / kSortWarps;
+
+PCB_DEVICE uint32_t sort_key(const void* tok, int tok64, const uint32_t* keys, int n, int V) {
+  if (keys != nullptr) return keys[n];
+  const long long t = load_id(tok, tok64, n);
+  return t >= 0 && t < V ? (uint32_t)t : (uint32_t)V;
+}
+
+__global__ void __launch_bounds__(kThreads)
+    sort_hist_kernel(const void* tok, int tok64, const uint32_t* __restrict__ keys, int N, int V, int shift,
+                     uint32_t* __restrict__ hist, int blocks) {
+  __shared__ uint32_t h[256];
+  h[threadIdx.x] = 0;
+  __syncthreads();
+  const int t0 = blockIdx.x * kSortTile;
+  for (int i = threadIdx.x; i < kSortTile && t0 + i < N; i += kThreads)
+    atomicAdd(&h[(sort_key(tok, tok64, keys, t0 + i, V) >> shift) & 255], 1u);   // counts: any order gives the same
+  __syncthreads();
+  hist[(long long)threadIdx.x * blocks + blockIdx.x] = h[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* __restrict__ hist, int total) {
+  __shared__ int sums[32];
+  int base = 0;
+  for (int t0 = 0; t0 < total; t0 += 1024) {
+    const int i = t0 + threadIdx.x;
+    const int v = i < total ? (int)hist[i] : 0;
+    int sum;
+    const int before = block_scan(v, sums, &sum);
+    if (i < total) hist[i] = base + before;
+    base += sum;
+  }
+}
+
+// A warp owns kPerWarp consecutive keys.  Digit counts per warp give each warp its first place of every digit;
+// lanes with the same digit take places in lane order.
+__global__ void __launch_bounds__(kThreads)
+    sort_scatter_kernel(const void* tok, int tok64, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx,
+                        int N, int V, int shift, const uint32_t* __restrict__ hist, int blocks,
+                        uint32_t* __restrict__ keys_out, uint32_t* __restrict__ idx_out) {
+  __shared__ uint32_t place[kSortWarps][256];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int i = lane; i < 256; i += 32) place[w][i] = 0;
+  __syncwarp();
+  const int t0 = blockIdx.x * kSortTile + w * kPerWarp;
+  for (int i = 0; i < kPerWarp; i += 32) {
+    const int n = t0 + i + lane;
+    if (n < N) atomicAdd(&place[w][(sort_key(tok, tok64, keys, n, V) >> shift) & 255], 1u);
+  }
+  __syncthreads();
+  {
+    uint32_t p = hist[(long long)threadIdx.x * blocks + blockIdx.x];
+#pragma unroll
+    for (int i = 0; i < kSortWarps; ++i) {
+      const uint32_t c = place[i][threadIdx.x];
+      place[i][threadIdx.x] = p;
+      p += c;
+    }
+  }
+  __syncthreads();
+  for (int i = 0; i < kPerWarp; i += 32) {
+    const int n = t0 + i + lane;
+    const bool in = n < N;
+    const uint32_t key = in ? sort_key(tok, tok64, keys, n, V) : 0u;
+    const uint32_t digit = in ? (key >> shift) & 255 : 256u;   // lanes past the end match one another only
+    const uint32_t same = __match_any_sync(0xffffffffu, digit);
+    const uint32_t rank = __popc(same & ((1u << lane) - 1));
+    uint32_t at = 0;
+    if (in) at = place[w][digit] + rank;
+    __syncwarp();
+    if (in && rank == 0) place[w][digit] += __popc(same);
+    __syncwarp();
+    if (in) {
+      keys_out[at] = key;
+      idx_out[at] = idx != nullptr ? idx[n] : (uint32_t)n;
+    }
+  }
+}
+
+// ---- sums over runs of equal tokens.  A block owns kChunk consecutive sorted entries and a slice of the columns;
+// a thread keeps VEC columns in registers over the run.  A run inside the chunk is written at once; the part of
+// a run that crosses a chunk's edge goes to a partial row, and join_kernel adds those in order.
+constexpr int kChunk = 32;
+
+template <typename TX, typename TW, int VEC>
+PCB_DEVICE void emit(TW* dw, uint32_t id, int D, int d0, float (&a)[VEC], float scale, int add) {
+  TW* o = dw + (long long)id * D + d0;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) a[e] *= scale;
+  if (add) {
+    float p[VEC];
+    load_vec<TW, VEC>(o, p);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) a[e] += p[e];
+  }
+  store_vec<TW, VEC>(o, a);
+}
+
+template <typename TX, typename TW, int VEC>
+__global__ void __launch_bounds__(kThreads)
+    run_sums_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx, const TX* __restrict__ dx,
+                    long long lddx, TW* __restrict__ dw, float* __restrict__ partial, int N, int V, int D, float scale,
+                    int add) {
+  __shared__ uint32_t s_key[kChunk + 2], s_idx[kChunk];
+  const int c0 = blockIdx.x * kChunk, cnt = min(kChunk, N - c0);
+  for (int i = threadIdx.x; i < cnt + 2; i += blockDim.x) {   // with both neighbours
+    const long long n = (long long)c0 + i - 1;
+    s_key[i] = n >= 0 && n < N ? keys[n] : 0xffffffffu;
+  }
+  for (int i = threadIdx.x; i < cnt; i += blockDim.x) s_idx[i] = idx[c0 + i];
+  __syncthreads();
+  const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (d0 >= D) return;
+  float acc[VEC] = {};
+  bool begun_before = s_key[0] == s_key[1];
+  constexpr int U = 8;
+  for (int i0 = 0; i0 < cnt; i0 += U) {
+    float r[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u < cnt && s_key[i0 + u + 1] < (uint32_t)V) load_vec<TX, VEC>(dx + s_idx[i0 + u] * lddx + d0, r[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      if (i >= cnt) break;
+      const uint32_t id = s_key[i + 1];
+      if (id >= (uint32_t)V) return;   // only tokens without a row follow
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += r[u][e];
+      const bool run_ends = s_key[i + 2] != id;
+      if (run_ends || i == cnt - 1) {
+        if (run_ends && !begun_before) {
+          emit<TX, TW, VEC>(dw, id, D, d0, acc, scale, add);
+        } else {
+          float* p = partial + ((long long)blockIdx.x * 2 + (begun_before ? 0 : 1)) * D + d0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+        begun_before = false;
+      }
+    }
+  }
+}
+
+// The runs that begin in this block's chunk and go on behind it: their parts in order.
+template <typename TW, int VEC>
+__global__ void __launch_bounds__(kThreads)
+    join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, TW* __restrict__ dw, int N, int V,
+                int D, float scale, int add) {
+  const int c0 = blockIdx.x * kChunk;
+  const long long last = (long long)c0 + kChunk - 1;
+  if (last + 1 >= N) return;
+  const uint32_t id = keys[last];
+  if (id >= (uint32_t)V || keys[last + 1] != id) return;
+  if (c0 > 0 && keys[c0 - 1] == id) return;   // begun in an earlier chunk
+  const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (d0 >= D) return;
+  float acc[VEC];
+  const float* p = partial + ((long long)blockIdx.x * 2 + 1) * D + d0;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = p[e];
+  for (int c = blockIdx.x + 1; (long long)c * kChunk < N && keys[(long long)c * kChunk] == id; ++c) {
+    p = partial + (long long)c * 2 * D + d0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] += p[e];
+  }
+  emit<float, TW, VEC>(dw, id, D, d0, acc, scale, add);
+}
+
+inline bool al(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline int launched() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
+
+}  // namespace vocab
+
+using namespace vocab;
+
+VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
+  VocabLayout l{};
+  long long at = 0;
+  auto take = [&](long long bytes) {
+    const long long o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  l.ldxc = (D + 7) / 8 * 8;
+  l.granules = 2 * ((V + 255) / 256);
+  l.xc = take((long long)N * l.ldxc * 2);
+  l.count = take(16);
+  l.row = take(4LL * N);
+  l.pos = take(4LL * N);
+  l.lse = take(4LL * N);
+  l.z = take(4LL * N * K);
+  l.ids = take(4LL * N * K);
+  if (distill) {
+    l.q = take(4LL * N * K);
+    l.lq = take(4LL * N * K);
+    l.len = take(4LL * N);
+    l.start = take(2LL * N * (l.granules + 1));
+  }
+  l.bytes = at;
+  return l;
+}
+
+static long long tiles_cost(long long tiles, int slots, long long kb) {
+  // waves of the persistent grid, each as long as its k-blocks and a fixed part for prologue and epilogue
+  return (tiles + slots - 1) / slots * (kb + 8);
+}
+
+void vocab_plan(int N, int V, int D, int want_piece, int num_sms, int* piece, int* splits) {
+  const long long all = (V + 255LL) / 256 * 256;
+  long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2LL * N) / 256 * 256;
+  p = std::max(256LL, std::min(p, all));
+  const long long pieces = (all + p - 1) / p;
+  p = (all / 256 + pieces - 1) / pieces * 256;   // pieces of one size
+  *piece = (int)p;
+  const int bn = D >= 256 ? 256 : 128;
+  const long long tiles = ((N + 255LL) / 256) * ((D + bn - 1) / bn), kb = (std::min<long long>(p, V) + 63) / 64;
+  int best = 1;
+  long long cost = -1;
+  for (int s = 1; s <= 16 && kb / s >= 4; ++s) {
+    const long long c = tiles_cost(tiles * s, num_sms / 2, (kb + s - 1) / s);
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  const long long kbps = (kb + best - 1) / best;
+  *splits = (int)((kb + kbps - 1) / kbps);
+}
+
+}  // namespace pcb
+
+using namespace pcb;
+using namespace pcb::vocab;
+
+int pcb_vocab_pad_rows(const void* src, long long ld, void* dst, long long ldd, int rows, int D, cudaStream_t s) {
+  const long long total = rows * ldd;
+  const int grid = (int)std::min<long long>((total + 255) / 256, 148 * 16);
+  pad_rows_kernel<<<grid, 256, 0, s>>>((const __nv_bfloat16*)src, ld, (__nv_bfloat16*)dst, ldd, total, D);
+  return launched();
+}
+
+static char* at(void* base, long long off) { return (char*)base + off; }
+
+int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s) {
+  const bool distill = a.tgt == nullptr;
+  if (a.N < 1 || a.V < 1 || a.D < 1 || a.K < 1 || a.K > kMaxK) return -1;
+  const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, distill);
+  int* count = (int*)at(saved, l.count);
+  int *row = (int*)at(saved, l.row), *pos = (int*)at(saved, l.pos), *ids = (int*)at(saved, l.ids);
+  float *lse = (float*)at(saved, l.lse), *z = (float*)at(saved, l.z);
+  float *q = distill ? (float*)at(saved, l.q) : nullptr, *lq = distill ? (float*)at(saved, l.lq) : nullptr;
+  int* len = distill ? (int*)at(saved, l.len) : nullptr;
+  unsigned short* start = distill ? (unsigned short*)at(saved, l.start) : nullptr;
+  __nv_bfloat16* xc = (__nv_bfloat16*)at(saved, l.xc);
+  const float T = distill ? a.temperature : 1.f;
+  const float c = 1.4426950408889634f / T;
+  if (distill) {
+    sort_targets_kernel<<<(a.N + 7) / 8, kThreads, 0, s>>>(a.ids, a.ids64, a.ld_ids, a.logits, a.logits_bf16,
+                                                         a.ld_logits, a.N, a.V, a.K, c, ids, q, lq, len, start,
+                                                         l.granules);
+    if (launched()) return -3;
+  }
+  const int blocks = std::max(1, std::min(2 * num_sms, (a.N + 7) / 8));
+  const int R = (a.N + blocks - 1) / blocks;
+  const int vec = a.D % 8 == 0 && a.ldx % 8 == 0 && al(a.x, 16);
+  pack_rows_kernel<<<blocks, kThreads, 0, s>>>(a.tgt, a.tgt64, a.ignore, len, a.V, (const __nv_bfloat16*)a.x, a.ldx,
+                                               a.N, a.D, R, vec, xc, l.ldxc, row, pos, distill ? nullptr : ids, count);
+  if (launched()) return -3;
+  GemmArgs g{};
+  g.M = a.N;
+  g.N = a.V;
+  g.K = a.D;
+  g.alpha = 1.f;
+  g.vh.count = count;
+  g.vh.row = row;
+  g.vh.c = c;
+  g.vh.part = (float2*)part;
+  g.vh.ld_part = a.N;
+  g.vh.ids = ids;
+  g.vh.z = z;
+  g.vh.K = a.K;
+  g.vh.start = start;
+  g.vh.ld_start = a.N;
+  int rc = pcb_gemm_pair_launch(xc, 0, l.ldxc, a.w, 0, a.ldw, EPI_VH_STAT, g, 256, 1, num_sms, s);
+  if (rc) return rc;
+  row_loss_kernel<<<(a.N + 31) / 32, 256, 0, s>>>((const float2*)part, l.granules, a.N, pos, z, q, lq, len, a.N, a.K, c,
+                                                 0.6931471805599453f * T * T, lse, a.loss);
+  if (launched()) return -3;
+  reduce_loss_kernel<<<1, 1024, 0, s>>>(a.loss, a.N, count, mean, a.scalars);
+  return launched();
+}
+
+int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
+  const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, a.distill != 0);
+  void* sv = const_cast<void*>(a.saved);
+  const int* count = (const int*)at(sv, l.count);
+  const int *row = (const int*)at(sv, l.row), *pos = (const int*)at(sv, l.pos);
+  const __nv_bfloat16* xc = (const __nv_bfloat16*)at(sv, l.xc);
+  const float* inv = a.mean ? a.scalars + 1 : nullptr;
+  const float T = a.distill ? a.temperature : 1.f;
+  const int bnd = a.D >= 256 ? 256 : 128;
+  for (int v0 = 0; v0 < a.V; v0 += a.piece) {
+    const int cols = std::min(a.piece, a.V - v0);
+    const __nv_bfloat16* w = (const __nv_bfloat16*)a.w + (long long)v0 * a.ldw;
+    GemmArgs g{};
+    g.M = a.N;
+    g.N = cols;
+    g.K = a.D;
+    g.alpha = 1.f;
+    g.C = a.g;
+    g.ldc = a.piece;
+    g.vh.count = count;
+    g.vh.row = row;
+    g.vh.c = 1.4426950408889634f / T;
+    g.vh.v0 = v0;
+    g.vh.lse = (const float*)at(sv, l.lse);
+    g.vh.ids = (const int*)at(sv, l.ids);
+    g.vh.K = a.K;
+    if (a.distill) {
+      g.vh.q = (const float*)at(sv, l.q);
+      g.vh.start = (const unsigned short*)at(sv, l.start);
+      g.vh.ld_start = a.N;
+    }
+    int rc = pcb_gemm_pair_launch(xc, 0, l.ldxc, w, 0, a.ldw, EPI_VH_GRAD, g, 256, 1, num_sms, s);
+    if (rc) return rc;
+    if (a.dw != nullptr) {
+      GemmArgs d{};
+      d.M = cols;
+      d.N = a.D;
+      d.K = a.N;
+      d.alpha = a.gout * T;
+      d.C = (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
+      d.ldc = a.lddw;
+      d.vh.count = count;
+      d.vh.scale = inv;
+      d.vh.scale2 = a.gout_dev;
+      d.vh.add = a.dw_add;
+      d.vh.out_f32 = a.dw_f32;
+      rc = pcb_gemm_pair_launch(a.g, 1, a.piece, xc, 1, l.ldxc, EPI_VH_DW, d, bnd, 1, num_sms, s);
+      if (rc) return rc;
+    }
+    if (a.dx != nullptr) {
+      GemmArgs d{};
+      d.M = a.N;
+      d.N = a.D;
+      d.K = cols;
+      d.alpha = 1.f;
+      d.C = a.slab;
+      d.ldc = a.ld_slab;
+      d.vh.count = count;
+      d.vh.add = v0 > 0;
+      d.vh.slab = (long long)a.N * a.ld_slab;
+      // a last piece with fewer k-blocks than the others could leave a split without any: it runs unsplit into slab 0
+      const int kb = (cols + 63) / 64, kbps = (kb + a.splits - 1) / a.splits;
+      const int splits = (kb + kbps - 1) / kbps;
+      rc = pcb_gemm_pair_launch(a.g, 0, a.piece, w, 1, a.ldw, EPI_VH_DX, d, bnd, splits, num_sms, s);
+      if (rc) return rc;
+    }
+  }
+  if (a.dx == nullptr) return 0;
+  const bool v4 = a.D % 4 == 0 && a.lddx % 4 == 0 && al(a.dx, a.dx_f32 ? 16 : 8);
+  const long long total = (long long)a.N * (v4 ? a.D / 4 : a.D);
+  const int grid = (int)std::min<long long>((total + kThreads - 1) / kThreads, num_sms * 16);
+  const long long stride = (long long)a.N * a.ld_slab;
+  auto go = [&](auto* dx, auto vec) {
+    using T2 = std::remove_pointer_t<decltype(dx)>;
+    finish_dx_kernel<T2, decltype(vec)::value><<<grid, kThreads, 0, s>>>(a.slab, stride, a.splits, a.ld_slab, pos, dx,
+                                                                         a.lddx, a.N, a.D, a.gout * T, inv, a.gout_dev);
+  };
+  if (a.dx_f32) {
+    if (v4) go((float*)a.dx, std::integral_constant<int, 4>{});
+    else go((float*)a.dx, std::integral_constant<int, 1>{});
+  } else {
+    if (v4) go((__nv_bfloat16*)a.dx, std::integral_constant<int, 4>{});
+    else go((__nv_bfloat16*)a.dx, std::integral_constant<int, 1>{});
+  }
+  return launched();
+}
+
+template <typename F>
+static void by_type(int w_bf16, int x_bf16, F f) {
+  if (w_bf16) {
+    if (x_bf16) f((__nv_bfloat16*)nullptr, (__nv_bfloat16*)nullptr);
+    else f((__nv_bfloat16*)nullptr, (float*)nullptr);
+  } else {
+    if (x_bf16) f((float*)nullptr, (__nv_bfloat16*)nullptr);
+    else f((float*)nullptr, (float*)nullptr);
+  }
+}
+
+int pcb_vocab_embed_fwd(const void* tok, int tok64, const void* w, int w_bf16, long long ldw, void* x, int x_bf16,
+                        int N, int V, int D, float scale, cudaStream_t s) {
+  const bool vec = D % 4 == 0 && ldw % 4 == 0 && al(w, w_bf16 ? 8 : 16) && al(x, x_bf16 ? 8 : 16);
+  const int per_row = vec ? D / 4 : D;
+  const long long total = (long long)N * per_row, blocks = (total + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffLL) return -1;
+  by_type(w_bf16, x_bf16, [&](auto* tw, auto* tx) {
+    using TW = std::remove_pointer_t<decltype(tw)>;
+    using TX = std::remove_pointer_t<decltype(tx)>;
+    if (vec)
+      lookup_kernel<TW, TX, 4><<<(unsigned)blocks, kThreads, 0, s>>>(tok, tok64, (const TW*)w, ldw, (TX*)x, total, per_row,
+                                                                    V, D, scale);
+    else
+      lookup_kernel<TW, TX, 1><<<(unsigned)blocks, kThreads, 0, s>>>(tok, tok64, (const TW*)w, ldw, (TX*)x, total, per_row,
+                                                                    V, D, scale);
+  });
+  return launched();
+}
+
+static long long up256(long long b) { return (b + 255) / 256 * 256; }
+
+long long pcb_vocab_embed_bwd_bytes(int N, int V, int D) {
+  const long long blocks = (N + kSortTile - 1) / kSortTile, chunks = (N + kChunk - 1) / kChunk;
+  return 4 * up256(4LL * N) + up256(4LL * 256 * blocks) + up256(8LL * chunks * D);
+}
+
+int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16, long long lddx, void* dw, int dw_bf16,
+                        int N, int V, int D, float scale, int add, void* ws, int num_sms, cudaStream_t s) {
+  const int blocks = (N + kSortTile - 1) / kSortTile, chunks = (N + kChunk - 1) / kChunk;
+  if (blocks > (1 << 22)) return -1;   // 256 counts a block are scanned as ints
+  char* p = (char*)ws;
+  uint32_t* buf[4];
+  for (auto& b : buf) {
+    b = (uint32_t*)p;
+    p += up256(4LL * N);
+  }
+  uint32_t* hist = (uint32_t*)p;
+  p += up256(4LL * 256 * blocks);
+  float* partial = (float*)p;
+  if (!add && cudaMemsetAsync(dw, 0, (size_t)V * D * (dw_bf16 ? 2 : 4), s) != cudaSuccess) return -3;
+  int bits = 1;
+  while (bits < 32 && (V >> bits) != 0) ++bits;   // keys run up to V
+  const uint32_t *keys = nullptr, *idx = nullptr;
+  int side = 0;
+  for (int shift = 0; shift < bits; shift += 8) {
+    sort_hist_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, N, V, shift, hist, blocks);
+    sort_scan_kernel<<<1, 1024, 0, s>>>(hist, 256 * blocks);
+    sort_scatter_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, idx, N, V, shift, hist, blocks, buf[2 * side],
+                                                    buf[2 * side + 1]);
+    if (launched()) return -3;
+    keys = buf[2 * side];
+    idx = buf[2 * side + 1];
+    side ^= 1;
+  }
+  const bool vec = D % 4 == 0 && lddx % 4 == 0 && al(dx, dx_bf16 ? 8 : 16) && al(dw, dw_bf16 ? 8 : 16);
+  const int cols = vec ? D / 4 : D;
+  const int threads = std::min(kThreads, (cols + 31) / 32 * 32);
+  const dim3 grid(chunks, (cols + threads - 1) / threads);
+  by_type(dw_bf16, dx_bf16, [&](auto* tw, auto* tx) {
+    using TW = std::remove_pointer_t<decltype(tw)>;
+    using TX = std::remove_pointer_t<decltype(tx)>;
+    auto go = [&](auto v) {
+      constexpr int VEC = decltype(v)::value;
+      run_sums_kernel<TX, TW, VEC><<<grid, threads, 0, s>>>(keys, idx, (const TX*)dx, lddx, (TW*)dw, partial, N, V, D,
+                                                            scale, add);
+      join_kernel<TW, VEC><<<grid, threads, 0, s>>>(keys, partial, (TW*)dw, N, V, D, scale, add);
+    };
+    if (vec) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1>{});
+  });
+  return launched();
+}

@@ -1,0 +1,92 @@
+// Host-safe API of the operators at the two ends of a decoder (csrc/vocab.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+namespace pcb {
+
+// Loss of the vocabulary head: softmax cross entropy, or distillation from a list of teacher logits per row.
+struct VocabHeadArgs {
+  const void* x;        // [N, D] bf16, row stride ldx
+  long long ldx;
+  const void* w;        // [V, D] bf16, row stride ldw (a multiple of 8, 16-byte aligned base)
+  long long ldw;
+  int N, V, D;
+  // cross entropy
+  const void* tgt;      // [N] int32 or int64 (nullptr: distillation)
+  int tgt64;
+  long long ignore;     // rows with this target are not counted; neither are targets outside [0, V)
+  // distillation
+  const void* ids;      // [N, K] int32 or int64; entries outside [0, V) are absent
+  int ids64;
+  long long ld_ids;
+  const void* logits;   // [N, K] fp32 or bf16; -inf entries are absent
+  int logits_bf16;
+  long long ld_logits;
+  int K;                // entries per row (1 for cross entropy)
+  float temperature;
+  float* loss;          // [N] row losses
+  float* scalars;       // [2]: sum or mean of the row losses, 1 / counted rows
+};
+
+// Where the forward keeps what the backward reads: byte offsets into one buffer.
+struct VocabLayout {
+  long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
+  long long ldxc;
+  long long count;   // int [4]: counted rows
+  long long row;     // int [N]: batch place of each packed row
+  long long pos;     // int [N]: packed place of each row, -1 where it is not counted
+  long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature
+  long long z;       // float [N, K]: logits at the target ids
+  long long ids;     // int [N, K] ascending ids
+  long long q;       // float [N, K] weights (distillation)
+  long long lq;      // float [N, K] log2 of the weights (distillation)
+  long long len;     // int [N] entries present (distillation)
+  long long start;   // unsigned short [granules + 1, N] (distillation)
+  int granules;      // 128-column halves of the 256-column tiles
+  long long bytes;
+};
+VocabLayout vocab_layout(int N, int V, int D, int K, bool distill);
+
+struct VocabGradArgs {
+  const void* w;
+  long long ldw;
+  int N, V, D, K;
+  int distill;
+  float temperature;
+  const void* saved;     // buffer of the forward
+  const float* scalars;
+  float gout;            // gradient of the loss: gout * *gout_dev (nullptr: 1) / (counted rows, for the mean)
+  const float* gout_dev;
+  int mean;
+  void* dx;              // [N, D] bf16 or fp32, row stride lddx (nullptr: not wanted)
+  long long lddx;
+  int dx_f32;
+  void* dw;              // [V, D] bf16 or fp32, row stride lddw (nullptr: not wanted)
+  long long lddw;
+  int dw_f32;
+  int dw_add;
+  int piece;             // columns per piece (a multiple of 256)
+  int splits;            // K splits of dx
+  void* g;               // [N, piece] bf16 workspace
+  float* slab;           // [splits, N, ld_slab] fp32 workspace
+  long long ld_slab;
+};
+
+// columns of the vocabulary handled at a time, and K splits of the dx product
+void vocab_plan(int N, int V, int D, int want_piece, int num_sms, int* piece, int* splits);
+
+}  // namespace pcb
+
+int pcb_vocab_pad_rows(const void* src, long long ld, void* dst, long long ldd, int rows, int D, cudaStream_t s);
+// `part`: [granules, N] float2 workspace
+int pcb_vocab_fwd(const pcb::VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s);
+int pcb_vocab_bwd(const pcb::VocabGradArgs& a, int num_sms, cudaStream_t s);
+
+// x[n] = scale * w[tok[n]]; rows of tokens outside [0, V) are zero
+int pcb_vocab_embed_fwd(const void* tok, int tok64, const void* w, int w_bf16, long long ldw, void* x, int x_bf16,
+                        int N, int V, int D, float scale, cudaStream_t s);
+// bytes of workspace of the embedding gradient
+long long pcb_vocab_embed_bwd_bytes(int N, int V, int D);
+// dw[v] (+)= scale * sum of dx[n] over tok[n] == v in ascending n
+int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16, long long lddx, void* dw, int dw_bf16,
+                        int N, int V, int D, float scale, int add, void* ws, int num_sms, cudaStream_t s);
