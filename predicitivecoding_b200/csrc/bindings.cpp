@@ -9,7 +9,9 @@
 #include <torch/extension.h>
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <atomic>
+#include <limits>
 #include <stdexcept>
 
 // Argument and launch checks raise std::invalid_argument (pybind11 turns it into ValueError).
@@ -363,136 +365,261 @@ int is_bf16(const at::Tensor& t, const char* name) {
   return t.scalar_type() == at::kBFloat16 ? 1 : 0;
 }
 
-// Loss of the vocabulary head.  x [N, D], w [V, D] bf16; either tgt [N] or ids, logits [N, K].  Allocates and returns
-// (row losses [N], scalars [2], the forward's buffer, w as the GEMMs read it: w itself, or a copy with 16-byte rows).
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> vocab_fwd(
-    const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& tgt, int64_t ignore,
-    const c10::optional<at::Tensor>& ids, const c10::optional<at::Tensor>& logits, double temperature, bool mean) {
-  req(x, at::kBFloat16, "x");
-  req(w, at::kBFloat16, "w");
+bool same_lead(const at::Tensor& t, const at::Tensor& x, int64_t tail) {   // t is [*x.shape[:-1]] plus `tail` dimensions
+  if (t.dim() != x.dim() - 1 + tail) return false;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i)
+    if (t.size(i) != x.size(i)) return false;
+  return true;
+}
+// [..., n] as [rows, n] with a contiguous inner dimension
+at::Tensor as_rows(const at::Tensor& t) {
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.stride(1) == 1 || r.size(1) <= 1 ? r : r.contiguous();
+}
+long long rows_apart(const at::Tensor& t) { return t.stride(0); }
+at::Tensor flat(const at::Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+
+// What a loss of the vocabulary head keeps for its gradients.
+struct HeadState {
+  at::Tensor saved, scalars, w;
+  std::vector<int64_t> lead;
+  int64_t N, V, D, K;
+  bool distill, mean, none;
+  double temperature;
+};
+
+// Loss of the vocabulary head: x [..., D], w [V, D] bf16; either targets [...] or ids, logits [..., K].  Allocates the
+// loss (a scalar, or one per row), what the gradients need, and w as the GEMMs read it when its rows are not 16-byte
+// aligned.
+std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x, const at::Tensor& w,
+                                          const at::Tensor* tgt, int64_t ignore, const at::Tensor* ids,
+                                          const at::Tensor* logits, double temperature, const std::string& reduction) {
+  PCB_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16, what, ": x must be a bf16 CUDA tensor");
+  PCB_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16, what, ": w must be a bf16 CUDA tensor");
+  PCB_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.numel() > 0 &&
+                (w.stride(1) == 1 || w.size(1) == 1),
+            what, ": x must be [..., D] and w [V, D] with a contiguous inner dimension");
+  PCB_CHECK(reduction == "mean" || reduction == "sum" || reduction == "none", what, ": reduction must be mean, sum or none");
+  PCB_CHECK(w.device() == x.device() && (!tgt || tgt->device() == x.device()) &&
+                (!ids || (ids->device() == x.device() && logits->device() == x.device())),
+            what, ": all operands must be on one device");
+  HeadState st{};
+  st.lead.assign(x.sizes().begin(), x.sizes().end() - 1);
+  st.mean = reduction == "mean";
+  st.none = reduction == "none";
+  st.distill = tgt == nullptr;
+  st.D = x.size(-1);
+  st.N = x.numel() / st.D;
+  st.V = w.size(0);
+  st.K = ids ? ids->size(-1) : 1;
+  st.temperature = temperature;
+  PCB_CHECK(st.N < (1LL << 30) && st.V < (1LL << 30) && st.D < (1LL << 24), what, ": an operand is too large");
+  st.w = w;
+  const at::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  if (st.N == 0) return {st.none ? at::zeros(st.lead, f32) : at::zeros({}, f32), st};
   pcb::VocabHeadArgs a{};
-  a.ldx = row_stride(x, "x");
-  a.ldw = row_stride(w, "w");
-  a.N = x.size(0);
-  a.D = x.size(1);
-  a.V = w.size(0);
-  PCB_CHECK(w.size(1) == a.D, "vocab_fwd: w must be [V, D]");
-  PCB_CHECK(a.N >= 1 && a.V >= 1 && a.D >= 1, "vocab_fwd: empty operand");
-  a.K = 1;
-  a.temperature = 1.f;
+  const at::Tensor x2 = as_rows(x);
+  at::Tensor t1, i2, l2;
+  a.x = x2.data_ptr();
+  a.ldx = rows_apart(x2);
+  a.N = st.N;
+  a.V = st.V;
+  a.D = st.D;
+  a.K = st.K;
+  a.temperature = (float)temperature;
   if (tgt) {
-    a.tgt64 = is64(*tgt, "targets");
-    PCB_CHECK(tgt->is_contiguous() && tgt->numel() == a.N, "vocab_fwd: targets must be [N] contiguous");
-    a.tgt = tgt->data_ptr();
+    t1 = flat(*tgt);
+    a.tgt64 = t1.scalar_type() == at::kLong;
+    a.tgt = t1.data_ptr();
     a.ignore = ignore;
   } else {
-    PCB_CHECK(ids && logits && ids->dim() == 2 && ids->sizes() == logits->sizes() && ids->size(0) == a.N,
-              "vocab_fwd: ids and logits must be [N, K]");
-    a.ids64 = is64(*ids, "ids");
-    a.logits_bf16 = is_bf16(*logits, "logits");
-    a.ld_ids = row_stride(*ids, "ids");
-    a.ld_logits = row_stride(*logits, "logits");
-    a.ids = ids->data_ptr();
-    a.logits = logits->data_ptr();
-    a.K = ids->size(1);
-    a.temperature = (float)temperature;
+    i2 = as_rows(*ids);
+    l2 = as_rows(*logits);
+    a.ids64 = i2.scalar_type() == at::kLong;
+    a.logits_bf16 = l2.scalar_type() == at::kBFloat16;
+    a.ld_ids = rows_apart(i2);
+    a.ld_logits = rows_apart(l2);
+    a.ids = i2.data_ptr();
+    a.logits = l2.data_ptr();
   }
-  const at::cuda::CUDAGuard guard(x.device());
-  at::Tensor wr = w;
+  a.ldw = rows_apart(w);
   if (a.ldw % 8 != 0 || a.ldw < a.D || (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) != 0) {
-    const int64_t ld = (a.D + 7) / 8 * 8;
-    wr = at::empty({a.V, ld}, w.options());
-    check(pcb_vocab_pad_rows(w.data_ptr(), a.ldw, wr.data_ptr(), ld, a.V, a.D, cur_stream()), "vocab_pad_rows");
+    const int64_t ld = (st.D + 7) / 8 * 8;
+    st.w = at::empty({st.V, ld}, w.options());
+    check(pcb_vocab_pad_rows(w.data_ptr(), a.ldw, st.w.data_ptr(), ld, a.V, a.D, cur_stream()), "vocab_pad_rows");
     a.ldw = ld;
   }
-  a.x = x.data_ptr();
-  a.w = wr.data_ptr();
-  const pcb::VocabLayout l = pcb::vocab_layout(a.N, a.V, a.D, a.K, !tgt);
-  at::Tensor saved = at::empty({l.bytes}, x.options().dtype(at::kByte));
-  at::Tensor part = at::empty({(int64_t)l.granules * a.N * 2}, x.options().dtype(at::kFloat));
-  at::Tensor loss = at::empty({a.N}, x.options().dtype(at::kFloat));
-  at::Tensor scalars = at::empty({2}, x.options().dtype(at::kFloat));
-  a.loss = loss.data_ptr<float>();
-  a.scalars = scalars.data_ptr<float>();
-  check(pcb_vocab_fwd(a, saved.data_ptr(), part.data_ptr(), mean ? 1 : 0, num_sms(), cur_stream()), "vocab_fwd",
-        tgt ? 4 : 5);
-  return {loss, scalars, saved, wr};
+  a.w = st.w.data_ptr();
+  const pcb::VocabLayout l = pcb::vocab_layout(a.N, a.V, a.D, a.K, st.distill);
+  st.saved = at::empty({l.bytes}, x.options().dtype(at::kByte));
+  const int64_t pairs = 2LL * l.granules * a.N;
+  at::Tensor part = at::empty({pairs + (st.none ? 0 : st.N)}, f32);   // the row losses behind the pairs
+  at::Tensor loss;
+  if (st.none) {
+    loss = at::empty(st.lead, f32);
+    a.loss = loss.data_ptr<float>();
+  } else {
+    st.scalars = at::empty({2}, f32);
+    a.scalars = st.scalars.data_ptr<float>();
+    a.loss = part.data_ptr<float>() + pairs;
+    loss = st.scalars.select(0, 0);
+  }
+  check(pcb_vocab_fwd(a, st.saved.data_ptr(), part.data_ptr(), st.mean ? 1 : 0, num_sms(), cur_stream()), what,
+        st.distill ? 4 : 3);
+  return {loss, st};
 }
 
-// Gradients of vocab_fwd's loss into dx [N, D] and dw [V, D] (either may be absent).  Allocates its workspaces.
-void vocab_bwd(const at::Tensor& saved, const at::Tensor& scalars, const at::Tensor& w, int64_t N, int64_t V, int64_t D,
-               int64_t K, bool distill, double temperature, bool mean, double gout,
-               const c10::optional<at::Tensor>& gout_dev, const c10::optional<at::Tensor>& dx,
-               const c10::optional<at::Tensor>& dw, bool dw_add, int64_t piece) {
+std::pair<at::Tensor, HeadState> vocab_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
+                                              int64_t ignore, const std::string& reduction) {
+  is64(targets, "ce_fwd: targets");
+  PCB_CHECK(x.dim() >= 1 && same_lead(targets, x, 0), "ce_fwd: targets must have x's leading shape");
+  return head_fwd("ce_fwd", x, w, &targets, ignore, nullptr, nullptr, 1.0, reduction);
+}
+
+std::pair<at::Tensor, HeadState> vocab_distill_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ids,
+                                                   const at::Tensor& logits, double temperature,
+                                                   const std::string& reduction) {
+  is64(ids, "distill_fwd: ids");
+  is_bf16(logits, "distill_fwd: logits");
+  PCB_CHECK(x.dim() >= 1 && same_lead(ids, x, 1) && ids.sizes() == logits.sizes(),
+            "distill_fwd: ids and logits must be [*x.shape[:-1], K]");
+  PCB_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= pcb::kVocabMaxEntries, "distill_fwd: between 1 and ",
+            pcb::kVocabMaxEntries, " entries per row");
+  PCB_CHECK(temperature > 0 && temperature < std::numeric_limits<float>::infinity(),
+            "distill_fwd: temperature must be positive and finite");
+  return head_fwd("distill_fwd", x, w, nullptr, -1, &ids, &logits, temperature, reduction);
+}
+
+// Gradients of a mean or summed loss, into dx [..., D] and dw [V, D] where given, else into new bf16 tensors.  Allocates
+// its workspaces.
+std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
+    const HeadState& st, double gout, const c10::optional<at::Tensor>& gout_dev, c10::optional<at::Tensor> dx,
+    c10::optional<at::Tensor> dw, bool need_dx, bool need_dw, bool accumulate, int64_t piece) {
+  PCB_CHECK(!st.none, "head_bwd: the gradient is of a mean or summed loss");
+  PCB_CHECK(!accumulate || dw, "head_bwd: accumulate needs dw");
+  PCB_CHECK(piece >= 0, "head_bwd: piece must not be negative");
   pcb::VocabGradArgs a{};
-  a.w = w.data_ptr();
-  a.ldw = row_stride(w, "w");
-  a.N = N;
-  a.V = V;
-  a.D = D;
-  a.K = K;
-  a.distill = distill;
-  a.temperature = (float)temperature;
-  PCB_CHECK(saved.numel() == pcb::vocab_layout(N, V, D, K, distill).bytes, "vocab_bwd: saved is of another loss");
-  a.saved = saved.data_ptr();
-  a.scalars = scalars.data_ptr<float>();
-  a.gout = (float)gout;
-  if (gout_dev) {
-    req(*gout_dev, at::kFloat, "gout");
-    PCB_CHECK(gout_dev->numel() == 1, "vocab_bwd: gout must hold one value");
-    a.gout_dev = gout_dev->data_ptr<float>();
-  }
-  a.mean = mean;
+  const auto dev = st.w.device();
   if (dx) {
-    a.dx_f32 = !is_bf16(*dx, "dx");
-    PCB_CHECK(dx->dim() == 2 && dx->size(0) == N && dx->size(1) == D, "vocab_bwd: dx must be [N, D]");
-    a.dx = dx->data_ptr();
-    a.lddx = row_stride(*dx, "dx");
+    a.dx_f32 = !is_bf16(*dx, "head_bwd: dx");
+    PCB_CHECK(dx->device() == dev && dx->dim() == (int64_t)st.lead.size() + 1 && dx->size(-1) == st.D &&
+                  std::equal(st.lead.begin(), st.lead.end(), dx->sizes().begin()) &&
+                  (dx->is_contiguous() || (dx->dim() == 2 && dx->stride(1) == 1 && dx->stride(0) >= st.D)),
+              "head_bwd: dx must be [*x.shape] on w's device, contiguous (or, as a matrix, with contiguous rows)");
   }
   if (dw) {
-    a.dw_f32 = !is_bf16(*dw, "dw");
-    PCB_CHECK(dw->dim() == 2 && dw->size(0) == V && dw->size(1) == D, "vocab_bwd: dw must be [V, D]");
-    a.dw = dw->data_ptr();
-    a.lddw = row_stride(*dw, "dw");
+    a.dw_f32 = !is_bf16(*dw, "head_bwd: dw");
+    PCB_CHECK(dw->device() == dev && dw->dim() == 2 && dw->size(0) == st.V && dw->size(1) == st.D &&
+                  (dw->is_contiguous() || (dw->stride(1) == 1 && dw->stride(0) >= st.D)),
+              "head_bwd: dw must be [V, D] on w's device with contiguous rows");
   }
-  a.dw_add = dw_add;
-  const at::cuda::CUDAGuard guard(w.device());
-  pcb::vocab_plan(N, V, D, (int)piece, num_sms(), &a.piece, &a.splits);
-  const int pieces = (V + a.piece - 1) / a.piece;
-  a.ld_slab = (D + 3) / 4 * 4;
-  at::Tensor g = at::empty({N * a.piece}, w.options().dtype(at::kBFloat16));
-  at::Tensor slab;
-  a.g = g.data_ptr();
+  if (gout_dev)
+    PCB_CHECK(gout_dev->scalar_type() == at::kFloat && gout_dev->numel() == 1 && gout_dev->device() == dev,
+              "head_bwd: gout must be a number or one fp32 value on w's device");
+  const at::cuda::CUDAGuard guard(dev);
+  if (!dx && need_dx) {
+    std::vector<int64_t> shape = st.lead;
+    shape.push_back(st.D);
+    dx = at::empty(shape, st.w.options());
+  }
+  if (!dw && need_dw) dw = at::empty({st.V, st.D}, st.w.options());
+  if (st.N == 0) {
+    if (dw && !accumulate) dw->zero_();
+    return {dx, dw};
+  }
+  if (!dx && !dw) return {dx, dw};
+  a.w = st.w.data_ptr();
+  a.ldw = rows_apart(st.w);
+  a.N = st.N;
+  a.V = st.V;
+  a.D = st.D;
+  a.K = st.K;
+  a.distill = st.distill;
+  a.temperature = (float)st.temperature;
+  a.saved = st.saved.data_ptr();
+  a.scalars = st.scalars.data_ptr<float>();
+  a.gout = (float)gout;
+  if (gout_dev) a.gout_dev = gout_dev->data_ptr<float>();
+  a.mean = st.mean;
   if (dx) {
-    slab = at::empty({a.splits * N * a.ld_slab}, w.options().dtype(at::kFloat));
-    a.slab = slab.data_ptr<float>();
+    a.dx = dx->data_ptr();
+    a.lddx = dx->dim() == 2 ? dx->stride(0) : st.D;
   }
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "vocab_bwd", pieces * (1 + (dx ? 1 : 0) + (dw ? 1 : 0)) + (dx ? 1 : 0));
+  if (dw) {
+    a.dw = dw->data_ptr();
+    a.lddw = rows_apart(*dw);
+  }
+  a.dw_add = accumulate;
+  pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), num_sms(), &a.piece, &a.splits);
+  const int pieces = (a.V + a.piece - 1) / a.piece;
+  a.ld_slab = (a.D + 3) / 4 * 4;
+  const int64_t gbytes = (st.N * a.piece * 2 + 255) / 256 * 256;
+  at::Tensor ws = at::empty({gbytes + (dx ? 4 * a.splits * st.N * a.ld_slab : 0)}, st.saved.options());
+  a.g = ws.data_ptr();
+  a.slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", pieces * (1 + (dx ? 1 : 0) + (dw ? 1 : 0)) + (dx ? 1 : 0));
+  return {dx, dw};
 }
 
-void vocab_embed_fwd(const at::Tensor& tok, const at::Tensor& w, double scale, at::Tensor& x) {
-  const int t64 = is64(tok, "tok"), wb = is_bf16(w, "w"), xb = is_bf16(x, "x");
+at::Tensor vocab_embed_fwd(const at::Tensor& tok, const at::Tensor& w, double scale, c10::optional<at::Tensor> out,
+                           at::ScalarType dtype) {
+  const int t64 = is64(tok, "embed_fwd: tok"), wb = is_bf16(w, "embed_fwd: w");
+  PCB_CHECK(w.dim() == 2 && (w.stride(1) == 1 || w.size(1) == 1) && w.numel() > 0,
+            "embed_fwd: w must be [V, D] with a contiguous inner dimension");
+  PCB_CHECK(tok.device() == w.device() && (!out || out->device() == w.device()), "embed_fwd: all operands must be on one device");
   const int64_t N = tok.numel(), V = w.size(0), D = w.size(1);
-  PCB_CHECK(tok.is_contiguous() && x.is_contiguous() && x.numel() == N * D, "embed_fwd: x must be [N, D] contiguous");
-  PCB_CHECK(N >= 1 && V >= 1 && D >= 1, "embed_fwd: empty operand");
+  PCB_CHECK(N < (1LL << 30) && V < (1LL << 31) && D < (1LL << 24), "embed_fwd: an operand is too large");
   const at::cuda::CUDAGuard guard(w.device());
-  check(pcb_vocab_embed_fwd(tok.data_ptr(), t64, w.data_ptr(), wb, row_stride(w, "w"), x.data_ptr(), xb, N, V, D,
-                            (float)scale, cur_stream()),
-        "vocab_embed_fwd");
+  if (out) {
+    is_bf16(*out, "embed_fwd: out");
+    PCB_CHECK(out->is_contiguous() && out->dim() == tok.dim() + 1 && out->size(-1) == D &&
+                  std::equal(tok.sizes().begin(), tok.sizes().end(), out->sizes().begin()),
+              "embed_fwd: out must be contiguous, [*tok.shape, D]");
+  } else {
+    PCB_CHECK(dtype == at::kFloat || dtype == at::kBFloat16, "embed_fwd: dtype must be float32 or bfloat16");
+    std::vector<int64_t> shape(tok.sizes().begin(), tok.sizes().end());
+    shape.push_back(D);
+    out = at::empty(shape, w.options().dtype(dtype));
+  }
+  if (N > 0) {
+    const at::Tensor t = flat(tok);
+    check(pcb_vocab_embed_fwd(t.data_ptr(), t64, w.data_ptr(), wb, rows_apart(w), out->data_ptr(),
+                              out->scalar_type() == at::kBFloat16, N, V, D, (float)scale, cur_stream()),
+          "embed_fwd");
+  }
+  return *out;
 }
 
 // Allocates its workspace.
-void vocab_embed_bwd(const at::Tensor& tok, const at::Tensor& dx, double scale, at::Tensor& dw, bool add) {
-  const int t64 = is64(tok, "tok"), wb = is_bf16(dw, "dw"), xb = is_bf16(dx, "dx");
-  const int64_t N = tok.numel(), V = dw.size(0), D = dw.size(1);
-  PCB_CHECK(tok.is_contiguous() && dw.is_contiguous(), "embed_bwd: tok and dw must be contiguous");
-  PCB_CHECK(dx.dim() == 2 && dx.size(0) == N && dx.size(1) == D, "embed_bwd: dx must be [N, D]");
-  PCB_CHECK(N >= 1 && V >= 1 && D >= 1, "embed_bwd: empty operand");
-  const at::cuda::CUDAGuard guard(dw.device());
-  at::Tensor ws = at::empty({pcb_vocab_embed_bwd_bytes(N, V, D)}, dw.options().dtype(at::kByte));
-  check(pcb_vocab_embed_bwd(tok.data_ptr(), t64, dx.data_ptr(), xb, row_stride(dx, "dx"), dw.data_ptr(), wb, N, V, D,
-                            (float)scale, add ? 1 : 0, ws.data_ptr(), num_sms(), cur_stream()),
-        "vocab_embed_bwd", 8);
+at::Tensor vocab_embed_bwd(const at::Tensor& tok, const at::Tensor& dx, int64_t V, double scale,
+                           c10::optional<at::Tensor> out, at::ScalarType dtype, bool accumulate) {
+  const int t64 = is64(tok, "embed_bwd: tok"), xb = is_bf16(dx, "embed_bwd: dx");
+  PCB_CHECK(dx.dim() >= 1 && same_lead(tok, dx, 0) && dx.size(-1) > 0, "embed_bwd: dx must be [*tok.shape, D]");
+  PCB_CHECK(tok.device() == dx.device() && (!out || out->device() == dx.device()), "embed_bwd: all operands must be on one device");
+  const int64_t N = tok.numel(), D = dx.size(-1);
+  PCB_CHECK(V >= 1 && N < (1LL << 30) && V < (1LL << 31) && D < (1LL << 24), "embed_bwd: vocab must be positive, and no operand too large");
+  const at::cuda::CUDAGuard guard(dx.device());
+  if (out) {
+    is_bf16(*out, "embed_bwd: out");
+    PCB_CHECK(out->is_contiguous() && out->dim() == 2 && out->size(0) == V && out->size(1) == D,
+              "embed_bwd: out must be contiguous, [vocab, D]");
+  } else {
+    PCB_CHECK(!accumulate, "embed_bwd: accumulate needs out");
+    PCB_CHECK(dtype == at::kFloat || dtype == at::kBFloat16, "embed_bwd: dtype must be float32 or bfloat16");
+    out = at::empty({V, D}, dx.options().dtype(dtype));
+  }
+  if (N == 0) {
+    if (!accumulate) out->zero_();
+    return *out;
+  }
+  const at::Tensor t = flat(tok), d2 = as_rows(dx);
+  at::Tensor ws = at::empty({pcb_vocab_embed_bwd_bytes(N, V, D)}, dx.options().dtype(at::kByte));
+  check(pcb_vocab_embed_bwd(t.data_ptr(), t64, d2.data_ptr(), xb, rows_apart(d2), out->data_ptr(),
+                            out->scalar_type() == at::kBFloat16, N, V, D, (float)scale, accumulate ? 1 : 0, ws.data_ptr(),
+                            num_sms(), cur_stream()),
+        "embed_bwd", 3);
+  return *out;
 }
 
 // ---------------------------------------------------------------- mixture of experts
@@ -1119,8 +1246,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("skinny_gemm", &skinny_gemm, py::arg("x"), py::arg("w"), py::arg("y"), py::arg("err") = py::none(),
         py::arg("trace") = py::none(), py::arg("swiglu") = false);
   m.def("skinny_qkv_rope", &skinny_qkv_rope);
-  m.def("vocab_fwd", &vocab_fwd);
-  m.def("vocab_bwd", &vocab_bwd);
+  py::class_<HeadState>(m, "HeadState")
+      .def_readonly("saved", &HeadState::saved)
+      .def_readonly("w", &HeadState::w)
+      .def_readonly("lead", &HeadState::lead)
+      .def_readonly("N", &HeadState::N)
+      .def_readonly("V", &HeadState::V)
+      .def_readonly("D", &HeadState::D)
+      .def_readonly("K", &HeadState::K)
+      .def_readonly("distill", &HeadState::distill)
+      .def_readonly("temperature", &HeadState::temperature);
+  m.def("vocab_ce_fwd", &vocab_ce_fwd);
+  m.def("vocab_distill_fwd", &vocab_distill_fwd);
+  m.def("vocab_head_bwd", &vocab_head_bwd);
   m.def("vocab_embed_fwd", &vocab_embed_fwd);
   m.def("vocab_embed_bwd", &vocab_embed_bwd);
   m.def("moe_route", &moe_route);

@@ -23,7 +23,7 @@ namespace pcb {
 namespace vocab {
 
 constexpr int kThreads = 256;
-constexpr int kMaxK = 256;   // teacher entries per row
+constexpr int kMaxK = kVocabMaxEntries;
 
 PCB_DEVICE long long load_id(const void* p, int is64, long long i) {
   return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
@@ -50,6 +50,49 @@ PCB_DEVICE int block_scan(int v, int* warp_sums, int* sum) {
   return before + inc - v;
 }
 
+template <typename T> PCB_DEVICE float to_f32(T v);
+template <> PCB_DEVICE float to_f32<float>(float v) { return v; }
+template <> PCB_DEVICE float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> PCB_DEVICE T from_f32(float v);
+template <> PCB_DEVICE float from_f32<float>(float v) { return v; }
+template <> PCB_DEVICE __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int VEC>
+PCB_DEVICE void load_vec(const T* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32<T>(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    static_assert(VEC % 4 == 0, "16-byte vectors");
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 f = reinterpret_cast<const float4*>(p)[i];
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+  } else if constexpr (VEC == 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
+    v[4] = bf16_lo(u.z); v[5] = bf16_hi(u.z); v[6] = bf16_lo(u.w); v[7] = bf16_hi(u.w);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
+  }
+}
+template <typename T, int VEC>
+PCB_DEVICE void store_vec(T* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else if constexpr (VEC == 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  }
+}
+
 // ---------------------------------------------------------------- packing
 // Packs the counted rows in order.  Block b owns rows [b R, (b + 1) R) and counts the rows before them by itself, so
 // that one launch does it without a scan over the blocks (8 bytes a row from L2, against 2 D a row copied).
@@ -60,6 +103,7 @@ __global__ void __launch_bounds__(kThreads)
                      int* __restrict__ tgt32, int* __restrict__ count) {
   __shared__ int sums[kThreads / 32];
   __shared__ int src[kThreads];
+  pdl_begin();
   auto counted = [&](int n) -> bool {
     if (len != nullptr) return len[n] > 0;
     const long long t = load_id(tgt, tgt64, n);
@@ -70,8 +114,15 @@ __global__ void __launch_bounds__(kThreads)
     __nv_bfloat16* d = xc + j * ldxc;
     if (vec) {
       const uint4* s = reinterpret_cast<const uint4*>(x + (long long)max(n, 0) * ldx);
-      for (int i = lane; i < (int)(ldxc / 8); i += 32)
-        reinterpret_cast<uint4*>(d)[i] = n < 0 ? make_uint4(0, 0, 0, 0) : s[i];
+      const int nv = (int)(ldxc / 8);
+      for (int i0 = lane; i0 < nv; i0 += 128) {
+        uint4 r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r[u] = n >= 0 && i0 + 32 * u < nv ? s[i0 + 32 * u] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i0 + 32 * u < nv) reinterpret_cast<uint4*>(d)[i0 + 32 * u] = r[u];
+      }
     } else {
       const __nv_bfloat16* s = x + (long long)max(n, 0) * ldx;
       for (int i = lane; i < (int)ldxc; i += 32) d[i] = n >= 0 && i < D ? s[i] : __float2bfloat16_rn(0.f);
@@ -100,7 +151,10 @@ __global__ void __launch_bounds__(kThreads)
     base += total;
   }
   if (blockIdx.x == gridDim.x - 1) {
-    if (threadIdx.x == 0) *count = base;
+    if (threadIdx.x == 0) {
+      count[0] = base;
+      count[1] = 0;   // blocks of row_loss_kernel that are done
+    }
     const int end = min(N, (max(base, 1) + 63) / 64 * 64);
     for (int j = base + (threadIdx.x >> 5); j < end; j += kThreads / 32) zero_or_copy(-1, j);
   }
@@ -125,6 +179,7 @@ __global__ void __launch_bounds__(kThreads)
                         unsigned short* __restrict__ start, int granules) {
   __shared__ int s_id[kThreads / 32][kMaxK];
   __shared__ int s_sorted[kThreads / 32][kMaxK];
+  pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = blockIdx.x * (kThreads / 32) + w;
   if (n >= N) return;   // whole warps
@@ -189,20 +244,27 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ---------------------------------------------------------------- row losses
-// 32 rows a block, 8 threads a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.
-__global__ void __launch_bounds__(256)
+// 32 rows a block, 32 threads a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.
+// The last block to finish adds the losses up, in a fixed order and in 64 bits: scalars[0] = their sum or mean,
+// scalars[1] = 1 / counted rows (both 0 when there are none).
+constexpr int kLossParts = 32;
+
+__global__ void __launch_bounds__(32 * kLossParts)
     row_loss_kernel(const float2* __restrict__ part, int granules, long long ld_part, const int* __restrict__ pos,
                     const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
                     const int* __restrict__ len, int N, int K, float c, float factor, float* __restrict__ lse_out,
-                    float* __restrict__ loss) {
-  __shared__ float sm[8][33], ss[8][33], sl[8][33];
+                    float* loss, int* count, int mean, float* __restrict__ scalars) {
+  __shared__ float sm[kLossParts][33], ss[kLossParts][33], sl[kLossParts][33];
+  __shared__ double sums[kLossParts];
+  __shared__ int last;
+  pdl_begin();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n = blockIdx.x * 32 + tx;
   const int j = n < N ? pos[n] : -1;
   float m = -INFINITY, s = 0.f;
   if (j >= 0) {
 #pragma unroll 4
-    for (int g = ty; g < granules; g += 8) {
+    for (int g = ty; g < granules; g += kLossParts) {
       const float2 p = part[g * ld_part + j];
       const float nm = fmaxf(m, p.x);
       const float ref = nm == -INFINITY ? 0.f : nm;
@@ -213,19 +275,21 @@ __global__ void __launch_bounds__(256)
   sm[ty][tx] = m;
   ss[ty][tx] = s;
   __syncthreads();
-  float mm = -INFINITY, tot = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) mm = fmaxf(mm, sm[i][tx]);
+  // warp ty joins the parts of column ty: lane = part
+  m = sm[tx][ty];
+  const float mm = warp_max(m);
   const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) tot += ss[i][tx] * exp2f(sm[i][tx] - ref);
-  const float lse = ref + log2f(tot);
+  const float tot = warp_sum(ss[tx][ty] * exp2f(m - ref));
+  __syncthreads();
+  if (tx == 0) sm[0][ty] = ref + log2f(tot);
+  __syncthreads();
+  const float lse = sm[0][tx];
   // sum_k q_k (log2 q_k + lse - c z_k), term by term: each is a difference of logarithms of the same size
   float l = 0.f;
   if (j >= 0) {
     const long long at = (long long)n * K;
     const int e = len != nullptr ? len[n] : 1;
-    for (int k = ty; k < e; k += 8) {
+    for (int k = ty; k < e; k += kLossParts) {
       const float d = fmaf(-c, z[at + k], lse);
       if (q == nullptr) l += d;
       else if (q[at + k] != 0.f) l += q[at + k] * (lq[at + k] + d);   // 0 log 0 = 0
@@ -233,143 +297,111 @@ __global__ void __launch_bounds__(256)
   }
   sl[ty][tx] = l;
   __syncthreads();
+  const float sum = warp_sum(sl[tx][ty]);
+  if (tx == 0) sl[0][ty] = sum;   // read by this warp only
+  __syncthreads();
   if (ty == 0 && n < N) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += sl[i][tx];
-    loss[n] = j >= 0 ? sum * factor : 0.f;
+    loss[n] = j >= 0 ? sl[0][tx] * factor : 0.f;
     if (j >= 0) lse_out[n] = lse;
   }
-}
-
-// scalars[0] = sum or mean of the row losses, scalars[1] = 1 / counted rows (0 when there are none); one block,
-// a fixed order, sums in 64 bits
-__global__ void __launch_bounds__(1024)
-    reduce_loss_kernel(const float* __restrict__ loss, int N, const int* __restrict__ count, int mean,
-                       float* __restrict__ scalars) {
-  __shared__ double part[32];
-  double s = 0.0;
-  for (int n = threadIdx.x; n < N; n += 1024) s += loss[n];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  if (scalars == nullptr) return;
+  __threadfence();
   __syncthreads();
-  if (threadIdx.x < 32) {
-    s = part[threadIdx.x];
+  if (threadIdx.x == 0) last = atomicAdd(&count[1], 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double t = 0.0;
+  for (int i = threadIdx.x; i < N; i += 32 * kLossParts) t += __ldcg(loss + i);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) {
-      const int c = *count;
-      scalars[0] = (float)(mean ? (c > 0 ? s / c : 0.0) : s);
-      scalars[1] = c > 0 ? 1.f / (float)c : 0.f;
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (tx == 0) sums[ty] = t;
+  __syncthreads();
+  if (ty == 0) {
+    t = sums[tx];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (tx == 0) {
+      const int rows = count[0];
+      scalars[0] = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
+      scalars[1] = rows > 0 ? 1.f / (float)rows : 0.f;
     }
   }
 }
 
 // dx of every row from the packed slabs: their sum in slab order, times the gradient's factor; zero where the row
-// is not counted
+// is not counted.  A warp per row and slice of columns.
+constexpr int kFinishVecs = 4;
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
     finish_dx_kernel(const float* __restrict__ slab, long long slab_stride, int slabs, long long ld,
                      const int* __restrict__ pos, T* __restrict__ dx, long long lddx, int N, int D, float alpha,
                      const float* __restrict__ scale, const float* __restrict__ scale2) {
-  const int per_row = (D + VEC - 1) / VEC;
-  const long long total = (long long)N * per_row;
+  pdl_begin();
+  const int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (n >= N) return;
+  const int j = pos[n];
   float a = alpha;
   if (scale != nullptr) a *= *scale;
   if (scale2 != nullptr) a *= *scale2;
-  for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
-    const int n = (int)(i / per_row);
-    const int d0 = (int)(i - (long long)n * per_row) * VEC;
-    const int j = pos[n];
-    float v[VEC] = {};
-    if (j >= 0) {
-      const float* s = slab + (long long)j * ld + d0;
-      for (int k = 0; k < slabs; ++k, s += slab_stride) {
-        if constexpr (VEC == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(s);
-          v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-        } else {
-          v[0] += *s;
-        }
-      }
+  const int d0 = (blockIdx.y * kFinishVecs * 32 + (threadIdx.x & 31)) * VEC;
+  const float* src = slab + (long long)max(j, 0) * ld + d0;
+  float v[kFinishVecs][VEC] = {};
+  if (j >= 0) {
+    for (int k = 0; k < slabs; ++k, src += slab_stride) {
+      float r[kFinishVecs][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] *= a;
+      for (int i = 0; i < kFinishVecs; ++i)
+        if (d0 + i * 32 * VEC < D) load_vec<float, VEC>(src + i * 32 * VEC, r[i]);
+#pragma unroll
+      for (int i = 0; i < kFinishVecs; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (d0 + i * 32 * VEC < D) v[i][e] += r[i][e];
     }
-    T* o = dx + n * lddx + d0;
-    if constexpr (sizeof(T) == 4) {
-      if constexpr (VEC == 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-      else *o = v[0];
-    } else {
-      if constexpr (VEC == 4) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      else *o = __float2bfloat16_rn(v[0]);
-    }
+  }
+  T* o = dx + n * lddx + d0;
+#pragma unroll
+  for (int i = 0; i < kFinishVecs; ++i) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[i][e] = j >= 0 ? a * v[i][e] : 0.f;
+    if (d0 + i * 32 * VEC < D) store_vec<T, VEC>(o + i * 32 * VEC, v[i]);
   }
 }
 
 // ---------------------------------------------------------------- embedding
-template <typename T> PCB_DEVICE float to_f32(T v);
-template <> PCB_DEVICE float to_f32<float>(float v) { return v; }
-template <> PCB_DEVICE float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> PCB_DEVICE T from_f32(float v);
-template <> PCB_DEVICE float from_f32<float>(float v) { return v; }
-template <> PCB_DEVICE __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// A warp copies kLookupVecs vectors a lane of one row; wide rows take several warps.  All loads of a lane are issued
+// before its first store.
+constexpr int kLookupVecs = 4;
 
-template <typename T, int VEC>
-PCB_DEVICE void load_vec(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32<T>(*p);
-  } else if constexpr (sizeof(T) == 4) {
-    static_assert(VEC % 4 == 0, "16-byte vectors");
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) {
-      const float4 f = reinterpret_cast<const float4*>(p)[i];
-      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
-    }
-  } else if constexpr (VEC == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
-    v[4] = bf16_lo(u.z); v[5] = bf16_hi(u.z); v[6] = bf16_lo(u.w); v[7] = bf16_hi(u.w);
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
-  }
-}
-template <typename T, int VEC>
-PCB_DEVICE void store_vec(T* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    *p = from_f32<T>(v[0]);
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else if constexpr (VEC == 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-  }
-}
-
-// one vector of VEC columns per thread
 template <typename TW, typename TX, int VEC>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(const void* __restrict__ tok, int tok64, const TW* __restrict__ w, long long ldw, TX* __restrict__ x,
-                  long long total, int per_row, int V, int D, float scale) {
-  const long long i = blockIdx.x * (long long)kThreads + threadIdx.x;
-  if (i >= total) return;
-  const long long n = i / per_row;
-  const int d0 = (int)(i - n * per_row) * VEC;
+                  int N, int V, int D, float scale) {
+  pdl_begin();
+  const int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (n >= N) return;
   const long long t = load_id(tok, tok64, n);
-  float v[VEC];
+  const bool in = t >= 0 && t < V;
+  const int d0 = (blockIdx.y * kLookupVecs * 32 + (threadIdx.x & 31)) * VEC;
+  const TW* src = w + (in ? t : 0) * ldw;
+  TX* dst = x + (long long)n * D;
+  float v[kLookupVecs][VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-  if (t >= 0 && t < V) {
-    load_vec<TW, VEC>(w + t * ldw + d0, v);
+  for (int i = 0; i < kLookupVecs; ++i) {
+    const int d = d0 + i * 32 * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] *= scale;
+    for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+    if (in && d < D) load_vec<TW, VEC>(src + d, v[i]);
   }
-  store_vec<TX, VEC>(x + n * D + d0, v);
+#pragma unroll
+  for (int i = 0; i < kLookupVecs; ++i) {
+    const int d = d0 + i * 32 * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[i][e] *= scale;
+    if (d < D) store_vec<TX, VEC>(dst + d, v[i]);
+  }
 }
 
 // ---- stable sort of (token, place) by token: least significant digit first, 8 bits a pass.  Tokens outside
@@ -455,10 +487,153 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// ---- the same sort in one launch for up to 64 K keys: a cluster of 8 blocks holds them in registers and exchanges
+// them through distributed shared memory, so a pass costs two cluster barriers instead of three launches.  The
+// other clusters of the grid meanwhile write the zeros of the gradient, which bound this part when the matrix is large.
+constexpr int kCluster = 8;
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+
+template <int ITEMS>
+constexpr int cluster_sort_smem() {
+  return kClusterWarps * 256 * 4 + kCluster * 256 * 4 + 4 * 256 * 4 + 256 * 4 + ITEMS * kClusterThreads * 8;
+}
+
+PCB_DEVICE void write_zeros(char* p, long long bytes, int part, int parts) {
+  const long long head = min(bytes, (long long)(-reinterpret_cast<uintptr_t>(p) & 15));
+  const long long vecs = (bytes - head) / 16, tail = head + vecs * 16;
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+  for (long long i = part * (long long)blockDim.x + threadIdx.x; i < vecs; i += (long long)parts * blockDim.x)
+    q[i] = make_uint4(0, 0, 0, 0);
+  if (part == 0) {
+    for (long long i = threadIdx.x; i < head; i += blockDim.x) p[i] = 0;
+    for (long long i = tail + threadIdx.x; i < bytes; i += blockDim.x) p[i] = 0;
+  }
+}
+
+template <int ITEMS>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads)
+    cluster_sort_kernel(const void* __restrict__ tok, int tok64, int N, int V, int bits, uint32_t* __restrict__ keys_out,
+                        uint32_t* __restrict__ idx_out, char* zeros, long long zero_bytes) {
+  extern __shared__ __align__(16) uint32_t sm[];
+  uint32_t* warp_count = sm;                                     // [warps][256]: keys of a digit, then its first place
+  uint32_t* count = warp_count + kClusterWarps * 256;            // [blocks][256], the same in every block
+  uint32_t* quarter = count + kCluster * 256;                    // [4][256]
+  uint32_t* first = quarter + 4 * 256;                           // [256] first place of this block's digit
+  unsigned long long* pairs = reinterpret_cast<unsigned long long*>(first + 256);   // [ITEMS * 1024] place << 32 | key
+  __shared__ int sums[32];
+  pdl_begin();
+  if (blockIdx.x >= kCluster) {   // whole clusters
+    write_zeros(zeros, zero_bytes, blockIdx.x - kCluster, gridDim.x - kCluster);
+    return;
+  }
+  constexpr int PER = ITEMS * kClusterThreads;
+  cluster_sync_all();   // every block of the cluster runs before another one writes to its shared memory
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int rank = (int)cluster_ctarank();
+  const int mine = max(0, min(PER, N - rank * PER));
+  uint32_t key[ITEMS], idx[ITEMS], place[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int k = (w * ITEMS + i) * 32 + lane;
+    key[i] = k < mine ? sort_key(tok, tok64, nullptr, rank * PER + k, V) : 0u;
+    idx[i] = (uint32_t)(rank * PER + k);
+  }
+  for (int shift = 0; shift < bits; shift += 8) {
+    const bool last = shift + 8 >= bits;
+    for (int i = tid; i < kClusterWarps * 256 / 4; i += kClusterThreads)
+      reinterpret_cast<uint4*>(warp_count)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    uint32_t* wc = warp_count + w * 256;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {   // place among the warp's keys of the same digit, in order
+      const bool in = (w * ITEMS + i) * 32 + lane < mine;
+      const uint32_t digit = in ? (key[i] >> shift) & 255 : 256u;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      const uint32_t before = __popc(same & ((1u << lane) - 1));
+      const uint32_t have = in ? wc[digit] : 0u;
+      place[i] = have + before;
+      __syncwarp();
+      if (in && before == 0) wc[digit] = have + __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    {   // over the warps: 4 threads a digit, 8 warps each
+      const int d = tid & 255, part = tid >> 8;
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c[j] = warp_count[(part * 8 + j) * 256 + d];
+        sum += c[j];
+      }
+      quarter[part * 256 + d] = sum;
+      __syncthreads();
+      uint32_t base = 0, all = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t v = quarter[j * 256 + d];
+        if (j < part) base += v;
+        all += v;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        warp_count[(part * 8 + j) * 256 + d] = base;
+        base += c[j];
+      }
+#pragma unroll
+      for (int j = 0; j < kCluster / 4; ++j)   // this block's count of the digit, to every block
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                         mapa_shared(smem_u32(count + rank * 256 + d), part * (kCluster / 4) + j)),
+                     "r"(all)
+                     : "memory");
+    }
+    cluster_sync_all();
+    {
+      uint32_t before = 0, all = 0;
+      if (tid < 256) {
+#pragma unroll
+        for (int j = 0; j < kCluster; ++j) {
+          const uint32_t v = count[j * 256 + tid];
+          if (j < rank) before += v;
+          all += v;
+        }
+      }
+      int total;
+      const int start = block_scan((int)all, sums, &total);
+      if (tid < 256) first[tid] = start + before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if ((w * ITEMS + i) * 32 + lane < mine) {
+        const uint32_t digit = (key[i] >> shift) & 255;
+        const uint32_t at = first[digit] + wc[digit] + place[i];
+        if (last) {
+          keys_out[at] = key[i];
+          idx_out[at] = idx[i];
+        } else {
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(pairs + at % PER), at / PER)),
+                       "l"((unsigned long long)idx[i] << 32 | key[i])
+                       : "memory");
+        }
+      }
+    }
+    if (last) break;
+    cluster_sync_all();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int k = (w * ITEMS + i) * 32 + lane;
+      const unsigned long long p = k < mine ? pairs[k] : 0ull;
+      key[i] = (uint32_t)p;
+      idx[i] = (uint32_t)(p >> 32);
+    }
+  }
+}
+
 // ---- sums over runs of equal tokens.  A block owns kChunk consecutive sorted entries and a slice of the columns;
 // a thread keeps VEC columns in registers over the run.  A run inside the chunk is written at once; the part of
 // a run that crosses a chunk's edge goes to a partial row, and join_kernel adds those in order.
-constexpr int kChunk = 32;
+constexpr int kChunk = 16;
 
 template <typename TX, typename TW, int VEC>
 PCB_DEVICE void emit(TW* dw, uint32_t id, int D, int d0, float (&a)[VEC], float scale, int add) {
@@ -480,6 +655,7 @@ __global__ void __launch_bounds__(kThreads)
                     long long lddx, TW* __restrict__ dw, float* __restrict__ partial, int N, int V, int D, float scale,
                     int add) {
   __shared__ uint32_t s_key[kChunk + 2], s_idx[kChunk];
+  pdl_begin();
   const int c0 = blockIdx.x * kChunk, cnt = min(kChunk, N - c0);
   for (int i = threadIdx.x; i < cnt + 2; i += blockDim.x) {   // with both neighbours
     const long long n = (long long)c0 + i - 1;
@@ -511,8 +687,7 @@ __global__ void __launch_bounds__(kThreads)
           emit<TX, TW, VEC>(dw, id, D, d0, acc, scale, add);
         } else {
           float* p = partial + ((long long)blockIdx.x * 2 + (begun_before ? 0 : 1)) * D + d0;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+          store_vec<float, VEC>(p, acc);
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
@@ -527,22 +702,36 @@ template <typename TW, int VEC>
 __global__ void __launch_bounds__(kThreads)
     join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, TW* __restrict__ dw, int N, int V,
                 int D, float scale, int add) {
-  const int c0 = blockIdx.x * kChunk;
-  const long long last = (long long)c0 + kChunk - 1;
-  if (last + 1 >= N) return;
-  const uint32_t id = keys[last];
-  if (id >= (uint32_t)V || keys[last + 1] != id) return;
+  pdl_begin();
+  const long long c0 = (long long)blockIdx.x * kChunk, next = c0 + kChunk;
+  if (next >= N) return;
+  const uint32_t id = keys[next - 1];
+  if (id >= (uint32_t)V || keys[next] != id) return;
   if (c0 > 0 && keys[c0 - 1] == id) return;   // begun in an earlier chunk
+  int parts = 0;                              // chunks behind this one that begin with the run
+  for (int more = blockDim.x; more == (int)blockDim.x;) {
+    const long long at = next + ((long long)parts + threadIdx.x) * kChunk;
+    more = __syncthreads_count(at < N && keys[at] == id);
+    parts += more;
+  }
   const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   if (d0 >= D) return;
   float acc[VEC];
   const float* p = partial + ((long long)blockIdx.x * 2 + 1) * D + d0;
+  load_vec<float, VEC>(p, acc);
+  p += D;
+  constexpr int U = 8;
+  for (int c = 0; c < parts; c += U) {
+    float r[U][VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = p[e];
-  for (int c = blockIdx.x + 1; (long long)c * kChunk < N && keys[(long long)c * kChunk] == id; ++c) {
-    p = partial + (long long)c * 2 * D + d0;
+    for (int u = 0; u < U; ++u)
+      if (c + u < parts) load_vec<float, VEC>(p + (long long)(c + u) * 2 * D, r[u]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] += p[e];
+    for (int u = 0; u < U; ++u) {
+      if (c + u >= parts) break;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += r[u][e];
+    }
   }
   emit<float, TW, VEC>(dw, id, D, d0, acc, scale, add);
 }
@@ -635,18 +824,17 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   __nv_bfloat16* xc = (__nv_bfloat16*)at(saved, l.xc);
   const float T = distill ? a.temperature : 1.f;
   const float c = 1.4426950408889634f / T;
-  if (distill) {
-    sort_targets_kernel<<<(a.N + 7) / 8, kThreads, 0, s>>>(a.ids, a.ids64, a.ld_ids, a.logits, a.logits_bf16,
-                                                         a.ld_logits, a.N, a.V, a.K, c, ids, q, lq, len, start,
-                                                         l.granules);
-    if (launched()) return -3;
-  }
-  const int blocks = std::max(1, std::min(2 * num_sms, (a.N + 7) / 8));
+  if (distill &&
+      pdl_launch(sort_targets_kernel, dim3((a.N + 7) / 8), dim3(kThreads), 0, s, a.ids, a.ids64, a.ld_ids, a.logits,
+                 a.logits_bf16, a.ld_logits, a.N, a.V, a.K, c, ids, q, lq, len, start, l.granules) != cudaSuccess)
+    return -3;
+  const int blocks = std::max(1, std::min(4 * num_sms, (a.N + 7) / 8));
   const int R = (a.N + blocks - 1) / blocks;
   const int vec = a.D % 8 == 0 && a.ldx % 8 == 0 && al(a.x, 16);
-  pack_rows_kernel<<<blocks, kThreads, 0, s>>>(a.tgt, a.tgt64, a.ignore, len, a.V, (const __nv_bfloat16*)a.x, a.ldx,
-                                               a.N, a.D, R, vec, xc, l.ldxc, row, pos, distill ? nullptr : ids, count);
-  if (launched()) return -3;
+  if (pdl_launch(pack_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a.tgt, a.tgt64, a.ignore, (const int*)len, a.V,
+                 (const __nv_bfloat16*)a.x, a.ldx, a.N, a.D, R, vec, xc, l.ldxc, row, pos, distill ? nullptr : ids,
+                 count) != cudaSuccess)
+    return -3;
   GemmArgs g{};
   g.M = a.N;
   g.N = a.V;
@@ -664,11 +852,9 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   g.vh.ld_start = a.N;
   int rc = pcb_gemm_pair_launch(xc, 0, l.ldxc, a.w, 0, a.ldw, EPI_VH_STAT, g, 256, 1, num_sms, s);
   if (rc) return rc;
-  row_loss_kernel<<<(a.N + 31) / 32, 256, 0, s>>>((const float2*)part, l.granules, a.N, pos, z, q, lq, len, a.N, a.K, c,
-                                                 0.6931471805599453f * T * T, lse, a.loss);
-  if (launched()) return -3;
-  reduce_loss_kernel<<<1, 1024, 0, s>>>(a.loss, a.N, count, mean, a.scalars);
-  return launched();
+  return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, l.granules,
+                    (long long)a.N, (const int*)pos, (const float*)z, (const float*)q, (const float*)lq, (const int*)len,
+                    a.N, a.K, c, 0.6931471805599453f * T * T, lse, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
 }
 
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
@@ -740,13 +926,15 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   }
   if (a.dx == nullptr) return 0;
   const bool v4 = a.D % 4 == 0 && a.lddx % 4 == 0 && al(a.dx, a.dx_f32 ? 16 : 8);
-  const long long total = (long long)a.N * (v4 ? a.D / 4 : a.D);
-  const int grid = (int)std::min<long long>((total + kThreads - 1) / kThreads, num_sms * 16);
   const long long stride = (long long)a.N * a.ld_slab;
+  int rc = 0;
   auto go = [&](auto* dx, auto vec) {
     using T2 = std::remove_pointer_t<decltype(dx)>;
-    finish_dx_kernel<T2, decltype(vec)::value><<<grid, kThreads, 0, s>>>(a.slab, stride, a.splits, a.ld_slab, pos, dx,
-                                                                         a.lddx, a.N, a.D, a.gout * T, inv, a.gout_dev);
+    constexpr int VEC = decltype(vec)::value;
+    const dim3 grid((a.N + 7) / 8, ((a.D + VEC - 1) / VEC + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
+    if (grid.y > 65535) { rc = -1; return; }
+    rc = pdl_launch(finish_dx_kernel<T2, VEC>, grid, dim3(kThreads), 0, s, (const float*)a.slab, stride, a.splits,
+                    a.ld_slab, pos, dx, a.lddx, a.N, a.D, a.gout * T, inv, a.gout_dev) == cudaSuccess ? 0 : -3;
   };
   if (a.dx_f32) {
     if (v4) go((float*)a.dx, std::integral_constant<int, 4>{});
@@ -755,7 +943,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     if (v4) go((__nv_bfloat16*)a.dx, std::integral_constant<int, 4>{});
     else go((__nv_bfloat16*)a.dx, std::integral_constant<int, 1>{});
   }
-  return launched();
+  return rc;
 }
 
 template <typename F>
@@ -771,73 +959,117 @@ static void by_type(int w_bf16, int x_bf16, F f) {
 
 int pcb_vocab_embed_fwd(const void* tok, int tok64, const void* w, int w_bf16, long long ldw, void* x, int x_bf16,
                         int N, int V, int D, float scale, cudaStream_t s) {
-  const bool vec = D % 4 == 0 && ldw % 4 == 0 && al(w, w_bf16 ? 8 : 16) && al(x, x_bf16 ? 8 : 16);
-  const int per_row = vec ? D / 4 : D;
-  const long long total = (long long)N * per_row, blocks = (total + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return -1;
+  int rc = 0;
   by_type(w_bf16, x_bf16, [&](auto* tw, auto* tx) {
     using TW = std::remove_pointer_t<decltype(tw)>;
     using TX = std::remove_pointer_t<decltype(tx)>;
-    if (vec)
-      lookup_kernel<TW, TX, 4><<<(unsigned)blocks, kThreads, 0, s>>>(tok, tok64, (const TW*)w, ldw, (TX*)x, total, per_row,
-                                                                    V, D, scale);
-    else
-      lookup_kernel<TW, TX, 1><<<(unsigned)blocks, kThreads, 0, s>>>(tok, tok64, (const TW*)w, ldw, (TX*)x, total, per_row,
-                                                                    V, D, scale);
+    auto go = [&](auto v) {
+      constexpr int VEC = decltype(v)::value;
+      const int vecs = (D + VEC - 1) / VEC;
+      const dim3 grid((N + 7) / 8, (vecs + 32 * kLookupVecs - 1) / (32 * kLookupVecs));
+      if (grid.y > 65535) { rc = -1; return; }
+      rc = pdl_launch(lookup_kernel<TW, TX, VEC>, grid, dim3(kThreads), 0, s, tok, tok64, (const TW*)w, ldw, (TX*)x, N, V,
+                      D, scale) == cudaSuccess ? 0 : -3;
+    };
+    if (D % 4 == 0 && ldw % 4 == 0 && al(w, w_bf16 ? 8 : 16) && al(x, x_bf16 ? 8 : 16)) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1>{});
   });
-  return launched();
+  return rc;
 }
 
 static long long up256(long long b) { return (b + 255) / 256 * 256; }
 
+// keys of one cluster's sort; longer batches take the launch-per-step sort
+constexpr int kClusterKeys = 8 * kCluster * kClusterThreads;
+
 long long pcb_vocab_embed_bwd_bytes(int N, int V, int D) {
   const long long blocks = (N + kSortTile - 1) / kSortTile, chunks = (N + kChunk - 1) / kChunk;
-  return 4 * up256(4LL * N) + up256(4LL * 256 * blocks) + up256(8LL * chunks * D);
+  return (N <= kClusterKeys ? 2 : 4) * up256(4LL * N) + (N <= kClusterKeys ? 0 : up256(4LL * 256 * blocks)) +
+         up256(8LL * chunks * D);
+}
+
+template <int ITEMS>
+static int launch_cluster_sort(const void* tok, int tok64, int N, int V, int bits, uint32_t* keys, uint32_t* idx,
+                               void* zeros, long long zero_bytes, int num_sms, cudaStream_t s) {
+  constexpr int smem = cluster_sort_smem<ITEMS>();
+  static bool attr_done = false;
+  if (!attr_done) {
+    if (cudaFuncSetAttribute(cluster_sort_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return -3;
+    attr_done = true;
+  }
+  // as many more clusters as there is for them to write, 64 KB a block at least
+  const int most = std::max(1, num_sms / kCluster - 2);
+  const int clusters = zero_bytes > 0 ? 1 + (int)std::min<long long>(most, (zero_bytes >> 19) + 1) : 1;
+  return pdl_launch(cluster_sort_kernel<ITEMS>, dim3(clusters * kCluster), dim3(kClusterThreads), smem, s, tok, tok64, N,
+                    V, bits, keys, idx, (char*)zeros, zero_bytes) == cudaSuccess ? 0 : -3;
 }
 
 int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16, long long lddx, void* dw, int dw_bf16,
                         int N, int V, int D, float scale, int add, void* ws, int num_sms, cudaStream_t s) {
   const int blocks = (N + kSortTile - 1) / kSortTile, chunks = (N + kChunk - 1) / kChunk;
   if (blocks > (1 << 22)) return -1;   // 256 counts a block are scanned as ints
+  const long long zero_bytes = add ? 0 : (long long)V * D * (dw_bf16 ? 2 : 4);
   char* p = (char*)ws;
-  uint32_t* buf[4];
-  for (auto& b : buf) {
-    b = (uint32_t*)p;
-    p += up256(4LL * N);
-  }
-  uint32_t* hist = (uint32_t*)p;
-  p += up256(4LL * 256 * blocks);
-  float* partial = (float*)p;
-  if (!add && cudaMemsetAsync(dw, 0, (size_t)V * D * (dw_bf16 ? 2 : 4), s) != cudaSuccess) return -3;
+  auto take = [&](long long bytes) {
+    char* q = p;
+    p += up256(bytes);
+    return q;
+  };
   int bits = 1;
   while (bits < 32 && (V >> bits) != 0) ++bits;   // keys run up to V
   const uint32_t *keys = nullptr, *idx = nullptr;
-  int side = 0;
-  for (int shift = 0; shift < bits; shift += 8) {
-    sort_hist_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, N, V, shift, hist, blocks);
-    sort_scan_kernel<<<1, 1024, 0, s>>>(hist, 256 * blocks);
-    sort_scatter_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, idx, N, V, shift, hist, blocks, buf[2 * side],
-                                                    buf[2 * side + 1]);
-    if (launched()) return -3;
-    keys = buf[2 * side];
-    idx = buf[2 * side + 1];
-    side ^= 1;
+  int rc = 0;
+  if (N <= kClusterKeys) {
+    uint32_t *k = (uint32_t*)take(4LL * N), *i = (uint32_t*)take(4LL * N);
+    auto sort = [&](auto items) {
+      return launch_cluster_sort<decltype(items)::value>(tok, tok64, N, V, bits, k, i, dw, zero_bytes, num_sms, s);
+    };
+    if (N <= kClusterKeys / 8) rc = sort(std::integral_constant<int, 1>{});
+    else if (N <= kClusterKeys / 4) rc = sort(std::integral_constant<int, 2>{});
+    else if (N <= kClusterKeys / 2) rc = sort(std::integral_constant<int, 4>{});
+    else rc = sort(std::integral_constant<int, 8>{});
+    if (rc) return rc;
+    keys = k;
+    idx = i;
+  } else {
+    uint32_t* buf[4];
+    for (auto& b : buf) b = (uint32_t*)take(4LL * N);
+    uint32_t* hist = (uint32_t*)take(4LL * 256 * blocks);
+    if (zero_bytes > 0 && cudaMemsetAsync(dw, 0, (size_t)zero_bytes, s) != cudaSuccess) return -3;
+    int side = 0;
+    for (int shift = 0; shift < bits; shift += 8) {
+      sort_hist_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, N, V, shift, hist, blocks);
+      sort_scan_kernel<<<1, 1024, 0, s>>>(hist, 256 * blocks);
+      sort_scatter_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, idx, N, V, shift, hist, blocks, buf[2 * side],
+                                                      buf[2 * side + 1]);
+      if (launched()) return -3;
+      keys = buf[2 * side];
+      idx = buf[2 * side + 1];
+      side ^= 1;
+    }
   }
-  const bool vec = D % 4 == 0 && lddx % 4 == 0 && al(dx, dx_bf16 ? 8 : 16) && al(dw, dw_bf16 ? 8 : 16);
-  const int cols = vec ? D / 4 : D;
-  const int threads = std::min(kThreads, (cols + 31) / 32 * 32);
-  const dim3 grid(chunks, (cols + threads - 1) / threads);
+  float* partial = (float*)take(8LL * chunks * D);
   by_type(dw_bf16, dx_bf16, [&](auto* tw, auto* tx) {
     using TW = std::remove_pointer_t<decltype(tw)>;
     using TX = std::remove_pointer_t<decltype(tx)>;
     auto go = [&](auto v) {
       constexpr int VEC = decltype(v)::value;
-      run_sums_kernel<TX, TW, VEC><<<grid, threads, 0, s>>>(keys, idx, (const TX*)dx, lddx, (TW*)dw, partial, N, V, D,
-                                                            scale, add);
-      join_kernel<TW, VEC><<<grid, threads, 0, s>>>(keys, partial, (TW*)dw, N, V, D, scale, add);
+      const int cols = (D + VEC - 1) / VEC;
+      const int threads = std::min(kThreads, (cols + 31) / 32 * 32);
+      const dim3 grid(chunks, (cols + threads - 1) / threads);
+      if (grid.y > 65535) { rc = -1; return; }
+      if (pdl_launch(run_sums_kernel<TX, TW, VEC>, grid, dim3(threads), 0, s, keys, idx, (const TX*)dx, lddx, (TW*)dw,
+                     partial, N, V, D, scale, add) != cudaSuccess ||
+          pdl_launch(join_kernel<TW, VEC>, grid, dim3(threads), 0, s, keys, (const float*)partial, (TW*)dw, N, V, D, scale,
+                     add) != cudaSuccess)
+        rc = -3;
     };
-    if (vec) go(std::integral_constant<int, 4>{});
+    const bool wide = dx_bf16 && D % 8 == 0 && lddx % 8 == 0 && al(dx, 16) && al(dw, 16);
+    if (wide) go(std::integral_constant<int, 8>{});
+    else if (D % 4 == 0 && lddx % 4 == 0 && al(dx, dx_bf16 ? 8 : 16) && al(dw, dw_bf16 ? 8 : 16))
+      go(std::integral_constant<int, 4>{});
     else go(std::integral_constant<int, 1>{});
   });
-  return launched();
+  return rc;
 }

@@ -4,6 +4,8 @@
 
 namespace pcb {
 
+constexpr int kVocabMaxEntries = 256;   // teacher entries per row
+
 // Loss of the vocabulary head: softmax cross entropy, or distillation from a list of teacher logits per row.
 struct VocabHeadArgs {
   const void* x;        // [N, D] bf16, row stride ldx
@@ -25,14 +27,14 @@ struct VocabHeadArgs {
   int K;                // entries per row (1 for cross entropy)
   float temperature;
   float* loss;          // [N] row losses
-  float* scalars;       // [2]: sum or mean of the row losses, 1 / counted rows
+  float* scalars;       // [2]: sum or mean of the row losses, 1 / counted rows (nullptr: not wanted)
 };
 
 // Where the forward keeps what the backward reads: byte offsets into one buffer.
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;
-  long long count;   // int [4]: counted rows
+  long long count;   // int [4]: counted rows, finished blocks of the loss kernel
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
   long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature
