@@ -381,7 +381,7 @@ at::Tensor flat(const at::Tensor& t) { return t.is_contiguous() ? t : t.contiguo
 
 // What a loss of the vocabulary head keeps for its gradients.
 struct HeadState {
-  at::Tensor saved, scalars, w;
+  at::Tensor saved, scalars, x, w;
   std::vector<int64_t> lead;
   int64_t N, V, D, K;
   bool distill, mean, none;
@@ -420,6 +420,7 @@ std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x,
   if (st.N == 0) return {st.none ? at::zeros(st.lead, f32) : at::zeros({}, f32), st};
   pcb::VocabHeadArgs a{};
   const at::Tensor x2 = as_rows(x);
+  st.x = x2;
   at::Tensor t1, i2, l2;
   a.x = x2.data_ptr();
   a.ldx = rows_apart(x2);
@@ -529,6 +530,8 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     return {dx, dw};
   }
   if (!dx && !dw) return {dx, dw};
+  a.x = st.x.data_ptr();
+  a.ldx = rows_apart(st.x);
   a.w = st.w.data_ptr();
   a.ldw = rows_apart(st.w);
   a.N = st.N;
@@ -551,14 +554,16 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     a.lddw = rows_apart(*dw);
   }
   a.dw_add = accumulate;
-  pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), num_sms(), &a.piece, &a.splits);
-  const int pieces = (a.V + a.piece - 1) / a.piece;
+  a.plan = pcb::vocab_plan(a.N, a.V, a.D, dx.has_value(), dw.has_value(), (int)std::min<int64_t>(piece, 1 << 30), num_sms());
   a.ld_slab = (a.D + 3) / 4 * 4;
-  const int64_t gbytes = (st.N * a.piece * 2 + 255) / 256 * 256;
-  at::Tensor ws = at::empty({gbytes + (dx ? 4 * a.splits * st.N * a.ld_slab : 0)}, st.saved.options());
+  const int64_t gbytes = (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
+  const int64_t dx_slab = (int64_t)a.plan.dx_splits * st.N * a.ld_slab;
+  const int64_t dw_slab = a.plan.dw_splits > 1 ? (int64_t)a.plan.dw_splits * st.V * a.ld_slab : 0;
+  at::Tensor ws = at::empty({gbytes + 4 * (dx_slab + dw_slab)}, st.saved.options());
   a.g = ws.data_ptr();
-  a.slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", pieces * (1 + (dx ? 1 : 0) + (dw ? 1 : 0)) + (dx ? 1 : 0));
+  a.dx_slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
+  a.dw_slab = a.dx_slab + dx_slab;
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", 2 * a.plan.pieces + (dx || dw_slab ? 1 : 0));
   return {dx, dw};
 }
 
@@ -1248,6 +1253,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("skinny_qkv_rope", &skinny_qkv_rope);
   py::class_<HeadState>(m, "HeadState")
       .def_readonly("saved", &HeadState::saved)
+      .def_readonly("x", &HeadState::x)
       .def_readonly("w", &HeadState::w)
       .def_readonly("lead", &HeadState::lead)
       .def_readonly("N", &HeadState::N)

@@ -20,7 +20,6 @@
 #include <mutex>
 
 #include "gemm_epilogue.cuh"
-#include "vocab_epilogue.cuh"
 
 namespace pcb {
 namespace pair {
@@ -58,7 +57,7 @@ struct Cfg {
   // SwiGLU backward), 4 KB for the [32 x 32] fp32 transpose scratch of the coalesced path
   static constexpr bool kTwoBoxes =
       EPI == EPI_BF16 || EPI == EPI_SWIGLU || EPI == EPI_RESID_F32 || EPI == EPI_SWIGLU_BWD || EPI == EPI_GELU_BWD ||
-      EPI == EPI_GELU || EPI == EPI_VH_GRAD || EPI == EPI_VH_DW;
+      EPI == EPI_GELU;
   static constexpr int EPI_WARP_BYTES = kTwoBoxes ? 8192 : 4096;
   // the deepest operand ring that fits: 227 KB - 1 KB (barriers, alignment gap) - staging - 1 KB slack
   static constexpr int STAGES_FIT = (232448 - 2048 - 8 * EPI_WARP_BYTES) / STAGE_BYTES;
@@ -204,9 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool leader = rank == 0;
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
-  int num_m = (args.M + 2 * kBM - 1) / (2 * kBM);
+  const int num_m = (args.M + 2 * kBM - 1) / (2 * kBM);
   const int num_n = (args.N + BN - 1) / BN;
-  int total_kb = (args.K + kBK - 1) / kBK;
+  const int total_kb = (args.K + kBK - 1) / kBK;
+  const int tiles = num_m * num_n * args.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if ((EPI == EPI_BF16 || EPI == EPI_SWIGLU || EPI == EPI_GELU) && args.c_tma) prefetch_tmap(&tmC);
     if ((EPI == EPI_SWIGLU || EPI == EPI_GELU || aux_tma<EPI>()) && args.c_tma) prefetch_tmap(&tmD);
     if (aux_tma<EPI>() && args.c_tma) prefetch_tmap(&tmC);
-    if ((EPI == EPI_VH_GRAD || EPI == EPI_VH_DW) && args.c_tma) prefetch_tmap(&tmC);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
@@ -244,16 +243,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // waits the same way before touching memory). Both are no-ops when the launch is not programmatic.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // vocabulary head: the number of packed rows is known on the device only (at least one tile runs, so that the
-  // gradients of a batch without counted rows are written as zeros)
-  int vh_rows = 0;
-  if (epi_vocab<EPI>()) {
-    vh_rows = min(*args.vh.count, EPI == EPI_VH_DW ? args.K : args.M);
-    const int r = max(vh_rows, 1);
-    if (EPI == EPI_VH_DW) total_kb = (r + kBK - 1) / kBK;
-    else num_m = (r + 2 * kBM - 1) / (2 * kBM);
-  }
-  const int tiles = num_m * num_n * args.splits;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -392,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int store_box = 0;      // bf16 TMA-store path: the staging box used next (alternates across tiles too)
     bool aux_ok = true;
     for (int tile = pair_id; tile < tiles && aux_ok; tile += num_pairs) {
-      int split, mb, nb;
-      tile_coords(tile, args, num_m, num_n, split, mb, nb);
+      int split_unused, mb, nb;
+      tile_coords(tile, args, num_m, num_n, split_unused, mb, nb);
       long long boff = 0;   // grouped, mode 1: this expert's bias block
       if (args.grp_mode) {
         int e, g0, g1;
@@ -423,101 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         aux_request(0, 0);
         if (BN / 64 > 1) aux_request(1, 1);
       }
-      VocabRow vr;   // vocabulary head: what this thread's row needs, fetched while the accumulator fills
-      if (EPI == EPI_VH_STAT || EPI == EPI_VH_GRAD) vr.template fetch<EPI>(args.vh, m, n0 + half * 128, vh_rows);
       PAIR_STAT_T0(st_w2);
       if (!mbar_wait(&tfull[acc], acc_phase, args.err, kErrTimeoutTmemFull, abort_flag)) break;
       PAIR_STAT_ADD(st_tfull, st_w2);
       PAIR_STAT_T0(st_b);
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      if (EPI == EPI_VH_STAT) {
-        vocab_stat(args, vr, tbase + half * 128, m, n0 + half * 128);
-      } else if (EPI == EPI_VH_GRAD) {
-        // two blocks of 64 columns per warp: softmax minus the targets, staged as a 128-byte-swizzled [32 x 64]
-        // bf16 box and written by one TMA store; the two boxes of a warp alternate
-        uint8_t* stg = smem + C::EPI_OFF + (warp - 2) * C::EPI_WARP_BYTES;
-        const int row0 = mb * 2 * kBM + rank * kBM + q * 32;
-#pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
-          const int nb0 = n0 + half * 128 + b * 64;
-          uint32_t pk[32];
-          vocab_grad64(args, vr, tbase + half * 128 + b * 64, nb0, pk);
-          if (row0 >= args.M || nb0 >= args.N) continue;   // nothing of the box inside C (warp-uniform)
-          uint8_t* box = stg + store_box * 4096;
-          store_box ^= 1;
-          if (lane == 0) bulk_group_wait_read<1>();   // the store that last read this box is done with it
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmC, box, nb0, row0);
-            bulk_group_commit();
-          }
-        }
-      } else if (EPI == EPI_VH_DW && args.c_tma) {
-        // bf16 gradient of the weights: the 64-column blocks of the bf16 output path, scaled by device scalars
-        uint8_t* stg = smem + C::EPI_OFF + (warp - 2) * C::EPI_WARP_BYTES;
-        const int row0 = mb * 2 * kBM + rank * kBM + q * 32;
-        const float alpha = vocab_scale(args);
-#pragma unroll 1
-        for (int c2 = half; c2 < BN / 64; c2 += 2) {
-          const int nb0 = n0 + c2 * 64;
-          uint32_t r0[32], r1[32], pk[32];
-          tmem_ld_32x32b_x32(tbase + c2 * 64, r0);
-          tmem_ld_32x32b_x32(tbase + c2 * 64 + 32, r1);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            pk[j] = pack_bf16x2(alpha * __uint_as_float(r0[2 * j]), alpha * __uint_as_float(r0[2 * j + 1]));
-            pk[16 + j] = pack_bf16x2(alpha * __uint_as_float(r1[2 * j]), alpha * __uint_as_float(r1[2 * j + 1]));
-          }
-          if (row0 >= args.M || nb0 >= args.N) continue;   // nothing of the box inside C (warp-uniform)
-          uint8_t* box = stg + store_box * 4096;
-          store_box ^= 1;
-          if (lane == 0) bulk_group_wait_read<1>();
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmC, box, nb0, row0);
-            bulk_group_commit();
-          }
-        }
-      } else if (EPI == EPI_VH_DX || EPI == EPI_VH_DW) {
-        // fp32 slabs of dx, and the gradients of the weights that no TMA store takes: each 32x32 chunk goes
-        // through this warp's scratch (16-byte cells, XOR-swizzled by row), then 8 lanes write one row segment
-        float4* scr = reinterpret_cast<float4*>(smem + C::EPI_OFF + (warp - 2) * C::EPI_WARP_BYTES);
-        const int row0 = mb * 2 * kBM + rank * kBM + q * 32;
-        const float alpha = EPI == EPI_VH_DW ? vocab_scale(args) : 1.f;
-        const int rows = EPI == EPI_VH_DX ? vh_rows : args.M;
-#pragma unroll 1
-        for (int c = half; c < BN / 32; c += 2) {
-          float v[32];
-          tmem_load_f32x32(tbase + c * 32, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            scr[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          __syncwarp();
-          const int c4 = lane & 7, ncol = n0 + c * 32 + c4 * 4;
-#pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int rr = it * 4 + (lane >> 3);
-            const float4 x = scr[rr * 8 + (c4 ^ (rr & 7))];
-            const float e[4] = {alpha * x.x, alpha * x.y, alpha * x.z, alpha * x.w};
-            if (row0 + rr < rows) vocab_store4<EPI>(args, split, row0 + rr, ncol, e);
-          }
-          __syncwarp();
-        }
-      } else if (aux_tma<EPI>() && args.c_tma) {
+      if (aux_tma<EPI>() && args.c_tma) {
         // chunk i of this warp = accumulator columns [32 (half + 2 i), +32); input boxes of chunk i go
         // to buffer i & 1 (4 KB: one fp32 box, or the gate and up bf16 boxes of 2 KB); the boxes of
         // chunks 0 and 1 were requested before the accumulator wait, chunk i + 2 is requested as soon as
@@ -929,8 +830,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  if ((EPI == EPI_BF16 || EPI == EPI_SWIGLU || EPI == EPI_GELU || EPI == EPI_VH_GRAD || EPI == EPI_VH_DW ||
-       aux_tma<EPI>()) && args.c_tma && warp >= 2 && lane == 0)
+  if ((EPI == EPI_BF16 || EPI == EPI_SWIGLU || EPI == EPI_GELU || aux_tma<EPI>()) && args.c_tma && warp >= 2 &&
+      lane == 0)
     bulk_group_wait_all();  // every TMA store has landed before the CTA exits
   __syncwarp();
   tc_fence_before();
@@ -1050,15 +951,8 @@ static int dispatch_pair(int epi, const CUtensorMap& ta, const CUtensorMap& tb, 
     case EPI_BF16_ACC: return launch_pair<BN, EPI_BF16_ACC>(ta, tb, tc, td, a, grid, s);
     case EPI_RESID_F32: return launch_pair<BN, EPI_RESID_F32>(ta, tb, tc, td, a, grid, s);
     case EPI_RS_BF16: return launch_pair<BN, EPI_RS_BF16>(ta, tb, tc, td, a, grid, s);
-    case EPI_VH_DX: return launch_pair<BN, EPI_VH_DX>(ta, tb, tc, td, a, grid, s);
-    case EPI_VH_DW: return launch_pair<BN, EPI_VH_DW>(ta, tb, tc, td, a, grid, s);
-    default: break;
+    default: return -2;
   }
-  if constexpr (BN == 256) {   // the 128-column halves of these epilogues are tied to the wide tile
-    if (epi == EPI_VH_STAT) return launch_pair<BN, EPI_VH_STAT>(ta, tb, tc, td, a, grid, s);
-    if (epi == EPI_VH_GRAD) return launch_pair<BN, EPI_VH_GRAD>(ta, tb, tc, td, a, grid, s);
-  }
-  return -2;
 }
 
 }  // namespace pcb
@@ -1081,7 +975,7 @@ int pcb_gemm_pair_launch(const void* A, int a_mn, long long lda, const void* B, 
   const int num_n = (N + bn - 1) / bn;
   const int total_kb = (K + 63) / 64;
   if (splits < 1) splits = 1;
-  if (splits > 1 && epi != EPI_RED_F32 && epi != EPI_VH_DX) return -4;
+  if (splits > 1 && epi != EPI_RED_F32) return -4;
   if (args.ag_world > 1) {
     // fused gather: K-major A spanning all chunks, whole 256-row tiles per chunk, no split-K
     if (a_mn != 0 || lda != K || (K % 8) != 0 || args.ag_rows % 256 != 0 || args.ag_world > 32 ||
@@ -1120,12 +1014,6 @@ int pcb_gemm_pair_launch(const void* A, int a_mn, long long lda, const void* B, 
   args.c_tma = 0;
   const bool c_ok = (reinterpret_cast<uintptr_t>(args.C) & 15) == 0 && (args.ldc % 8) == 0;
   if (epi == EPI_BF16 && c_ok && make_map2(&tc, args.C, N, M, args.ldc, 64, 32)) args.c_tma = 1;
-  if (epi == EPI_VH_GRAD) {   // the gradient block is a workspace with 16-byte rows: always by TMA
-    if (!c_ok || !make_map2(&tc, args.C, N, M, args.ldc, 64, 32)) return -1;
-    args.c_tma = 1;
-  }
-  if (epi == EPI_VH_DW && c_ok && !args.vh.out_f32 && !args.vh.add && make_map2(&tc, args.C, N, M, args.ldc, 64, 32))
-    args.c_tma = 1;
   // SwiGLU forward: pre (C, [M, N]) and act (D, [M, N / 2]) in [32 x 32] boxes with 64-byte swizzle
   if (epi == EPI_SWIGLU && c_ok && args.D != nullptr && (reinterpret_cast<uintptr_t>(args.D) & 15) == 0 &&
       (args.ldd % 8) == 0 && make_map2(&tc, args.C, N, M, args.ldc, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) &&

@@ -20,38 +20,7 @@ enum GemmEpi : int {
   EPI_RESID_F32 = 12,  // C(f32)  = aux(f32) + alpha*acc + bias (residual stream: x_out = x_in + f(x))
   EPI_RS_BF16 = 13,    // reduce-scatter partials: row m goes to owner c = m / rs_rows, slot rs_rank of
                        // owner c's buffer rs_peers[c] ([world * rs_rows, N] bf16, row stride ldc)
-  // vocabulary head (csrc/vocab.cu; CTA-pair kernel only, see VocabHead)
-  EPI_VH_STAT = 14,    // per row and 128 logits: (max, sum of 2^(logit c - max)) and the logits at the row's target ids
-  EPI_VH_GRAD = 15,    // C(bf16) = softmax - target distribution (rows past the count: 0)
-  EPI_VH_DX = 16,      // C(f32) = or += acc, one [M, ldc] slab per K split
-  EPI_VH_DW = 17,      // C(bf16 or f32) = or += alpha * (device scalars) * acc
-  EPI_COUNT = 18,
-};
-
-// Operands of the vocabulary-head epilogues.  The M rows of the logits product are the counted rows of the
-// batch, packed; `row[j]` is packed row j's place in the batch, and everything kept per row (lse, target lists,
-// picked logits) is indexed by that place.
-struct VocabHead {
-  const int* count;       // device: packed rows in use; tiles cover max(1, *count) of the M (or, dW, K) rows
-  const int* row;         // [M]
-  float c;                // log2(e) / temperature: exponents are taken to base 2
-  int v0;                 // first vocabulary id of this launch's columns (a multiple of 256)
-  float2* part;           // STAT: [2 * ceil(V / 256)][ld_part] (max, sum), by packed row
-  long long ld_part;
-  const float* lse;       // GRAD: base-2 log-sum-exp of logit * c
-  // the target distribution: K entries per row, ids ascending.  Without `start` K is 1 (class targets, weight 1)
-  const int* ids;
-  const float* q;         // weights (nullptr: 1)
-  float* z;               // STAT: [rows, K] logits at the ids
-  int K;
-  const unsigned short* start;  // [2 * ceil(V / 256) + 1][ld_start]: first entry with id >= 128 g
-  long long ld_start;
-  // DX / DW
-  const float* scale;     // device scalars multiplied into DW (nullptr: 1)
-  const float* scale2;
-  int add;                // C += instead of C =
-  int out_f32;            // DW: C is fp32
-  long long slab;         // DX: elements between the slabs of two K splits
+  EPI_COUNT = 14,
 };
 
 struct GemmArgs {
@@ -119,7 +88,6 @@ struct GemmArgs {
   int grp_m;
   long long grp_b_off;
   long long grp_bias_off;
-  VocabHead vh;
 };
 
 // Pair-kernel cycle counters (builds with PCB_GEMM_STATS): copies 12 counters to `out` and clears them.
@@ -139,7 +107,3 @@ int pcb_gemm_launch(const void* A, int a_mn, long long lda, const void* B, int b
 // (likewise).  Returns 0 on success, -1 bad operands, -6 bad group description.
 int pcb_gemm_grouped_launch(const void* A, int a_mn, long long lda, const void* B, int b_mn, long long ldb,
                             int epi, pcb::GemmArgs args, int num_sms, cudaStream_t stream);
-
-// CTA-pair launch with a chosen column tile and K split (see gemm2_tcgen05.cu).
-int pcb_gemm_pair_launch(const void* A, int a_mn, long long lda, const void* B, int b_mn, long long ldb, int epi,
-                         pcb::GemmArgs args, int bn, int splits, int num_sms, cudaStream_t stream);

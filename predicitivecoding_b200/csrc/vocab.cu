@@ -5,19 +5,19 @@
 // softmax q of K teacher logits at temperature T):
 //     loss_n = T^2 sum_k q_k (log q_k - log p_k),  p = softmax(l / T)   (T = 1, one target: lse(l) - l_t)
 //     d loss_n / d l = T (p - q),   dx = c (p - q) w,   dw = c (p - q)^T x,   c = T gout / counted rows
-// The logits [N, V] are never kept.  The forward's GEMM epilogue reduces each row's 128 columns to (max, sum) and picks
-// the logits at the targets; the backward makes the logits again, a piece of the vocabulary at a time, and its
-// epilogue turns them into bf16 p - q, which two more GEMMs read: dw of the piece is finished there, dx is
+// The logits [N, V] are never kept.  The forward's product (csrc/vocab_gemm.cu) reduces each row's 128 columns to (max,
+// sum) and picks the logits at the targets; the backward makes the logits again, a piece of the vocabulary at a
+// time, and turns them into bf16 p - q, which two more products read: dw of the piece is finished there, dx is
 // accumulated over the pieces in fp32.  8 N V D operations instead of 6, for N * piece * 2 bytes of workspace.
 // Rows without a target (masked prompts, padding) are taken out first: the counted rows are packed in order,
-// every GEMM runs over their number, known on the device only, and what stands in the other rows (NaN too) is
-// never read.
+// the products run over their number, known on the device only, and what stands in the other rows (NaN too) is
+// never read.  When all rows are counted the products read x itself.
 #include <algorithm>
 #include <cstdio>
 
 #include "common.cuh"
-#include "gemm_api.h"
 #include "vocab_api.h"
+#include "vocab_gemm.cuh"
 
 namespace pcb {
 namespace vocab {
@@ -94,68 +94,106 @@ PCB_DEVICE void store_vec(T* p, const float (&v)[VEC]) {
 }
 
 // ---------------------------------------------------------------- packing
-// Packs the counted rows in order.  Block b owns rows [b R, (b + 1) R) and counts the rows before them by itself, so
-// that one launch does it without a scan over the blocks (8 bytes a row from L2, against 2 D a row copied).
-__global__ void __launch_bounds__(kThreads)
-    pack_rows_kernel(const void* __restrict__ tgt, int tgt64, long long ignore, const int* __restrict__ len, int V,
-                     const __nv_bfloat16* __restrict__ x, long long ldx, int N, int D, int R, int vec,
-                     __nv_bfloat16* __restrict__ xc, long long ldxc, int* __restrict__ row, int* __restrict__ pos,
-                     int* __restrict__ tgt32, int* __restrict__ count) {
+struct PackArgs {
+  const void* tgt;       // class targets, or
+  int tgt64;
+  long long ignore;
+  const int* len;        // entries of each row's target list
+  int V, N, D;
+  const __nv_bfloat16* x;
+  long long ldx;
+  int vec;               // x in 16-byte vectors
+  int in_place;          // x may be read in place when every row is counted
+  const int* counts;     // counted rows of every kCountRows (nullptr: each block counts for itself)
+  __nv_bfloat16* xc;
+  long long ldxc;
+  int *row, *pos, *tgt32, *count;
+  float* loss;
+};
+constexpr int kCountRows = kThreads;
+constexpr int kSelfCountRows = 8192;   // longer batches are counted by a launch of their own
+
+PCB_DEVICE bool counted(const PackArgs& a, int n) {
+  if (a.len != nullptr) return a.len[n] > 0;
+  const long long t = load_id(a.tgt, a.tgt64, n);
+  return t >= 0 && t < a.V && t != a.ignore;
+}
+
+__global__ void __launch_bounds__(kCountRows) count_rows_kernel(PackArgs a, int* __restrict__ counts) {
+  pdl_begin();
+  const int n = blockIdx.x * kCountRows + threadIdx.x;
+  const int c = __syncthreads_count(n < a.N && counted(a, n));
+  if (threadIdx.x == 0) counts[blockIdx.x] = c;
+}
+
+// Packs the counted rows in order; block b owns rows [b R, (b + 1) R).  In a short batch each block counts the rows
+// before and behind its own by itself (8 bytes a row from L2 against 2 D a row copied), which saves a launch.
+__global__ void __launch_bounds__(kThreads) pack_rows_kernel(PackArgs a, int R) {
   __shared__ int sums[kThreads / 32];
   __shared__ int src[kThreads];
   pdl_begin();
-  auto counted = [&](int n) -> bool {
-    if (len != nullptr) return len[n] > 0;
-    const long long t = load_id(tgt, tgt64, n);
-    return t >= 0 && t < V && t != ignore;
-  };
   auto zero_or_copy = [&](int n, long long j) {   // one warp: packed row j from row n, or zeros (n < 0)
     const int lane = threadIdx.x & 31;
-    __nv_bfloat16* d = xc + j * ldxc;
-    if (vec) {
-      const uint4* s = reinterpret_cast<const uint4*>(x + (long long)max(n, 0) * ldx);
-      const int nv = (int)(ldxc / 8);
+    __nv_bfloat16* d = a.xc + j * a.ldxc;
+    const __nv_bfloat16* s = a.x + (long long)max(n, 0) * a.ldx;
+    if (a.vec) {
+      const int nv = (int)(a.ldxc / 8);
       for (int i0 = lane; i0 < nv; i0 += 128) {
         uint4 r[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) r[u] = n >= 0 && i0 + 32 * u < nv ? s[i0 + 32 * u] : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < 4; ++u)
+          r[u] = n >= 0 && i0 + 32 * u < nv ? reinterpret_cast<const uint4*>(s)[i0 + 32 * u] : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           if (i0 + 32 * u < nv) reinterpret_cast<uint4*>(d)[i0 + 32 * u] = r[u];
       }
     } else {
-      const __nv_bfloat16* s = x + (long long)max(n, 0) * ldx;
-      for (int i = lane; i < (int)ldxc; i += 32) d[i] = n >= 0 && i < D ? s[i] : __float2bfloat16_rn(0.f);
+      for (int i = lane; i < (int)a.ldxc; i += 32) d[i] = n >= 0 && i < a.D ? s[i] : __float2bfloat16_rn(0.f);
     }
   };
-  const int r0 = (int)min((long long)N, (long long)blockIdx.x * R), r1 = (int)min((long long)N, (long long)r0 + R);
-  int before = 0;
-  for (int n = threadIdx.x; n < r0; n += kThreads) before += counted(n) ? 1 : 0;
-  int base;
-  block_scan(before, sums, &base);
-  for (int t0 = r0; t0 < r1; t0 += kThreads) {
-    const int n = t0 + threadIdx.x;
-    const bool c = n < r1 && counted(n);
-    int total;
-    const int k = block_scan(c ? 1 : 0, sums, &total);
-    if (n < r1) {
-      pos[n] = c ? base + k : -1;
-      if (tgt32 != nullptr) tgt32[n] = c ? (int)load_id(tgt, tgt64, n) : -1;
+  const int r0 = (int)min((long long)a.N, (long long)blockIdx.x * R), r1 = (int)min((long long)a.N, (long long)r0 + R);
+  int before = 0, others = 0;   // counted rows in front of this block's, and in all other blocks
+  if (a.counts != nullptr) {
+    const int blocks = (a.N + kCountRows - 1) / kCountRows;   // R is kCountRows
+    for (int i = threadIdx.x; i < blocks; i += kThreads) {
+      const int c = a.counts[i];
+      if (i < (int)blockIdx.x) before += c;
+      if (i != (int)blockIdx.x) others += c;
     }
-    if (c) {
-      row[base + k] = n;
-      src[k] = n;
+  } else {
+    for (int n = threadIdx.x; n < a.N; n += kThreads) {
+      if (n >= r0 && n < r1) continue;
+      const int c = counted(a, n) ? 1 : 0;
+      if (n < r0) before += c;
+      others += c;
     }
-    __syncthreads();
-    for (int i = threadIdx.x >> 5; i < total; i += kThreads / 32) zero_or_copy(src[i], base + i);
-    base += total;
   }
+  int base, rest;
+  block_scan(before, sums, &base);
+  block_scan(others, sums, &rest);
+  const int n = r0 + threadIdx.x;   // R is at most kThreads
+  const bool c = n < r1 && counted(a, n);
+  int total;
+  const int k = block_scan(c ? 1 : 0, sums, &total);
+  if (n < r1) {
+    a.pos[n] = c ? base + k : -1;
+    if (a.tgt32 != nullptr) a.tgt32[n] = c ? (int)load_id(a.tgt, a.tgt64, n) : -1;
+    if (!c) a.loss[n] = 0.f;
+  }
+  if (c) {
+    a.row[base + k] = n;
+    src[k] = n;
+  }
+  __syncthreads();
+  if (!(a.in_place && rest + total == a.N))
+    for (int i = threadIdx.x >> 5; i < total; i += kThreads / 32) zero_or_copy(src[i], base + i);
+  base += total;
   if (blockIdx.x == gridDim.x - 1) {
     if (threadIdx.x == 0) {
-      count[0] = base;
-      count[1] = 0;   // blocks of row_loss_kernel that are done
+      a.count[0] = base;
+      a.count[1] = 0;   // blocks of row_loss_kernel that are done
     }
-    const int end = min(N, (max(base, 1) + 63) / 64 * 64);
+    const int end = min(a.N, (max(base, 1) + 63) / 64 * 64);
     for (int j = base + (threadIdx.x >> 5); j < end; j += kThreads / 32) zero_or_copy(-1, j);
   }
 }
@@ -250,7 +288,7 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kLossParts = 32;
 
 __global__ void __launch_bounds__(32 * kLossParts)
-    row_loss_kernel(const float2* __restrict__ part, int granules, long long ld_part, const int* __restrict__ pos,
+    row_loss_kernel(const float2* __restrict__ part, int granules, const int* __restrict__ row,
                     const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
                     const int* __restrict__ len, int N, int K, float c, float factor, float* __restrict__ lse_out,
                     float* loss, int* count, int mean, float* __restrict__ scalars) {
@@ -259,13 +297,14 @@ __global__ void __launch_bounds__(32 * kLossParts)
   __shared__ int last;
   pdl_begin();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int n = blockIdx.x * 32 + tx;
-  const int j = n < N ? pos[n] : -1;
+  const int j = blockIdx.x * 32 + tx;   // packed row
+  const bool live = j < min(count[0], N);
+  const int n = live ? row[j] : 0;
   float m = -INFINITY, s = 0.f;
-  if (j >= 0) {
+  if (live) {
 #pragma unroll 4
     for (int g = ty; g < granules; g += kLossParts) {
-      const float2 p = part[g * ld_part + j];
+      const float2 p = part[(long long)g * N + j];
       const float nm = fmaxf(m, p.x);
       const float ref = nm == -INFINITY ? 0.f : nm;
       s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
@@ -286,11 +325,11 @@ __global__ void __launch_bounds__(32 * kLossParts)
   const float lse = sm[0][tx];
   // sum_k q_k (log2 q_k + lse - c z_k), term by term: each is a difference of logarithms of the same size
   float l = 0.f;
-  if (j >= 0) {
+  if (live) {
     const long long at = (long long)n * K;
     const int e = len != nullptr ? len[n] : 1;
     for (int k = ty; k < e; k += kLossParts) {
-      const float d = fmaf(-c, z[at + k], lse);
+      const float d = fmaf(-c, z[(long long)j * K + k], lse);
       if (q == nullptr) l += d;
       else if (q[at + k] != 0.f) l += q[at + k] * (lq[at + k] + d);   // 0 log 0 = 0
     }
@@ -300,9 +339,9 @@ __global__ void __launch_bounds__(32 * kLossParts)
   const float sum = warp_sum(sl[tx][ty]);
   if (tx == 0) sl[0][ty] = sum;   // read by this warp only
   __syncthreads();
-  if (ty == 0 && n < N) {
-    loss[n] = j >= 0 ? sl[0][tx] * factor : 0.f;
-    if (j >= 0) lse_out[n] = lse;
+  if (ty == 0 && live) {
+    loss[n] = sl[0][tx] * factor;
+    lse_out[j] = lse;
   }
   if (scalars == nullptr) return;
   __threadfence();
@@ -329,44 +368,72 @@ __global__ void __launch_bounds__(32 * kLossParts)
   }
 }
 
-// dx of every row from the packed slabs: their sum in slab order, times the gradient's factor; zero where the row
-// is not counted.  A warp per row and slice of columns.
+// Gradients from their fp32 slabs: the sum in slab order, times the gradient's factor.  The first N rows are dx's, found
+// by their packed place, zero where the row is not counted; the others dw's, when it was split.  A warp per row
+// and slice of columns.
 constexpr int kFinishVecs = 4;
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads)
-    finish_dx_kernel(const float* __restrict__ slab, long long slab_stride, int slabs, long long ld,
-                     const int* __restrict__ pos, T* __restrict__ dx, long long lddx, int N, int D, float alpha,
-                     const float* __restrict__ scale, const float* __restrict__ scale2) {
+struct FinishArgs {
+  const float* dx_slab;
+  const float* dw_slab;
+  int dx_splits, dw_splits;
+  const int* pos;
+  void *dx, *dw;
+  long long ld_slab, lddx, lddw;
+  int dx_f32, dw_f32, dw_add;
+  int N, V, D;           // N = 0 where dx is not wanted, V = 0 where dw is not in slabs
+  float alpha;
+  const float* scale;
+  const float* scale2;
+};
+
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a, int nrows) {
   pdl_begin();
-  const int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (n >= N) return;
-  const int j = pos[n];
-  float a = alpha;
-  if (scale != nullptr) a *= *scale;
-  if (scale2 != nullptr) a *= *scale2;
+  int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (n >= a.N + a.V) return;
+  const bool w = n >= a.N;
+  if (w) n -= a.N;
+  const int j = w ? n : a.pos[n];
+  float f = a.alpha;
+  if (a.scale != nullptr) f *= *a.scale;
+  if (a.scale2 != nullptr) f *= *a.scale2;
   const int d0 = (blockIdx.y * kFinishVecs * 32 + (threadIdx.x & 31)) * VEC;
-  const float* src = slab + (long long)max(j, 0) * ld + d0;
+  const float* src = (w ? a.dw_slab : a.dx_slab) + (long long)max(j, 0) * a.ld_slab + d0;
+  const long long stride = (w ? (long long)a.V : (long long)nrows) * a.ld_slab;
+  const int slabs = w ? a.dw_splits : a.dx_splits;
   float v[kFinishVecs][VEC] = {};
   if (j >= 0) {
-    for (int k = 0; k < slabs; ++k, src += slab_stride) {
+    for (int k = 0; k < slabs; ++k, src += stride) {
       float r[kFinishVecs][VEC];
 #pragma unroll
       for (int i = 0; i < kFinishVecs; ++i)
-        if (d0 + i * 32 * VEC < D) load_vec<float, VEC>(src + i * 32 * VEC, r[i]);
+        if (d0 + i * 32 * VEC < a.D) load_vec<float, VEC>(src + i * 32 * VEC, r[i]);
 #pragma unroll
       for (int i = 0; i < kFinishVecs; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (d0 + i * 32 * VEC < D) v[i][e] += r[i][e];
+          if (d0 + i * 32 * VEC < a.D) v[i][e] += r[i][e];
     }
   }
-  T* o = dx + n * lddx + d0;
+  const bool f32 = w ? a.dw_f32 : a.dx_f32;
+  const long long at = n * (w ? a.lddw : a.lddx) + d0;
+  float* of = (float*)(w ? a.dw : a.dx) + at;
+  __nv_bfloat16* oh = (__nv_bfloat16*)(w ? a.dw : a.dx) + at;
 #pragma unroll
   for (int i = 0; i < kFinishVecs; ++i) {
+    if (d0 + i * 32 * VEC >= a.D) break;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[i][e] = j >= 0 ? a * v[i][e] : 0.f;
-    if (d0 + i * 32 * VEC < D) store_vec<T, VEC>(o + i * 32 * VEC, v[i]);
+    for (int e = 0; e < VEC; ++e) v[i][e] = j >= 0 ? f * v[i][e] : 0.f;
+    if (w && a.dw_add) {
+      float p[VEC];
+      if (f32) load_vec<float, VEC>(of + i * 32 * VEC, p);
+      else load_vec<__nv_bfloat16, VEC>(oh + i * 32 * VEC, p);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i][e] += p[e];
+    }
+    if (f32) store_vec<float, VEC>(of + i * 32 * VEC, v[i]);
+    else store_vec<__nv_bfloat16, VEC>(oh + i * 32 * VEC, v[i]);
   }
 }
 
@@ -770,31 +837,55 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
   return l;
 }
 
-static long long tiles_cost(long long tiles, int slots, long long kb) {
-  // waves of the persistent grid, each as long as its k-blocks and a fixed part for prologue and epilogue
-  return (tiles + slots - 1) / slots * (kb + 8);
+// Splits of the two gradient products.  A tile costs its k-blocks and about 8 more for what the next tile's products do
+// not hide; the pairs of SMs walk the list of dw's tiles, then dx's, in turn, so the longest walk is one of a few
+// pairs.  Slabs cost their bytes, written and read once: a k-block of a 256-column tile takes the time of about 2.4 MB.
+static double walk(long long t1, double c1, long long t2, double c2, long long pairs) {
+  double most = 0;
+  const long long at[4] = {0, t1 % pairs, (t1 + t2) % pairs - 1, t1 % pairs - 1};
+  for (long long p : at) {
+    if (p < 0) p = pairs - 1;
+    const long long n1 = t1 > p ? (t1 - p + pairs - 1) / pairs : 0;
+    const long long n = t1 + t2 > p ? (t1 + t2 - p + pairs - 1) / pairs : 0;
+    most = std::max(most, n1 * c1 + (n - n1) * c2);
+  }
+  return most;
 }
 
-void vocab_plan(int N, int V, int D, int want_piece, int num_sms, int* piece, int* splits) {
+long long vocab_g_rows(int N) { return (N + 255LL) / 256 * 256 + kTwoTermRows; }
+
+VocabPlan vocab_plan(int N, int V, int D, bool dx, bool dw, int want_piece, int num_sms) {
+  VocabPlan r{};
   const long long all = (V + 255LL) / 256 * 256;
   long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2LL * N) / 256 * 256;
   p = std::max(256LL, std::min(p, all));
-  const long long pieces = (all + p - 1) / p;
-  p = (all / 256 + pieces - 1) / pieces * 256;   // pieces of one size
-  *piece = (int)p;
-  const int bn = D >= 256 ? 256 : 128;
-  const long long tiles = ((N + 255LL) / 256) * ((D + bn - 1) / bn), kb = (std::min<long long>(p, V) + 63) / 64;
-  int best = 1;
-  long long cost = -1;
-  for (int s = 1; s <= 16 && kb / s >= 4; ++s) {
-    const long long c = tiles_cost(tiles * s, num_sms / 2, (kb + s - 1) / s);
-    if (cost < 0 || c < cost) {
-      cost = c;
-      best = s;
+  r.pieces = (int)((all + p - 1) / p);
+  p = (all / 256 + r.pieces - 1) / r.pieces * 256;   // pieces of one size
+  r.piece = (int)p;
+  r.pieces = (int)((all + p - 1) / p);
+  const int bn = head_bn(D);
+  const long long num_n = (D + bn - 1) / bn, pairs = std::max(1, num_sms / 2);
+  const long long dw_tiles = (p / 256) * num_n, dx_tiles = ((N + 255LL) / 256) * num_n;
+  const double k = bn / 256.0, two = N <= kTwoTermRows ? 2.0 : 1.0;
+  const double kb_dw = two * k * ((N + 63) / 64), kb_dx = two * k * ((std::min<long long>(p, V) + 63) / 64);
+  // as if both were wanted, so that a gradient is the same with and without the other
+  double best = -1;
+  for (int s1 = 1; s1 <= (r.pieces == 1 ? 8 : 1); s1 *= 2) {
+    if (s1 > 1 && kb_dw < 4 * s1) break;
+    for (int s2 = 1; s2 <= 16; s2 += s2 < 4 ? 1 : s2 < 8 ? 2 : 4) {
+      if (s2 > 1 && kb_dx < 4 * s2) break;
+      const double slabs = 8.0 * D * ((s1 > 1 ? (double)s1 * p : 0.0) + (double)s2 * N) / 2.4e6;
+      const double c = walk(dw_tiles * s1, kb_dw / s1 + 8 * k, dx_tiles * s2, kb_dx / s2 + 8 * k, pairs) + slabs;
+      if (best < 0 || c < best) {
+        best = c;
+        r.dw_splits = s1;
+        r.dx_splits = s2;
+      }
     }
   }
-  const long long kbps = (kb + best - 1) / best;
-  *splits = (int)((kb + kbps - 1) / kbps);
+  if (!dw) r.dw_splits = 0;
+  if (!dx) r.dx_splits = 0;
+  return r;
 }
 
 }  // namespace pcb
@@ -811,139 +902,144 @@ int pcb_vocab_pad_rows(const void* src, long long ld, void* dst, long long ldd, 
 
 static char* at(void* base, long long off) { return (char*)base + off; }
 
+// whether the products may read x itself: rows that a tensor map can describe
+static bool readable(const void* x, long long ldx, int D) {
+  return D % 8 == 0 && ldx % 8 == 0 && ldx >= D && al(x, 16);
+}
+
 int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s) {
   const bool distill = a.tgt == nullptr;
   if (a.N < 1 || a.V < 1 || a.D < 1 || a.K < 1 || a.K > kMaxK) return -1;
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, distill);
-  int* count = (int*)at(saved, l.count);
-  int *row = (int*)at(saved, l.row), *pos = (int*)at(saved, l.pos), *ids = (int*)at(saved, l.ids);
+  int *row = (int*)at(saved, l.row), *ids = (int*)at(saved, l.ids), *count = (int*)at(saved, l.count);
   float *lse = (float*)at(saved, l.lse), *z = (float*)at(saved, l.z);
   float *q = distill ? (float*)at(saved, l.q) : nullptr, *lq = distill ? (float*)at(saved, l.lq) : nullptr;
   int* len = distill ? (int*)at(saved, l.len) : nullptr;
   unsigned short* start = distill ? (unsigned short*)at(saved, l.start) : nullptr;
-  __nv_bfloat16* xc = (__nv_bfloat16*)at(saved, l.xc);
   const float T = distill ? a.temperature : 1.f;
   const float c = 1.4426950408889634f / T;
   if (distill &&
       pdl_launch(sort_targets_kernel, dim3((a.N + 7) / 8), dim3(kThreads), 0, s, a.ids, a.ids64, a.ld_ids, a.logits,
                  a.logits_bf16, a.ld_logits, a.N, a.V, a.K, c, ids, q, lq, len, start, l.granules) != cudaSuccess)
     return -3;
-  const int blocks = std::max(1, std::min(4 * num_sms, (a.N + 7) / 8));
-  const int R = (a.N + blocks - 1) / blocks;
-  const int vec = a.D % 8 == 0 && a.ldx % 8 == 0 && al(a.x, 16);
-  if (pdl_launch(pack_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, a.tgt, a.tgt64, a.ignore, (const int*)len, a.V,
-                 (const __nv_bfloat16*)a.x, a.ldx, a.N, a.D, R, vec, xc, l.ldxc, row, pos, distill ? nullptr : ids,
-                 count) != cudaSuccess)
-    return -3;
-  GemmArgs g{};
-  g.M = a.N;
-  g.N = a.V;
-  g.K = a.D;
-  g.alpha = 1.f;
-  g.vh.count = count;
-  g.vh.row = row;
-  g.vh.c = c;
-  g.vh.part = (float2*)part;
-  g.vh.ld_part = a.N;
-  g.vh.ids = ids;
-  g.vh.z = z;
-  g.vh.K = a.K;
-  g.vh.start = start;
-  g.vh.ld_start = a.N;
-  int rc = pcb_gemm_pair_launch(xc, 0, l.ldxc, a.w, 0, a.ldw, EPI_VH_STAT, g, 256, 1, num_sms, s);
+  PackArgs p{};
+  p.tgt = a.tgt;
+  p.tgt64 = a.tgt64;
+  p.ignore = a.ignore;
+  p.len = len;
+  p.V = a.V;
+  p.N = a.N;
+  p.D = a.D;
+  p.x = (const __nv_bfloat16*)a.x;
+  p.ldx = a.ldx;
+  p.vec = a.D % 8 == 0 && a.ldx % 8 == 0 && al(a.x, 16);
+  p.in_place = readable(a.x, a.ldx, a.D);
+  p.xc = (__nv_bfloat16*)at(saved, l.xc);
+  p.ldxc = l.ldxc;
+  p.row = row;
+  p.pos = (int*)at(saved, l.pos);
+  p.tgt32 = distill ? nullptr : ids;
+  p.count = count;
+  p.loss = a.loss;
+  int blocks, R;
+  if (a.N > kSelfCountRows) {
+    blocks = (a.N + kCountRows - 1) / kCountRows;
+    R = kCountRows;
+    int* counts = (int*)part;   // the pairs are written later
+    if (pdl_launch(count_rows_kernel, dim3(blocks), dim3(kCountRows), 0, s, p, counts) != cudaSuccess) return -3;
+    p.counts = counts;
+  } else {
+    blocks = std::max(1, std::min(2 * num_sms, (a.N + 7) / 8));   // 64 or more: at most 128 rows each
+    R = (a.N + blocks - 1) / blocks;
+  }
+  if (pdl_launch(pack_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, p, R) != cudaSuccess) return -3;
+  HeadGemm g{};
+  g.N = a.N;
+  g.D = a.D;
+  g.cols = a.V;
+  g.count = count;
+  g.c = c;
+  g.row = row;
+  g.ids = ids;
+  g.K = a.K;
+  g.start = start;
+  g.part = (float2*)part;
+  g.z = z;
+  const int rc = pcb_head_gemm(HEAD_STAT, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, 0, num_sms, s);
   if (rc) return rc;
   return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, l.granules,
-                    (long long)a.N, (const int*)pos, (const float*)z, (const float*)q, (const float*)lq, (const int*)len,
-                    a.N, a.K, c, 0.6931471805599453f * T * T, lse, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+                    (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
+                    0.6931471805599453f * T * T, lse, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
 }
 
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, a.distill != 0);
   void* sv = const_cast<void*>(a.saved);
-  const int* count = (const int*)at(sv, l.count);
-  const int *row = (const int*)at(sv, l.row), *pos = (const int*)at(sv, l.pos);
-  const __nv_bfloat16* xc = (const __nv_bfloat16*)at(sv, l.xc);
-  const float* inv = a.mean ? a.scalars + 1 : nullptr;
+  const void* x_all = readable(a.x, a.ldx, a.D) ? a.x : nullptr;
   const float T = a.distill ? a.temperature : 1.f;
-  const int bnd = a.D >= 256 ? 256 : 128;
-  for (int v0 = 0; v0 < a.V; v0 += a.piece) {
-    const int cols = std::min(a.piece, a.V - v0);
+  HeadGemm g{};
+  g.N = a.N;
+  g.D = a.D;
+  g.count = (const int*)at(sv, l.count);
+  g.c = 1.4426950408889634f / T;
+  g.row = (const int*)at(sv, l.row);
+  g.ids = (const int*)at(sv, l.ids);
+  g.K = a.K;
+  if (a.distill) {
+    g.q = (const float*)at(sv, l.q);
+    g.start = (const unsigned short*)at(sv, l.start);
+  }
+  g.lse = (const float*)at(sv, l.lse);
+  g.g_low = (a.N + 255) / 256 * 256;
+  g.dw_splits = a.plan.dw_splits;
+  g.dx_splits = a.plan.dx_splits;
+  g.lddw = a.lddw;
+  g.dw_f32 = a.dw_f32;
+  g.dw_add = a.dw_add;
+  g.alpha = a.gout * T;
+  g.scale = a.mean ? a.scalars + 1 : nullptr;
+  g.scale2 = a.gout_dev;
+  g.dx_slab = a.dx_slab;
+  g.dw_slab = a.dw_slab;
+  g.ld_slab = a.ld_slab;
+  for (int v0 = 0; v0 < a.V; v0 += a.plan.piece) {
+    g.v0 = v0;
+    g.cols = std::min(a.plan.piece, a.V - v0);
+    g.dx_add = v0 > 0;
+    g.dw = a.dw == nullptr ? nullptr : (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
     const __nv_bfloat16* w = (const __nv_bfloat16*)a.w + (long long)v0 * a.ldw;
-    GemmArgs g{};
-    g.M = a.N;
-    g.N = cols;
-    g.K = a.D;
-    g.alpha = 1.f;
-    g.C = a.g;
-    g.ldc = a.piece;
-    g.vh.count = count;
-    g.vh.row = row;
-    g.vh.c = 1.4426950408889634f / T;
-    g.vh.v0 = v0;
-    g.vh.lse = (const float*)at(sv, l.lse);
-    g.vh.ids = (const int*)at(sv, l.ids);
-    g.vh.K = a.K;
-    if (a.distill) {
-      g.vh.q = (const float*)at(sv, l.q);
-      g.vh.start = (const unsigned short*)at(sv, l.start);
-      g.vh.ld_start = a.N;
-    }
-    int rc = pcb_gemm_pair_launch(xc, 0, l.ldxc, w, 0, a.ldw, EPI_VH_GRAD, g, 256, 1, num_sms, s);
-    if (rc) return rc;
-    if (a.dw != nullptr) {
-      GemmArgs d{};
-      d.M = cols;
-      d.N = a.D;
-      d.K = a.N;
-      d.alpha = a.gout * T;
-      d.C = (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
-      d.ldc = a.lddw;
-      d.vh.count = count;
-      d.vh.scale = inv;
-      d.vh.scale2 = a.gout_dev;
-      d.vh.add = a.dw_add;
-      d.vh.out_f32 = a.dw_f32;
-      rc = pcb_gemm_pair_launch(a.g, 1, a.piece, xc, 1, l.ldxc, EPI_VH_DW, d, bnd, 1, num_sms, s);
-      if (rc) return rc;
-    }
-    if (a.dx != nullptr) {
-      GemmArgs d{};
-      d.M = a.N;
-      d.N = a.D;
-      d.K = cols;
-      d.alpha = 1.f;
-      d.C = a.slab;
-      d.ldc = a.ld_slab;
-      d.vh.count = count;
-      d.vh.add = v0 > 0;
-      d.vh.slab = (long long)a.N * a.ld_slab;
-      // a last piece with fewer k-blocks than the others could leave a split without any: it runs unsplit into slab 0
-      const int kb = (cols + 63) / 64, kbps = (kb + a.splits - 1) / a.splits;
-      const int splits = (kb + kbps - 1) / kbps;
-      rc = pcb_gemm_pair_launch(a.g, 0, a.piece, w, 1, a.ldw, EPI_VH_DX, d, bnd, splits, num_sms, s);
+    for (int mode : {HEAD_GRAD, HEAD_BWD}) {
+      const int rc = pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, a.plan.piece, num_sms, s);
       if (rc) return rc;
     }
   }
-  if (a.dx == nullptr) return 0;
-  const bool v4 = a.D % 4 == 0 && a.lddx % 4 == 0 && al(a.dx, a.dx_f32 ? 16 : 8);
-  const long long stride = (long long)a.N * a.ld_slab;
-  int rc = 0;
-  auto go = [&](auto* dx, auto vec) {
-    using T2 = std::remove_pointer_t<decltype(dx)>;
-    constexpr int VEC = decltype(vec)::value;
-    const dim3 grid((a.N + 7) / 8, ((a.D + VEC - 1) / VEC + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
-    if (grid.y > 65535) { rc = -1; return; }
-    rc = pdl_launch(finish_dx_kernel<T2, VEC>, grid, dim3(kThreads), 0, s, (const float*)a.slab, stride, a.splits,
-                    a.ld_slab, pos, dx, a.lddx, a.N, a.D, a.gout * T, inv, a.gout_dev) == cudaSuccess ? 0 : -3;
-  };
-  if (a.dx_f32) {
-    if (v4) go((float*)a.dx, std::integral_constant<int, 4>{});
-    else go((float*)a.dx, std::integral_constant<int, 1>{});
-  } else {
-    if (v4) go((__nv_bfloat16*)a.dx, std::integral_constant<int, 4>{});
-    else go((__nv_bfloat16*)a.dx, std::integral_constant<int, 1>{});
-  }
-  return rc;
+  FinishArgs f{};
+  f.dx_slab = a.dx_slab;
+  f.dw_slab = a.dw_slab;
+  f.dx_splits = a.plan.dx_splits;
+  f.dw_splits = a.plan.dw_splits;
+  f.pos = (const int*)at(sv, l.pos);
+  f.dx = a.dx;
+  f.dw = a.dw;
+  f.ld_slab = a.ld_slab;
+  f.lddx = a.lddx;
+  f.lddw = a.lddw;
+  f.dx_f32 = a.dx_f32;
+  f.dw_f32 = a.dw_f32;
+  f.dw_add = a.dw_add;
+  f.N = a.dx != nullptr ? a.N : 0;
+  f.V = a.plan.dw_splits > 1 ? a.V : 0;
+  f.D = a.D;
+  f.alpha = g.alpha;
+  f.scale = g.scale;
+  f.scale2 = g.scale2;
+  if (f.N + f.V == 0) return 0;
+  const bool v4 = a.D % 4 == 0 && (f.N == 0 || (a.lddx % 4 == 0 && al(a.dx, a.dx_f32 ? 16 : 8))) &&
+                  (f.V == 0 || (a.lddw % 4 == 0 && al(a.dw, a.dw_f32 ? 16 : 8)));
+  const int vecs = v4 ? a.D / 4 : a.D;
+  const dim3 grid((f.N + f.V + 7) / 8, (vecs + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
+  if (grid.y > 65535) return -1;
+  return pdl_launch(v4 ? finish_kernel<4> : finish_kernel<1>, grid, dim3(kThreads), 0, s, f, a.N) == cudaSuccess ? 0 : -3;
 }
 
 template <typename F>

@@ -49,7 +49,16 @@ struct VocabLayout {
 };
 VocabLayout vocab_layout(int N, int V, int D, int K, bool distill);
 
+// How the backward goes over the vocabulary: columns at a time, and K splits of the two products (0: not wanted).
+struct VocabPlan {
+  int piece, pieces;
+  int dw_splits, dx_splits;
+};
+VocabPlan vocab_plan(int N, int V, int D, bool dx, bool dw, int want_piece, int num_sms);
+
 struct VocabGradArgs {
+  const void* x;         // as the forward read it
+  long long ldx;
   const void* w;
   long long ldw;
   int N, V, D, K;
@@ -67,15 +76,13 @@ struct VocabGradArgs {
   long long lddw;
   int dw_f32;
   int dw_add;
-  int piece;             // columns per piece (a multiple of 256)
-  int splits;            // K splits of dx
-  void* g;               // [N, piece] bf16 workspace
-  float* slab;           // [splits, N, ld_slab] fp32 workspace
+  VocabPlan plan;
+  void* g;               // workspace: bf16 [vocab_g_rows(N), piece]
+  float* dx_slab;        // workspace: [dx_splits, N, ld_slab]
+  float* dw_slab;        // workspace: [dw_splits, V, ld_slab] when dw_splits > 1
   long long ld_slab;
 };
-
-// columns of the vocabulary handled at a time, and K splits of the dx product
-void vocab_plan(int N, int V, int D, int want_piece, int num_sms, int* piece, int* splits);
+long long vocab_g_rows(int N);
 
 }  // namespace pcb
 

@@ -1,0 +1,618 @@
+// The tensor-core products of the vocabulary head, on CTA pairs (tcgen05 cta_group::2): one 256 x BN tile per pair of
+// SMs, operands by TMA into a ring of shared-memory stages, accumulators double-buffered in TMEM, so that the
+// epilogue of a tile runs under the products of the next.  Persistent: one pair of CTAs per pair of SMs walks the tiles.
+//
+//   STAT, GRAD   logits tile = x w^T; a thread of the epilogue owns one row (a TMEM lane) and 128 of its logits, so
+//                the softmax statistics need no exchange between threads, and the row's few targets in those
+//                columns are met by walking its ascending list
+//   BWD          dw = g^T x (rows = vocabulary, K = counted rows) and dx = g w (rows = counted rows, K = vocabulary)
+//                as one list of tiles: neither product fills whole waves of 74 pairs by itself, the two share g in
+//                L2, and a small batch saves a launch.  K is split where there are few tiles; the parts go to fp32
+//                slabs that are added in order, not through atomics.
+//
+// The number of counted rows is known on the device only; every role derives the same tile list from it.  All waits are
+// bounded.  No load uses cluster multicast.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "common.cuh"
+#include "vocab_gemm.cuh"
+
+namespace pcb {
+namespace head {
+
+constexpr int kBM = 128;   // rows per CTA (256 per pair)
+constexpr int kBK = 64;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+
+template <int MODE, int BN>
+struct Cfg {
+  static constexpr int A_BYTES = kBM * kBK * 2;
+  static constexpr int B_BYTES = (BN / 2) * kBK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN;
+  // per epilogue warp: two [32 x 64] bf16 boxes for TMA stores, of which the fp32 path uses one as scratch
+  static constexpr int EPI_WARP_BYTES = MODE == HEAD_STAT ? 0 : 8192;
+  static constexpr int STAGES_FIT = (232448 - 2048 - kEpiWarps * EPI_WARP_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+  static constexpr int EPI_OFF = STAGES * STAGE_BYTES + 1024;
+  static constexpr int SMEM_BYTES = EPI_OFF + kEpiWarps * EPI_WARP_BYTES + 1024;
+  static_assert(SMEM_BYTES <= 232448, "dynamic shared memory above the 227 KB per-block limit");
+  static_assert(8 * (2 * STAGES + 4) + 8 <= 1024, "barriers do not fit behind the ring");
+};
+
+struct Shape {   // what the number of counted rows makes of a launch
+  int rows;      // counted rows
+  int dw_n, tiles;
+  int num_n;     // column blocks
+  int num_m;     // row blocks (BWD: of dx)
+  int kb_dw, kb_dx;   // k-blocks of the whole contraction (STAT, GRAD: kb_dx)
+  bool two;      // two-term g
+};
+
+struct Tile {
+  bool dw;
+  int mb, nb, split;
+  int kb0, kb1;
+};
+
+template <int MODE, int BN>
+PCB_DEVICE Shape shape_of(const HeadGemm& a) {
+  Shape s;
+  s.rows = min(*a.count, a.N);
+  const int r = max(s.rows, 1);   // one tile at least: gradients of a batch without counted rows are zeros
+  s.num_m = (r + 2 * kBM - 1) / (2 * kBM);
+  s.two = MODE != HEAD_STAT && s.rows <= kTwoTermRows;
+  if (MODE == HEAD_BWD) {
+    s.num_n = (a.D + BN - 1) / BN;
+    s.kb_dw = (r + kBK - 1) / kBK;
+    s.kb_dx = (a.cols + kBK - 1) / kBK;
+    s.dw_n = (a.cols + 2 * kBM - 1) / (2 * kBM) * s.num_n * a.dw_splits;
+    s.tiles = s.dw_n + s.num_m * s.num_n * a.dx_splits;
+  } else {
+    s.num_n = (a.cols + BN - 1) / BN;
+    s.kb_dw = 0;
+    s.kb_dx = (a.D + kBK - 1) / kBK;
+    s.dw_n = 0;
+    s.tiles = s.num_m * s.num_n;
+  }
+  return s;
+}
+
+template <int MODE>
+PCB_DEVICE Tile tile_of(const HeadGemm& a, const Shape& s, int t) {
+  Tile r;
+  if (MODE == HEAD_BWD) {
+    r.dw = t < s.dw_n;
+    const int splits = r.dw ? a.dw_splits : a.dx_splits, kb = r.dw ? s.kb_dw : s.kb_dx;
+    if (!r.dw) t -= s.dw_n;
+    r.nb = t % s.num_n;
+    t /= s.num_n;
+    r.split = t % splits;
+    r.mb = t / splits;
+    r.kb0 = (int)((long long)kb * r.split / splits);
+    r.kb1 = (int)((long long)kb * (r.split + 1) / splits);
+    if (s.two) {   // the two terms of g take turns, k-block by k-block
+      r.kb0 *= 2;
+      r.kb1 *= 2;
+    }
+  } else {
+    r.dw = false;
+    r.split = 0;
+    if (a.row_blocks_last) {
+      r.nb = t % s.num_n;
+      r.mb = t / s.num_n;
+    } else {
+      r.mb = t % s.num_m;
+      r.nb = t / s.num_m;
+    }
+    r.kb0 = 0;
+    r.kb1 = s.kb_dx;
+  }
+  return r;
+}
+
+// ---------------------------------------------------------------- epilogues of the logits
+PCB_DEVICE void load32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld_32x32b_x32(taddr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+// v[o] for a run-time o: a tree of selects, since registers have no run-time index
+PCB_DEVICE float pick32(const float (&v)[32], int o) {
+  float a[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a[j] = (o & 16) ? v[16 + j] : v[j];
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1) {
+#pragma unroll
+    for (int j = 0; j < w; ++j) a[j] = (o & w) ? a[w + j] : a[j];
+  }
+  return a[0];
+}
+
+// One packed row's part of the target list: the entries whose ids fall in this thread's 128 columns.
+struct RowTargets {
+  bool live;      // a counted row
+  float lse;
+  long long at;   // entry of the next target, by batch row
+  long long to_z; // add: the same entry by packed row
+  int left;       // entries left in these columns
+  int next;       // column of the next one relative to the first of the 128; past them when none is left
+  int lo;         // vocabulary id of the first of the 128 columns
+
+  template <int MODE>
+  PCB_DEVICE void fetch(const HeadGemm& h, int m, int col0, int rows) {
+    lse = 0.f;
+    at = to_z = 0;
+    left = 0;
+    next = 1 << 30;
+    lo = h.v0 + col0;
+    live = m < rows;
+    if (!live) return;
+    const int n = h.row[m];
+    if (MODE == HEAD_GRAD) lse = h.lse[m];
+    at = (long long)n * h.K;
+    to_z = (long long)(m - n) * h.K;
+    if (h.start != nullptr) {
+      const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
+      const int e = s[0];
+      left = s[h.N] - e;
+      at += e;
+    } else {
+      const int t = h.ids[n] - lo;
+      left = t >= 0 && t < 128 ? 1 : 0;
+    }
+    if (left > 0) next = h.ids[at] - lo;
+  }
+  PCB_DEVICE void advance(const HeadGemm& h) {
+    ++at;
+    next = --left > 0 ? h.ids[at] - lo : 1 << 30;
+  }
+};
+
+// (max, sum 2^(c l - max)) of this thread's 128 logits, in one pass with a running maximum, and the logits at the
+// row's targets.  The maximum stays in units of c l, and the sum is taken against that rounded value, so the
+// log-sum-exp made of the pair carries no error of the product c * max.
+PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int m, int col0) {
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
+    if (nvalid <= 0) break;
+    float v[32];
+    load32(taddr + 32 * i, v);
+    while (r.next < 32 * (i + 1)) {
+      a.z[r.at + r.to_z] = pick32(v, r.next - 32 * i);
+      r.advance(a);
+    }
+    __syncwarp();
+    if (nvalid < 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : -INFINITY;
+    }
+    float cm = v[0];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) cm = fmaxf(cm, v[j]);
+    const float nm = fmaxf(mx, cm * a.c);
+    const float ref = nm == -INFINITY ? 0.f : nm;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      s0 += ex2_approx(fmaf(v[j], a.c, -ref));
+      s1 += ex2_approx(fmaf(v[j + 1], a.c, -ref));
+    }
+    sum = sum * ex2_approx(mx - ref) + (s0 + s1);
+    mx = nm;
+  }
+  if (r.live) a.part[(long long)((a.v0 + col0) >> 7) * a.N + m] = make_float2(mx, sum);
+}
+
+// 32 columns of softmax - target distribution, starting `base` columns into this thread's 128.  The factor 1 / count
+// is applied in fp32 behind the products that read them: rounding a shared factor into every entry would bias all of
+// them alike.
+PCB_DEVICE void grad32(const HeadGemm& a, RowTargets& r, uint32_t taddr, int base, float (&v)[32]) {
+  load32(taddr, v);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = r.live ? ex2_approx(fmaf(v[j], a.c, -r.lse)) : 0.f;
+  while (r.next < base + 32) {
+    const int o = r.next - base;
+    const float q = a.q != nullptr ? a.q[r.at] : 1.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] -= j == o ? q : 0.f;
+    r.advance(a);
+  }
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------- stores
+// a lane's 64 bf16 as its row of the 128-byte-swizzled [32 x 64] box, written by one TMA store; the two boxes of a warp
+// alternate
+PCB_DEVICE void store_box64(const CUtensorMap* map, uint8_t* stg, int& box_at, const uint32_t (&pk)[32], int col, int row,
+                            int lane) {
+  uint8_t* box = stg + box_at * 4096;
+  box_at ^= 1;
+  if (lane == 0) bulk_group_wait_read<1>();   // the store that last read this box is done with it
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map, box, col, row);
+    bulk_group_commit();
+  }
+}
+
+PCB_DEVICE bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+PCB_DEVICE void store4(float* c, float (&o)[4], int nv, bool add) {
+  if (nv == 4 && aligned(c, 16)) {
+    float4* p = reinterpret_cast<float4*>(c);
+    if (add) {
+      const float4 f = *p;
+      o[0] += f.x; o[1] += f.y; o[2] += f.z; o[3] += f.w;
+    }
+    *p = make_float4(o[0], o[1], o[2], o[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < nv) c[j] = add ? c[j] + o[j] : o[j];
+  }
+}
+PCB_DEVICE void store4(__nv_bfloat16* c, float (&o)[4], int nv, bool add) {
+  if (nv == 4 && aligned(c, 8)) {
+    uint2* p = reinterpret_cast<uint2*>(c);
+    if (add) {
+      const uint2 u = *p;
+      o[0] += bf16_lo(u.x); o[1] += bf16_hi(u.x); o[2] += bf16_lo(u.y); o[3] += bf16_hi(u.y);
+    }
+    *p = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < nv) c[j] = __float2bfloat16_rn(add ? __bfloat162float(c[j]) + o[j] : o[j]);
+  }
+}
+
+// ---------------------------------------------------------------- kernel
+// STAT, GRAD: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x.
+template <int MODE, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
+                const __grid_constant__ CUtensorMap tmX, const HeadGemm a) {
+  using C = Cfg<MODE, BN>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair_id = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&tfull[s], 1);
+      mbar_init(&tempty[s], 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    if (MODE != HEAD_STAT) prefetch_tmap(&tmC);
+    if (MODE == HEAD_BWD) prefetch_tmap(&tmD);
+    prefetch_tmap(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();   // barriers of both CTAs initialised, TMEM allocated in both
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_begin();
+  const Shape sh = shape_of<MODE, BN>(a);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer (both CTAs) ----------------
+      const bool whole = a.dense && sh.rows == a.N;
+      const CUtensorMap* x = whole ? &tmX : MODE == HEAD_BWD ? &tmD : &tmA;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair_id; t < sh.tiles && ok; t += num_pairs) {
+        const Tile tile = tile_of<MODE>(a, sh, t);
+        const int m0 = tile.mb * 2 * kBM + rank * kBM;
+        const int n0 = tile.nb * BN + rank * (BN / 2);
+        for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, nullptr, kErrTimeoutEmpty, abort_flag)) { ok = false; break; }
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
+          uint8_t* sa = smem + stage * C::STAGE_BYTES;
+          uint8_t* sb = sa + C::A_BYTES;
+          if (MODE == HEAD_BWD) {
+            const int k0 = (sh.two ? kb >> 1 : kb) * kBK;
+            const int low = sh.two && (kb & 1) ? a.g_low : 0;
+#pragma unroll
+            for (int p = 0; p < kBM / 64; ++p) {
+              if (tile.dw) tma_load_2d_pair(sa + p * 8192, &tmA, &full[stage], m0 + 64 * p, k0 + low);
+              else tma_load_2d_pair(sa + p * 8192, &tmA, &full[stage], k0, m0 + 64 * p + low);
+            }
+#pragma unroll
+            for (int p = 0; p < BN / 128; ++p)
+              tma_load_2d_pair(sb + p * 8192, tile.dw ? x : &tmB, &full[stage], n0 + 64 * p, k0);
+          } else {
+            tma_load_2d_pair(sa, x, &full[stage], kb * kBK, m0);
+            tma_load_2d_pair(sb, &tmB, &full[stage], kb * kBK, n0);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------- MMA issuer (leader only) ----------------
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int t = pair_id; t < sh.tiles && ok; t += num_pairs) {
+        const Tile tile = tile_of<MODE>(a, sh, t);
+        const bool a_mn = MODE == HEAD_BWD && tile.dw;
+        constexpr bool b_mn = MODE == HEAD_BWD;
+        const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, a_mn, b_mn);
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, nullptr, kErrTimeoutTmemEmpty, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
+          if (!mbar_wait(&full[stage], phase, nullptr, kErrTimeoutFull, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
+          const uint32_t sb = sa + C::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t ad = a_mn ? make_smem_desc(sa + k * 2048, 8192, 1024, 2) : make_smem_desc(sa + k * 32, 16, 1024, 2);
+            const uint64_t bd = b_mn ? make_smem_desc(sb + k * 2048, 8192, 1024, 2) : make_smem_desc(sb + k * 32, 16, 1024, 2);
+            umma_bf16_pair(d_tmem, ad, bd, idesc, (kb > tile.kb0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit_pair(&empty[stage], 0x3);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit_pair(&tfull[acc], 0x3);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else {
+    // ---------------- epilogue warps (both CTAs, 128 rows each) ----------------
+    const int q = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t tempty_leader0 = mapa_shared(smem_u32(&tempty[0]), 0);
+    const uint32_t tempty_leader1 = mapa_shared(smem_u32(&tempty[1]), 0);
+    uint8_t* stg = smem + C::EPI_OFF + (warp - 2) * C::EPI_WARP_BYTES;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    int box_at = 0;
+    float scale = 1.f;
+    if (MODE == HEAD_BWD && a.dw_splits == 1) {
+      scale = a.alpha;
+      if (a.scale != nullptr) scale *= *a.scale;
+      if (a.scale2 != nullptr) scale *= *a.scale2;
+    }
+    for (int t = pair_id; t < sh.tiles; t += num_pairs) {
+      const Tile tile = tile_of<MODE>(a, sh, t);
+      const int row0 = tile.mb * 2 * kBM + rank * kBM + q * 32;
+      const int n0 = tile.nb * BN;
+      RowTargets r;   // what this thread's row needs, fetched while the accumulator fills
+      if (MODE != HEAD_BWD) r.template fetch<MODE>(a, row0 + lane, n0 + half * 128, sh.rows);
+      if (!mbar_wait(&tfull[acc], acc_phase, nullptr, kErrTimeoutTmemFull, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
+      if (MODE == HEAD_STAT) {
+        stat128(a, r, tbase + half * 128, row0 + lane, n0 + half * 128);
+      } else if (MODE == HEAD_GRAD) {
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+          const int base = b * 64, col = n0 + half * 128 + base;
+          if (col >= a.cols) break;   // warp-uniform
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            grad32(a, r, tbase + half * 128 + base + 32 * h, base + 32 * h, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const uint32_t p = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+              hi[16 * h + j] = p;
+              lo[16 * h + j] = sh.two ? pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p)) : 0u;
+            }
+          }
+          store_box64(&tmC, stg, box_at, hi, col, row0, lane);
+          if (sh.two) store_box64(&tmC, stg, box_at, lo, col, row0 + a.g_low, lane);
+        }
+      } else if (tile.dw && a.dw_tma) {
+#pragma unroll 1
+        for (int c2 = half; c2 < BN / 64; c2 += 2) {
+          const int col = n0 + c2 * 64;
+          if (row0 >= a.cols || col >= a.D) break;   // nothing of the box inside dw (warp-uniform)
+          uint32_t r0[32], r1[32], pk[32];
+          tmem_ld_32x32b_x32(tbase + c2 * 64, r0);
+          tmem_ld_32x32b_x32(tbase + c2 * 64 + 32, r1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            pk[j] = pack_bf16x2(scale * __uint_as_float(r0[2 * j]), scale * __uint_as_float(r0[2 * j + 1]));
+            pk[16 + j] = pack_bf16x2(scale * __uint_as_float(r1[2 * j]), scale * __uint_as_float(r1[2 * j + 1]));
+          }
+          store_box64(&tmC, stg, box_at, pk, col, row0, lane);
+        }
+      } else {
+        // fp32 slabs, and the gradients of the weights that no TMA store takes: each 32 x 32 chunk goes through this
+        // warp's scratch (16-byte cells, XOR-swizzled by row), then 8 lanes write one row segment
+        float4* scr = reinterpret_cast<float4*>(stg);
+        const bool none = tile.kb0 == tile.kb1;   // a split without k-blocks: nothing was accumulated
+        const int rows = tile.dw ? a.cols : sh.rows;
+        const bool slab = !tile.dw || a.dw_splits > 1;
+        float* base = tile.dw ? (a.dw_splits > 1 ? a.dw_slab + (long long)tile.split * a.cols * a.ld_slab : (float*)a.dw)
+                              : a.dx_slab + (long long)tile.split * a.N * a.ld_slab;
+        const long long ld = slab ? a.ld_slab : a.lddw;
+        const bool add = tile.dw ? !slab && a.dw_add : a.dx_add;
+        const float f = slab ? 1.f : scale;
+#pragma unroll 1
+        for (int c = half; c < BN / 32; c += 2) {
+          float v[32];
+          load32(tbase + c * 32, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            scr[lane * 8 + (j ^ (lane & 7))] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                    : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          __syncwarp();
+          const int c4 = lane & 7, col = n0 + c * 32 + c4 * 4;
+          const int nv = min(4, a.D - col);
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int rr = it * 4 + (lane >> 3), m = row0 + rr;
+            const float4 x = scr[rr * 8 + (c4 ^ (rr & 7))];
+            float e[4] = {f * x.x, f * x.y, f * x.z, f * x.w};
+            if (m < rows && nv > 0) {
+              if (slab || a.dw_f32) store4(base + m * ld + col, e, nv, add);
+              else store4(reinterpret_cast<__nv_bfloat16*>(a.dw) + m * ld + col, e, nv, add);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive(&tempty[acc]);
+        else mbar_arrive_remote(acc ? tempty_leader1 : tempty_leader0);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (MODE != HEAD_STAT && lane == 0) bulk_group_wait_all();   // every TMA store has landed
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();   // both CTAs done with TMEM and with each other's barriers
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+}
+
+// ---------------------------------------------------------------- host
+static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// bf16 [outer, inner] rows of stride ld, boxes of [rows, 64] with the 128-byte swizzle
+static bool map2(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int rows) {
+  auto fn = encoder();
+  if (fn == nullptr || !((reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % 8 == 0)) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)rows};
+  const cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MODE, int BN>
+static int launch(const CUtensorMap (&t)[5], const HeadGemm& a, int tiles, int num_sms, cudaStream_t s) {
+  using C = Cfg<MODE, BN>;
+  static bool attr_done = false;
+  if (!attr_done) {
+    if (cudaFuncSetAttribute(head_kernel<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) != cudaSuccess)
+      return -3;
+    attr_done = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * std::min(tiles, num_sms / 2), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_env_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, head_kernel<MODE, BN>, t[0], t[1], t[2], t[3], t[4], a) == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace head
+}  // namespace pcb
+
+using namespace pcb;
+using namespace pcb::head;
+
+int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
+                  const void* w, long long ldw, void* g, long long ldg, int num_sms, cudaStream_t s) {
+  if (a.N < 1 || a.D < 1 || a.cols < 1 || num_sms < 2) return -1;
+  CUtensorMap t[5];
+  memset(t, 0, sizeof(t));
+  const int num_m = (a.N + 255) / 256;
+  const bool bwd = mode == HEAD_BWD;
+  const int xrows = bwd ? 64 : kBM;
+  CUtensorMap& tx = t[bwd ? 3 : 0];
+  if (!map2(&tx, x, a.D, a.N, ldx, xrows)) return -5;
+  a.dense = x_all != nullptr;
+  if (!a.dense) t[4] = tx;
+  else if (!map2(&t[4], x_all, a.D, a.N, ldx_all, xrows)) return -5;
+  if (!bwd) {
+    if (!map2(&t[1], w, a.D, a.cols, ldw, 128)) return -5;
+    if (mode == HEAD_GRAD && !map2(&t[2], g, a.cols, a.g_low + kTwoTermRows, ldg, 32)) return -5;
+    // the blocks that run side by side share the operand with the larger footprint
+    a.row_blocks_last = a.N > a.cols;
+    const int tiles = num_m * ((a.cols + 255) / 256);
+    return mode == HEAD_STAT ? launch<HEAD_STAT, 256>(t, a, tiles, num_sms, s) : launch<HEAD_GRAD, 256>(t, a, tiles, num_sms, s);
+  }
+  if (!map2(&t[0], g, a.cols, a.g_low + kTwoTermRows, ldg, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
+  a.dw_tma = a.dw_splits == 1 && !a.dw_f32 && !a.dw_add && map2(&t[2], a.dw, a.D, a.cols, a.lddw, 32);
+  if (!a.dw_tma) t[2] = t[0];
+  const int bn = head_bn(a.D);
+  const int num_n = (a.D + bn - 1) / bn;
+  const int tiles = ((a.cols + 255) / 256) * num_n * a.dw_splits + num_m * num_n * a.dx_splits;
+  return bn == 256 ? launch<HEAD_BWD, 256>(t, a, tiles, num_sms, s) : launch<HEAD_BWD, 128>(t, a, tiles, num_sms, s);
+}

@@ -1,0 +1,61 @@
+// Products of the vocabulary head (csrc/vocab_gemm.cu): what one launch reads and writes.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace pcb {
+
+// Up to this many counted rows, p - q is carried as two bf16 terms.  A gradient of few rows has few large entries,
+// so one rounding of them to 8 bits shows in its norm (up to 2^-8); over more rows the roundings average to about the
+// one that the bf16 result takes anyway.  It is the rows of one tile: the second term costs one more pass of
+// matrix instructions over a tile that reading the weights bounds.
+constexpr int kTwoTermRows = 256;
+
+enum HeadMode : int {
+  HEAD_STAT = 0,   // logits -> (max, sum) of every 128 of a row, and the logits at its targets
+  HEAD_GRAD = 1,   // logits -> g = softmax - target distribution, bf16
+  HEAD_BWD = 2,    // dw = g^T x and dx = g w in one launch
+};
+
+struct HeadGemm {
+  int N, D;               // rows of the batch, width
+  int cols;               // columns of the vocabulary in this launch
+  int v0;                 // the first of them (a multiple of 256)
+  const int* count;       // device: counted rows, packed in front
+  int dense;              // x itself may be read in place of the packed rows when all are counted
+  float c;                // log2(e) / temperature: exponents are taken to base 2
+  int row_blocks_last;    // order of tiles: 1 = the column blocks of one row block run side by side
+  // target distribution: K entries a row, ids ascending; without `start`, one id of weight 1
+  const int* row;         // [N] batch row of each packed row
+  const int* ids;         // [N, K], by batch row
+  const float* q;
+  int K;
+  const unsigned short* start;   // [2 ceil(V / 256) + 1, N]: first entry with id >= 128 g, by batch row
+  // STAT
+  float2* part;           // [2 ceil(V / 256), N] (max, sum), by packed row
+  float* z;               // [N, K] logits at the ids, by packed row
+  // GRAD, BWD
+  const float* lse;       // [N] base-2 log-sum-exp, by packed row
+  int g_low;              // row of g where the second terms begin (a multiple of 256, at least N)
+  // BWD
+  int dw_splits, dx_splits;   // 0: not wanted
+  void* dw;               // [cols, D], row stride lddw; or, with dw_splits > 1, fp32 slabs [dw_splits, cols, ld_slab]
+  long long lddw;
+  int dw_f32, dw_add, dw_tma;
+  float alpha;            // dw *= alpha * scale * scale2 (not the slabs)
+  const float* scale;
+  const float* scale2;
+  float* dx_slab;         // [dx_splits, N, ld_slab]
+  int dx_add;
+  float* dw_slab;
+  long long ld_slab;
+};
+
+// Columns of a tile of the gradients' products: 128 where 256 would leave an eighth or more of the columns empty.
+inline int head_bn(int D) { return (D + 255) / 256 * 256 - (D + 127) / 128 * 128 > 0 && D < 1024 ? 128 : 256; }
+
+}  // namespace pcb
+
+// x: packed rows [N, ldx]; x_all: the batch itself (nullptr: cannot be read in place); w: [cols, D] rows v0..; g: [g_low +
+// kTwoTermRows, ldg].  Returns 0, -1 (operands), -3 (launch), -5 (tensor map).
+int pcb_head_gemm(int mode, pcb::HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
+                  const void* w, long long ldw, void* g, long long ldg, int num_sms, cudaStream_t s);

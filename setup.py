@@ -68,6 +68,7 @@ setup(
                 os.path.join(CSRC, "vision.cu"),
                 os.path.join(CSRC, "moe.cu"),
                 os.path.join(CSRC, "vocab.cu"),
+                os.path.join(CSRC, "vocab_gemm.cu"),
                 os.path.join(CSRC, "skinny.cu"),
                 os.path.join(CSRC, "runtime.cpp"),
             ],
