@@ -554,11 +554,11 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     a.lddw = rows_apart(*dw);
   }
   a.dw_add = accumulate;
-  a.plan = pcb::vocab_plan(a.N, a.V, a.D, dx.has_value(), dw.has_value(), (int)std::min<int64_t>(piece, 1 << 30), num_sms());
+  a.plan = pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), num_sms());
   a.ld_slab = (a.D + 3) / 4 * 4;
   const int64_t gbytes = (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
-  const int64_t dx_slab = (int64_t)a.plan.dx_splits * st.N * a.ld_slab;
-  const int64_t dw_slab = a.plan.dw_splits > 1 ? (int64_t)a.plan.dw_splits * st.V * a.ld_slab : 0;
+  const int64_t dx_slab = dx ? (int64_t)a.plan.slab_rows * a.ld_slab : 0;
+  const int64_t dw_slab = dw && a.plan.dw_max > 1 ? (int64_t)a.plan.dw_max * st.V * a.ld_slab : 0;
   at::Tensor ws = at::empty({gbytes + 4 * (dx_slab + dw_slab)}, st.saved.options());
   a.g = ws.data_ptr();
   a.dx_slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);

@@ -177,11 +177,11 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(PackArgs a, int R) 
   const int k = block_scan(c ? 1 : 0, sums, &total);
   if (n < r1) {
     a.pos[n] = c ? base + k : -1;
-    if (a.tgt32 != nullptr) a.tgt32[n] = c ? (int)load_id(a.tgt, a.tgt64, n) : -1;
     if (!c) a.loss[n] = 0.f;
   }
   if (c) {
     a.row[base + k] = n;
+    if (a.tgt32 != nullptr) a.tgt32[base + k] = (int)load_id(a.tgt, a.tgt64, n);
     src[k] = n;
   }
   __syncthreads();
@@ -376,32 +376,34 @@ constexpr int kFinishVecs = 4;
 struct FinishArgs {
   const float* dx_slab;
   const float* dw_slab;
-  int dx_splits, dw_splits;
+  const int* count;
+  const int* plan;       // K splits of dw and dx
   const int* pos;
   void *dx, *dw;
   long long ld_slab, lddx, lddw;
   int dx_f32, dw_f32, dw_add;
-  int N, V, D;           // N = 0 where dx is not wanted, V = 0 where dw is not in slabs
+  int N, V, D;           // N = 0 where dx is not wanted, V = 0 where dw cannot be in slabs
   float alpha;
   const float* scale;
   const float* scale2;
 };
 
 template <int VEC>
-__global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a, int nrows) {
+__global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a) {
   pdl_begin();
   int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (n >= a.N + a.V) return;
   const bool w = n >= a.N;
   if (w) n -= a.N;
+  const int slabs = a.plan[w ? 0 : 1];
+  if (w && slabs == 1) return;   // written by the product itself
   const int j = w ? n : a.pos[n];
   float f = a.alpha;
   if (a.scale != nullptr) f *= *a.scale;
   if (a.scale2 != nullptr) f *= *a.scale2;
   const int d0 = (blockIdx.y * kFinishVecs * 32 + (threadIdx.x & 31)) * VEC;
   const float* src = (w ? a.dw_slab : a.dx_slab) + (long long)max(j, 0) * a.ld_slab + d0;
-  const long long stride = (w ? (long long)a.V : (long long)nrows) * a.ld_slab;
-  const int slabs = w ? a.dw_splits : a.dx_splits;
+  const long long stride = (w ? a.V : (max(a.count[0], 1) + 255) / 256 * 256) * a.ld_slab;
   float v[kFinishVecs][VEC] = {};
   if (j >= 0) {
     for (int k = 0; k < slabs; ++k, src += stride) {
@@ -837,24 +839,9 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
   return l;
 }
 
-// Splits of the two gradient products.  A tile costs its k-blocks and about 8 more for what the next tile's products do
-// not hide; the pairs of SMs walk the list of dw's tiles, then dx's, in turn, so the longest walk is one of a few
-// pairs.  Slabs cost their bytes, written and read once: a k-block of a 256-column tile takes the time of about 2.4 MB.
-static double walk(long long t1, double c1, long long t2, double c2, long long pairs) {
-  double most = 0;
-  const long long at[4] = {0, t1 % pairs, (t1 + t2) % pairs - 1, t1 % pairs - 1};
-  for (long long p : at) {
-    if (p < 0) p = pairs - 1;
-    const long long n1 = t1 > p ? (t1 - p + pairs - 1) / pairs : 0;
-    const long long n = t1 + t2 > p ? (t1 + t2 - p + pairs - 1) / pairs : 0;
-    most = std::max(most, n1 * c1 + (n - n1) * c2);
-  }
-  return most;
-}
-
 long long vocab_g_rows(int N) { return (N + 255LL) / 256 * 256 + kTwoTermRows; }
 
-VocabPlan vocab_plan(int N, int V, int D, bool dx, bool dw, int want_piece, int num_sms) {
+VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms) {
   VocabPlan r{};
   const long long all = (V + 255LL) / 256 * 256;
   long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2LL * N) / 256 * 256;
@@ -863,28 +850,12 @@ VocabPlan vocab_plan(int N, int V, int D, bool dx, bool dw, int want_piece, int 
   p = (all / 256 + r.pieces - 1) / r.pieces * 256;   // pieces of one size
   r.piece = (int)p;
   r.pieces = (int)((all + p - 1) / p);
+  // dw is split where its tiles do not fill the GPU; dx has room for a few splits of every row, and for all splits of a
+  // few rows
   const int bn = head_bn(D);
-  const long long num_n = (D + bn - 1) / bn, pairs = std::max(1, num_sms / 2);
-  const long long dw_tiles = (p / 256) * num_n, dx_tiles = ((N + 255LL) / 256) * num_n;
-  const double k = bn / 256.0, two = N <= kTwoTermRows ? 2.0 : 1.0;
-  const double kb_dw = two * k * ((N + 63) / 64), kb_dx = two * k * ((std::min<long long>(p, V) + 63) / 64);
-  // as if both were wanted, so that a gradient is the same with and without the other
-  double best = -1;
-  for (int s1 = 1; s1 <= (r.pieces == 1 ? 8 : 1); s1 *= 2) {
-    if (s1 > 1 && kb_dw < 4 * s1) break;
-    for (int s2 = 1; s2 <= 16; s2 += s2 < 4 ? 1 : s2 < 8 ? 2 : 4) {
-      if (s2 > 1 && kb_dx < 4 * s2) break;
-      const double slabs = 8.0 * D * ((s1 > 1 ? (double)s1 * p : 0.0) + (double)s2 * N) / 2.4e6;
-      const double c = walk(dw_tiles * s1, kb_dw / s1 + 8 * k, dx_tiles * s2, kb_dx / s2 + 8 * k, pairs) + slabs;
-      if (best < 0 || c < best) {
-        best = c;
-        r.dw_splits = s1;
-        r.dx_splits = s2;
-      }
-    }
-  }
-  if (!dw) r.dw_splits = 0;
-  if (!dx) r.dx_splits = 0;
+  const long long tiles = p / 256 * ((D + bn - 1) / bn);
+  r.dw_max = r.pieces == 1 ? (int)std::max(1LL, std::min(8LL, num_sms / 2 / tiles)) : 1;
+  r.slab_rows = (int)std::min((N + 255LL) / 256 * 256 + 16 * 256, 1LL << 30);
   return r;
 }
 
@@ -974,7 +945,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
 
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, a.distill != 0);
-  void* sv = const_cast<void*>(a.saved);
+  void* sv = a.saved;
   const void* x_all = readable(a.x, a.ldx, a.D) ? a.x : nullptr;
   const float T = a.distill ? a.temperature : 1.f;
   HeadGemm g{};
@@ -991,8 +962,11 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   }
   g.lse = (const float*)at(sv, l.lse);
   g.g_low = (a.N + 255) / 256 * 256;
-  g.dw_splits = a.plan.dw_splits;
-  g.dx_splits = a.plan.dx_splits;
+  g.plan = (int*)at(a.saved, l.count) + 2;
+  g.want_dw = a.dw != nullptr;
+  g.want_dx = a.dx != nullptr;
+  g.dw_max = a.plan.dw_max;
+  g.slab_rows = a.plan.slab_rows;
   g.lddw = a.lddw;
   g.dw_f32 = a.dw_f32;
   g.dw_add = a.dw_add;
@@ -1016,8 +990,8 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   FinishArgs f{};
   f.dx_slab = a.dx_slab;
   f.dw_slab = a.dw_slab;
-  f.dx_splits = a.plan.dx_splits;
-  f.dw_splits = a.plan.dw_splits;
+  f.count = g.count;
+  f.plan = g.plan;
   f.pos = (const int*)at(sv, l.pos);
   f.dx = a.dx;
   f.dw = a.dw;
@@ -1028,7 +1002,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   f.dw_f32 = a.dw_f32;
   f.dw_add = a.dw_add;
   f.N = a.dx != nullptr ? a.N : 0;
-  f.V = a.plan.dw_splits > 1 ? a.V : 0;
+  f.V = a.dw != nullptr && a.plan.dw_max > 1 ? a.V : 0;
   f.D = a.D;
   f.alpha = g.alpha;
   f.scale = g.scale;
@@ -1039,7 +1013,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   const int vecs = v4 ? a.D / 4 : a.D;
   const dim3 grid((f.N + f.V + 7) / 8, (vecs + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
   if (grid.y > 65535) return -1;
-  return pdl_launch(v4 ? finish_kernel<4> : finish_kernel<1>, grid, dim3(kThreads), 0, s, f, a.N) == cudaSuccess ? 0 : -3;
+  return pdl_launch(v4 ? finish_kernel<4> : finish_kernel<1>, grid, dim3(kThreads), 0, s, f) == cudaSuccess ? 0 : -3;
 }
 
 template <typename F>

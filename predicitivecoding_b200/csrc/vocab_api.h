@@ -34,12 +34,12 @@ struct VocabHeadArgs {
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;
-  long long count;   // int [4]: counted rows, finished blocks of the loss kernel
+  long long count;   // int [4]: counted rows, finished blocks of the loss kernel, K splits of dw and dx
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
-  long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature
-  long long z;       // float [N, K]: logits at the target ids
-  long long ids;     // int [N, K] ascending ids
+  long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature, by packed row
+  long long z;       // float [N, K]: logits at the target ids, by packed row
+  long long ids;     // int [N, K] ascending ids (cross entropy: the targets by packed row)
   long long q;       // float [N, K] weights (distillation)
   long long lq;      // float [N, K] log2 of the weights (distillation)
   long long len;     // int [N] entries present (distillation)
@@ -49,12 +49,13 @@ struct VocabLayout {
 };
 VocabLayout vocab_layout(int N, int V, int D, int K, bool distill);
 
-// How the backward goes over the vocabulary: columns at a time, and K splits of the two products (0: not wanted).
+// Workspaces of the backward.  The vocabulary is taken `piece` columns at a time.
 struct VocabPlan {
   int piece, pieces;
-  int dw_splits, dx_splits;
+  int dw_max;            // most K splits of the dw product
+  int slab_rows;         // rows of dx_slab
 };
-VocabPlan vocab_plan(int N, int V, int D, bool dx, bool dw, int want_piece, int num_sms);
+VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms);
 
 struct VocabGradArgs {
   const void* x;         // as the forward read it
@@ -64,7 +65,7 @@ struct VocabGradArgs {
   int N, V, D, K;
   int distill;
   float temperature;
-  const void* saved;     // buffer of the forward
+  void* saved;           // buffer of the forward
   const float* scalars;
   float gout;            // gradient of the loss: gout * *gout_dev (nullptr: 1) / (counted rows, for the mean)
   const float* gout_dev;
@@ -78,8 +79,8 @@ struct VocabGradArgs {
   int dw_add;
   VocabPlan plan;
   void* g;               // workspace: bf16 [vocab_g_rows(N), piece]
-  float* dx_slab;        // workspace: [dx_splits, N, ld_slab]
-  float* dw_slab;        // workspace: [dw_splits, V, ld_slab] when dw_splits > 1
+  float* dx_slab;        // workspace: fp32 [slab_rows, ld_slab]
+  float* dw_slab;        // workspace: fp32 [dw_max, V, ld_slab] when dw_max > 1
   long long ld_slab;
 };
 long long vocab_g_rows(int N);

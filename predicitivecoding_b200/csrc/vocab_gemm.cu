@@ -47,10 +47,15 @@ struct Cfg {
 
 struct Shape {   // what the number of counted rows makes of a launch
   int rows;      // counted rows
-  int dw_n, tiles;
   int num_n;     // column blocks
   int num_m;     // row blocks (BWD: of dx)
   int kb_dw, kb_dx;   // k-blocks of the whole contraction (STAT, GRAD: kb_dx)
+  int dw_tiles;
+  int tiles;     // STAT, GRAD: all; BWD: of dx
+  int dx_more;   // BWD: the pairs below this one have one dx tile more than the others
+  int dx_least;  // dx tiles of the others
+  int catch_up;  // dw tiles that the others do in the time of one dx tile
+  int dw_splits, dx_splits;   // 0: not wanted
   bool two;      // two-term g
 };
 
@@ -60,47 +65,77 @@ struct Tile {
   int kb0, kb1;
 };
 
+// k-blocks that a tile costs besides its own
+constexpr int kTileOverhead = 4;
+
+// K splits of dw and dx.  With the schedule below all pairs of SMs are busy for the mean of the work and half a tile of
+// dw, unless either product has too few tiles; slabs cost their bytes, written and read once, of which the time of
+// one k-block of a 256-column tile moves 2.4 MB.  As if both were wanted, so that a gradient is the same with and
+// without the other.
+PCB_DEVICE void plan_splits(const HeadGemm& a, int rows, int pairs, int* plan) {
+  const int bn = head_bn(a.D), num_n = (a.D + bn - 1) / bn;
+  const int r = max(rows, 1), two = rows <= kTwoTermRows ? 2 : 1;
+  const float kb_dw = two * ((r + kBK - 1) / kBK), kb_dx = two * ((a.cols + kBK - 1) / kBK);
+  const int dw = (a.cols + 255) / 256 * num_n, dx = (r + 255) / 256 * num_n;
+  const float slab = 8.f * a.D / 2.4e6f * (256 / bn);   // per row
+  const int dx_max = min(kMaxDxSplits, a.slab_rows / ((r + 255) / 256 * 256));
+  float best = INFINITY;
+  for (int s1 = 1; s1 <= a.dw_max && (s1 == 1 || kb_dw >= 4 * s1); s1 *= 2) {
+    const float c1 = kb_dw / s1 + kTileOverhead;
+    const float alone = (dw * s1 + pairs - 1) / pairs * c1;
+    for (int s2 = 1; s2 <= dx_max && (s2 == 1 || kb_dx >= 4 * s2); ++s2) {
+      const float c2 = kb_dx / s2 + kTileOverhead;
+      const float even = (dw * s1 * c1 + dx * s2 * c2) / pairs + 0.5f * c1;
+      const float c = fmaxf(fmaxf(even, alone), (dx * s2 + pairs - 1) / pairs * c2) + slab * ((s1 > 1 ? s1 * a.cols : 0) + s2 * r);
+      if (c < best) {
+        best = c;
+        plan[0] = s1;
+        plan[1] = s2;
+      }
+    }
+  }
+}
+
 template <int MODE, int BN>
-PCB_DEVICE Shape shape_of(const HeadGemm& a) {
+PCB_DEVICE Shape shape_of(const HeadGemm& a, int pairs) {
   Shape s;
   s.rows = min(*a.count, a.N);
   const int r = max(s.rows, 1);   // one tile at least: gradients of a batch without counted rows are zeros
   s.num_m = (r + 2 * kBM - 1) / (2 * kBM);
   s.two = MODE != HEAD_STAT && s.rows <= kTwoTermRows;
+  s.dw_tiles = s.kb_dw = s.dx_more = s.dx_least = s.catch_up = s.dw_splits = s.dx_splits = 0;
   if (MODE == HEAD_BWD) {
+    if (a.want_dw) s.dw_splits = a.plan[0];
+    if (a.want_dx) s.dx_splits = a.plan[1];
     s.num_n = (a.D + BN - 1) / BN;
     s.kb_dw = (r + kBK - 1) / kBK;
     s.kb_dx = (a.cols + kBK - 1) / kBK;
-    s.dw_n = (a.cols + 2 * kBM - 1) / (2 * kBM) * s.num_n * a.dw_splits;
-    s.tiles = s.dw_n + s.num_m * s.num_n * a.dx_splits;
+    s.dw_tiles = (a.cols + 2 * kBM - 1) / (2 * kBM) * s.num_n * s.dw_splits;
+    s.tiles = s.num_m * s.num_n * s.dx_splits;
+    s.dx_more = s.tiles % pairs;
+    s.dx_least = s.tiles / pairs;
+    if (s.dx_more > 0 && s.dw_splits > 0) {
+      const int k = s.two ? 2 : 1;
+      const int c_dx = k * s.kb_dx / s.dx_splits + kTileOverhead, c_dw = k * s.kb_dw / s.dw_splits + kTileOverhead;
+      s.catch_up = (c_dx + c_dw / 2) / c_dw;
+    }
   } else {
     s.num_n = (a.cols + BN - 1) / BN;
-    s.kb_dw = 0;
     s.kb_dx = (a.D + kBK - 1) / kBK;
-    s.dw_n = 0;
     s.tiles = s.num_m * s.num_n;
   }
   return s;
 }
 
+// The u-th tile of a pair; false behind its last.  BWD: dx's few long tiles go round first.  The pairs that got one
+// less do dw's first tiles among themselves for that time, then dw's other tiles go round all pairs: the order in
+// which pairs become free when all tiles take their expected time, so neighbouring tiles of dw run side by side and
+// share their operands in L2, and the pairs end within about one of its tiles of one another.
 template <int MODE>
-PCB_DEVICE Tile tile_of(const HeadGemm& a, const Shape& s, int t) {
-  Tile r;
-  if (MODE == HEAD_BWD) {
-    r.dw = t < s.dw_n;
-    const int splits = r.dw ? a.dw_splits : a.dx_splits, kb = r.dw ? s.kb_dw : s.kb_dx;
-    if (!r.dw) t -= s.dw_n;
-    r.nb = t % s.num_n;
-    t /= s.num_n;
-    r.split = t % splits;
-    r.mb = t / splits;
-    r.kb0 = (int)((long long)kb * r.split / splits);
-    r.kb1 = (int)((long long)kb * (r.split + 1) / splits);
-    if (s.two) {   // the two terms of g take turns, k-block by k-block
-      r.kb0 *= 2;
-      r.kb1 *= 2;
-    }
-  } else {
+PCB_DEVICE bool tile_at(const HeadGemm& a, const Shape& s, int pair, int pairs, int u, Tile& r) {
+  if (MODE != HEAD_BWD) {
+    const int t = pair + u * pairs;
+    if (t >= s.tiles) return false;
     r.dw = false;
     r.split = 0;
     if (a.row_blocks_last) {
@@ -112,8 +147,32 @@ PCB_DEVICE Tile tile_of(const HeadGemm& a, const Shape& s, int t) {
     }
     r.kb0 = 0;
     r.kb1 = s.kb_dx;
+    return true;
   }
-  return r;
+  const bool more = pair < s.dx_more;
+  const int mine = s.dx_least + (more ? 1 : 0);
+  int t;
+  r.dw = u >= mine;
+  if (!r.dw) {
+    t = pair + u * pairs;
+  } else {
+    const int j = u - mine, fewer = pairs - s.dx_more, early = s.catch_up * fewer;
+    if (!more && j < s.catch_up) t = pair - s.dx_more + j * fewer;
+    else t = early + pair + (j - (more ? 0 : s.catch_up)) * pairs;
+    if (t >= s.dw_tiles) return false;
+  }
+  const int splits = r.dw ? s.dw_splits : s.dx_splits, kb = r.dw ? s.kb_dw : s.kb_dx;
+  r.nb = t % s.num_n;
+  t /= s.num_n;
+  r.split = t % splits;
+  r.mb = t / splits;
+  r.kb0 = (int)((long long)kb * r.split / splits);
+  r.kb1 = (int)((long long)kb * (r.split + 1) / splits);
+  if (s.two) {   // the two terms of g take turns, k-block by k-block
+    r.kb0 *= 2;
+    r.kb1 *= 2;
+  }
+  return true;
 }
 
 // ---------------------------------------------------------------- epilogues of the logits
@@ -138,98 +197,149 @@ PCB_DEVICE float pick32(const float (&v)[32], int o) {
   return a[0];
 }
 
-// One packed row's part of the target list: the entries whose ids fall in this thread's 128 columns.
+// One packed row's part of the target list: the entries whose ids fall in this thread's 128 columns.  Its loads depend on
+// one another (row -> first entry -> id), so they are spread over the tile before the one that needs them.
 struct RowTargets {
-  bool live;      // a counted row
+  bool live;        // a counted row
   float lse;
-  long long at;   // entry of the next target, by batch row
-  long long to_z; // add: the same entry by packed row
-  int left;       // entries left in these columns
-  int next;       // column of the next one relative to the first of the 128; past them when none is left
-  int lo;         // vocabulary id of the first of the 128 columns
+  int n, m;         // the row's place in the batch and among the packed rows
+  int lo;           // vocabulary id of the first of the 128 columns
+  int entry, left;  // next entry of the row's list, entries left in these columns
+  int next;         // its column relative to `lo`; past the 128 when none is left
 
   template <int MODE>
-  PCB_DEVICE void fetch(const HeadGemm& h, int m, int col0, int rows) {
-    lse = 0.f;
-    at = to_z = 0;
-    left = 0;
-    next = 1 << 30;
+  PCB_DEVICE void load_row(const HeadGemm& h, int packed, int col0, int rows) {
+    m = packed;
     lo = h.v0 + col0;
-    live = m < rows;
+    live = packed < rows;
+    n = 0;
+    next = 1 << 30;
+    entry = left = 0;
+    lse = 0.f;
     if (!live) return;
-    const int n = h.row[m];
     if (MODE == HEAD_GRAD) lse = h.lse[m];
-    at = (long long)n * h.K;
-    to_z = (long long)(m - n) * h.K;
-    if (h.start != nullptr) {
-      const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
-      const int e = s[0];
-      left = s[h.N] - e;
-      at += e;
-    } else {
-      const int t = h.ids[n] - lo;
-      left = t >= 0 && t < 128 ? 1 : 0;
-    }
-    if (left > 0) next = h.ids[at] - lo;
+    if (h.start != nullptr) n = h.row[m];
+    else next = h.ids[m] - lo;   // class targets stand by packed row
   }
+  PCB_DEVICE void load_entries(const HeadGemm& h) {
+    if (h.start != nullptr) {
+      if (!live) return;
+      const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
+      entry = s[0];
+      left = s[h.N] - entry;
+    } else {
+      left = next >= 0 && next < 128 ? 1 : 0;
+      if (left == 0) next = 1 << 30;
+    }
+  }
+  PCB_DEVICE void load_next(const HeadGemm& h) {
+    if (h.start != nullptr && left > 0) next = h.ids[(long long)n * h.K + entry] - lo;
+  }
+  PCB_DEVICE float weight(const HeadGemm& h) const { return h.q != nullptr ? h.q[(long long)n * h.K + entry] : 1.f; }
+  PCB_DEVICE float* z(const HeadGemm& h) const { return h.z + (long long)m * h.K + entry; }
   PCB_DEVICE void advance(const HeadGemm& h) {
-    ++at;
-    next = --left > 0 ? h.ids[at] - lo : 1 << 30;
+    ++entry;
+    next = 1 << 30;
+    if (--left > 0) load_next(h);
   }
 };
 
+// tcgen05.wait::ld that names the registers it completes, so that no use of them moves above it while the next
+// load is in flight
+PCB_DEVICE void wait32(uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+        "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :
+      : "memory");
+}
+
 // (max, sum 2^(c l - max)) of this thread's 128 logits, in one pass with a running maximum, and the logits at the
 // row's targets.  The maximum stays in units of c l, and the sum is taken against that rounded value, so the
-// log-sum-exp made of the pair carries no error of the product c * max.
-PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int m, int col0) {
+// log-sum-exp made of the pair carries no error of the product c * max.  The next 32 columns come from TMEM while
+// these are worked on; `between(i)` runs after 32 columns.
+template <typename F>
+PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int col0, F between) {
   float mx = -INFINITY, sum = 0.f;
-#pragma unroll 1
+  uint32_t buf[2][32];
+  tmem_ld_32x32b_x32(taddr, buf[0]);
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
-    if (nvalid <= 0) break;
+    wait32(buf[i & 1]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
-    load32(taddr + 32 * i, v);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[i & 1][j]);
     while (r.next < 32 * (i + 1)) {
-      a.z[r.at + r.to_z] = pick32(v, r.next - 32 * i);
+      *r.z(a) = pick32(v, r.next - 32 * i);
       r.advance(a);
     }
     __syncwarp();
+    const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
     if (nvalid < 32) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : -INFINITY;
     }
-    float cm = v[0];
+    float cm[4];
 #pragma unroll
-    for (int j = 1; j < 32; ++j) cm = fmaxf(cm, v[j]);
-    const float nm = fmaxf(mx, cm * a.c);
+    for (int j = 0; j < 4; ++j) cm[j] = v[j];
+#pragma unroll
+    for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], v[j]);
+    const float nm = fmaxf(mx, fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * a.c);
     const float ref = nm == -INFINITY ? 0.f : nm;
-    float s0 = 0.f, s1 = 0.f;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      s0 += ex2_approx(fmaf(v[j], a.c, -ref));
-      s1 += ex2_approx(fmaf(v[j + 1], a.c, -ref));
-    }
-    sum = sum * ex2_approx(mx - ref) + (s0 + s1);
+    for (int j = 0; j < 32; ++j) s[j & 3] += ex2_approx(fmaf(v[j], a.c, -ref));
+    sum = sum * ex2_approx(mx - ref) + ((s[0] + s[1]) + (s[2] + s[3]));
     mx = nm;
+    between(i);
   }
-  if (r.live) a.part[(long long)((a.v0 + col0) >> 7) * a.N + m] = make_float2(mx, sum);
+  if (r.live) a.part[(long long)(r.lo >> 7) * a.N + r.m] = make_float2(mx, sum);
 }
 
-// 32 columns of softmax - target distribution, starting `base` columns into this thread's 128.  The factor 1 / count
-// is applied in fp32 behind the products that read them: rounding a shared factor into every entry would bias all of
-// them alike.
-PCB_DEVICE void grad32(const HeadGemm& a, RowTargets& r, uint32_t taddr, int base, float (&v)[32]) {
-  load32(taddr, v);
+// 128 columns of softmax - target distribution as bf16, 64 at a time handed to `store` (high terms, and with TWO the low
+// ones).  The factor 1 / count is applied in fp32 behind the products that read them: rounding a shared factor into
+// every entry would bias all of them alike.
+template <bool TWO, typename F, typename S>
+PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, F between, S store) {
+  const bool all = __all_sync(0xffffffffu, r.live);
+  uint32_t buf[2][32];
+  uint32_t hi[32], low[TWO ? 32 : 1];
+  tmem_ld_32x32b_x32(taddr, buf[0]);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = r.live ? ex2_approx(fmaf(v[j], a.c, -r.lse)) : 0.f;
-  while (r.next < base + 32) {
-    const int o = r.next - base;
-    const float q = a.q != nullptr ? a.q[r.at] : 1.f;
+  for (int i = 0; i < 4; ++i) {
+    wait32(buf[i & 1]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
+    float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] -= j == o ? q : 0.f;
-    r.advance(a);
+    for (int j = 0; j < 32; ++j) v[j] = ex2_approx(fmaf(__uint_as_float(buf[i & 1][j]), a.c, -r.lse));
+    if (!all) {   // what stands in a row that is not counted may be anything
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = r.live ? v[j] : 0.f;
+    }
+    while (r.next < 32 * (i + 1)) {
+      const int o = r.next - 32 * i;
+      const float q = r.weight(a);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] -= j == o ? q : 0.f;
+      r.advance(a);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t p = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      hi[16 * (i & 1) + j] = p;
+      if constexpr (TWO) low[16 * (i & 1) + j] = pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p));
+    }
+    if (i & 1) {
+      store(i >> 1, hi, false);
+      if constexpr (TWO) store(i >> 1, low, true);
+    }
+    between(i);
   }
-  __syncwarp();
 }
 
 // ---------------------------------------------------------------- stores
@@ -337,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_begin();
-  const Shape sh = shape_of<MODE, BN>(a);
+  const Shape sh = shape_of<MODE, BN>(a, num_pairs);
+  Tile tile;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -347,8 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair_id; t < sh.tiles && ok; t += num_pairs) {
-        const Tile tile = tile_of<MODE>(a, sh, t);
+      for (int u = 0; ok && tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
         const int m0 = tile.mb * 2 * kBM + rank * kBM;
         const int n0 = tile.nb * BN + rank * (BN / 2);
         for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
@@ -376,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
+    if (MODE == HEAD_GRAD && lane == 0 && !leader && pair_id == 0 && a.v0 == 0) plan_splits(a, sh.rows, a.bwd_pairs, a.plan);
     if (lane == 0 && leader) {
       // ---------------- MMA issuer (leader only) ----------------
       int stage = 0;
@@ -383,8 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
-      for (int t = pair_id; t < sh.tiles && ok; t += num_pairs) {
-        const Tile tile = tile_of<MODE>(a, sh, t);
+      for (int u = 0; ok && tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
         const bool a_mn = MODE == HEAD_BWD && tile.dw;
         constexpr bool b_mn = MODE == HEAD_BWD;
         const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, a_mn, b_mn);
@@ -422,43 +532,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_phase = 0;
     int box_at = 0;
     float scale = 1.f;
-    if (MODE == HEAD_BWD && a.dw_splits == 1) {
+    if (MODE == HEAD_BWD && sh.dw_splits == 1) {
       scale = a.alpha;
       if (a.scale != nullptr) scale *= *a.scale;
       if (a.scale2 != nullptr) scale *= *a.scale2;
     }
-    for (int t = pair_id; t < sh.tiles; t += num_pairs) {
-      const Tile tile = tile_of<MODE>(a, sh, t);
+    RowTargets ahead;
+    if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, 0, tile)) {
+      ahead.template load_row<MODE>(a, tile.mb * 2 * kBM + rank * kBM + q * 32 + lane, tile.nb * BN + half * 128, sh.rows);
+      ahead.load_entries(a);
+      ahead.load_next(a);
+    }
+    for (int u = 0; tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
       const int row0 = tile.mb * 2 * kBM + rank * kBM + q * 32;
       const int n0 = tile.nb * BN;
-      RowTargets r;   // what this thread's row needs, fetched while the accumulator fills
-      if (MODE != HEAD_BWD) r.template fetch<MODE>(a, row0 + lane, n0 + half * 128, sh.rows);
+      // the next tile's rows and targets are fetched under this one's arithmetic
+      RowTargets r = ahead;
+      int row0_next = 0, n0_next = 0, rows_next = 0;
+      Tile after;
+      if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, u + 1, after)) {
+        row0_next = after.mb * 2 * kBM + rank * kBM + q * 32;
+        n0_next = after.nb * BN;
+        rows_next = sh.rows;
+      }
+      auto between = [&](int i) {
+        if (i == 0) ahead.template load_row<MODE>(a, row0_next + lane, n0_next + half * 128, rows_next);
+        if (i == 1) ahead.load_entries(a);
+        if (i == 2) ahead.load_next(a);
+      };
       if (!mbar_wait(&tfull[acc], acc_phase, nullptr, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if (MODE == HEAD_STAT) {
-        stat128(a, r, tbase + half * 128, row0 + lane, n0 + half * 128);
+        stat128(a, r, tbase + half * 128, n0 + half * 128, between);
       } else if (MODE == HEAD_GRAD) {
-#pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
-          const int base = b * 64, col = n0 + half * 128 + base;
-          if (col >= a.cols) break;   // warp-uniform
-          uint32_t hi[32], lo[32];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[32];
-            grad32(a, r, tbase + half * 128 + base + 32 * h, base + 32 * h, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const uint32_t p = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-              hi[16 * h + j] = p;
-              lo[16 * h + j] = sh.two ? pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p)) : 0u;
-            }
-          }
-          store_box64(&tmC, stg, box_at, hi, col, row0, lane);
-          if (sh.two) store_box64(&tmC, stg, box_at, lo, col, row0 + a.g_low, lane);
-        }
-      } else if (tile.dw && a.dw_tma) {
+        auto store = [&](int b, const uint32_t (&pk)[32], bool low) {
+          const int col = n0 + half * 128 + 64 * b;
+          if (col < a.cols) store_box64(&tmC, stg, box_at, pk, col, row0 + (low ? a.g_low : 0), lane);   // warp-uniform
+        };
+        if (sh.two) grad128<true>(a, r, tbase + half * 128, between, store);
+        else grad128<false>(a, r, tbase + half * 128, between, store);
+      } else if (tile.dw && a.dw_tma && sh.dw_splits == 1) {
 #pragma unroll 1
         for (int c2 = half; c2 < BN / 64; c2 += 2) {
           const int col = n0 + c2 * 64;
@@ -480,9 +594,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float4* scr = reinterpret_cast<float4*>(stg);
         const bool none = tile.kb0 == tile.kb1;   // a split without k-blocks: nothing was accumulated
         const int rows = tile.dw ? a.cols : sh.rows;
-        const bool slab = !tile.dw || a.dw_splits > 1;
-        float* base = tile.dw ? (a.dw_splits > 1 ? a.dw_slab + (long long)tile.split * a.cols * a.ld_slab : (float*)a.dw)
-                              : a.dx_slab + (long long)tile.split * a.N * a.ld_slab;
+        const bool slab = !tile.dw || sh.dw_splits > 1;
+        float* base = !tile.dw ? a.dx_slab + (long long)tile.split * (sh.num_m * 256) * a.ld_slab
+                      : slab   ? a.dw_slab + (long long)tile.split * a.cols * a.ld_slab
+                               : (float*)a.dw;
         const long long ld = slab ? a.ld_slab : a.lddw;
         const bool add = tile.dw ? !slab && a.dw_add : a.dx_add;
         const float f = slab ? 1.f : scale;
@@ -590,6 +705,7 @@ using namespace pcb::head;
 int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
                   const void* w, long long ldw, void* g, long long ldg, int num_sms, cudaStream_t s) {
   if (a.N < 1 || a.D < 1 || a.cols < 1 || num_sms < 2) return -1;
+  a.bwd_pairs = num_sms / 2;   // tiles of the gradients are split until there are enough; a pair without one ends at once
   CUtensorMap t[5];
   memset(t, 0, sizeof(t));
   const int num_m = (a.N + 255) / 256;
@@ -609,10 +725,8 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
     return mode == HEAD_STAT ? launch<HEAD_STAT, 256>(t, a, tiles, num_sms, s) : launch<HEAD_GRAD, 256>(t, a, tiles, num_sms, s);
   }
   if (!map2(&t[0], g, a.cols, a.g_low + kTwoTermRows, ldg, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
-  a.dw_tma = a.dw_splits == 1 && !a.dw_f32 && !a.dw_add && map2(&t[2], a.dw, a.D, a.cols, a.lddw, 32);
+  a.dw_tma = a.want_dw && !a.dw_f32 && !a.dw_add && map2(&t[2], a.dw, a.D, a.cols, a.lddw, 32);
   if (!a.dw_tma) t[2] = t[0];
   const int bn = head_bn(a.D);
-  const int num_n = (a.D + bn - 1) / bn;
-  const int tiles = ((a.cols + 255) / 256) * num_n * a.dw_splits + num_m * num_n * a.dx_splits;
-  return bn == 256 ? launch<HEAD_BWD, 256>(t, a, tiles, num_sms, s) : launch<HEAD_BWD, 128>(t, a, tiles, num_sms, s);
+  return bn == 256 ? launch<HEAD_BWD, 256>(t, a, a.bwd_pairs, num_sms, s) : launch<HEAD_BWD, 128>(t, a, a.bwd_pairs, num_sms, s);
 }

@@ -24,9 +24,9 @@ struct HeadGemm {
   int dense;              // x itself may be read in place of the packed rows when all are counted
   float c;                // log2(e) / temperature: exponents are taken to base 2
   int row_blocks_last;    // order of tiles: 1 = the column blocks of one row block run side by side
-  // target distribution: K entries a row, ids ascending; without `start`, one id of weight 1
+  // target distribution: K entries a row, ids ascending, by batch row; without `start`, one id of weight 1, by packed row
   const int* row;         // [N] batch row of each packed row
-  const int* ids;         // [N, K], by batch row
+  const int* ids;         // [N, K]
   const float* q;
   int K;
   const unsigned short* start;   // [2 ceil(V / 256) + 1, N]: first entry with id >= 128 g, by batch row
@@ -36,22 +36,28 @@ struct HeadGemm {
   // GRAD, BWD
   const float* lse;       // [N] base-2 log-sum-exp, by packed row
   int g_low;              // row of g where the second terms begin (a multiple of 256, at least N)
-  // BWD
-  int dw_splits, dx_splits;   // 0: not wanted
-  void* dw;               // [cols, D], row stride lddw; or, with dw_splits > 1, fp32 slabs [dw_splits, cols, ld_slab]
+  // BWD.  The K splits of the two products depend on the number of counted rows: GRAD of the first
+  // piece of the vocabulary works them out and leaves them in plan[0] (dw) and plan[1] (dx).
+  int* plan;
+  int want_dw, want_dx;
+  int bwd_pairs;          // pairs of CTAs of the BWD launch (set by pcb_head_gemm)
+  int dw_max;             // most splits of dw
+  int slab_rows;          // rows of dx_slab: its splits times the counted rows, rounded up to 256, fit in
+  void* dw;               // [cols, D], row stride lddw (unsplit)
   long long lddw;
   int dw_f32, dw_add, dw_tma;
   float alpha;            // dw *= alpha * scale * scale2 (not the slabs)
   const float* scale;
   const float* scale2;
-  float* dx_slab;         // [dx_splits, N, ld_slab]
+  float* dx_slab;         // [splits][counted rows rounded up to 256, ld_slab], packed rows
   int dx_add;
-  float* dw_slab;
+  float* dw_slab;         // [splits][cols, ld_slab] when dw is split
   long long ld_slab;
 };
 
 // Columns of a tile of the gradients' products: 128 where 256 would leave an eighth or more of the columns empty.
-inline int head_bn(int D) { return (D + 255) / 256 * 256 - (D + 127) / 128 * 128 > 0 && D < 1024 ? 128 : 256; }
+constexpr int kMaxDxSplits = 16;
+__host__ __device__ inline int head_bn(int D) { return (D + 255) / 256 * 256 - (D + 127) / 128 * 128 > 0 && D < 1024 ? 128 : 256; }
 
 }  // namespace pcb
 
