@@ -29,9 +29,9 @@ PCB_DEVICE long long load_id(const void* p, int is64, long long i) {
   return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
 
-// Exclusive prefix sum of one int per thread over the block (blockDim a multiple of 32, at most 1024); total in *sum.
-PCB_DEVICE int block_scan(int v, int* warp_sums, int* sum) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+// Exclusive prefix sum of one int per thread over the block's first nw warps (all threads call it); total in *sum.
+PCB_DEVICE int block_scan(int v, int* warp_sums, int* sum, int nw) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -39,7 +39,7 @@ PCB_DEVICE int block_scan(int v, int* warp_sums, int* sum) {
     if (lane >= o) inc += t;
   }
   __syncthreads();   // the sums of the previous call have been read
-  if (lane == 31) warp_sums[w] = inc;
+  if (lane == 31 && w < nw) warp_sums[w] = inc;
   __syncthreads();
   int before = 0, total = 0;
   for (int i = 0; i < nw; ++i) {
@@ -76,6 +76,15 @@ PCB_DEVICE void load_vec(const T* p, float (&v)[VEC]) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
     v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
   }
+}
+// the same vector as loaded, for loads kept in flight in registers
+template <typename T, int VEC>
+struct Raw {
+  using type = std::conditional_t<VEC == 1, T, std::conditional_t<VEC * sizeof(T) == 16, uint4, uint2>>;
+};
+template <typename T, int VEC>
+PCB_DEVICE void unpack(const typename Raw<T, VEC>::type& r, float (&v)[VEC]) {
+  load_vec<T, VEC>(reinterpret_cast<const T*>(&r), v);
 }
 template <typename T, int VEC>
 PCB_DEVICE void store_vec(T* p, const float (&v)[VEC]) {
@@ -169,12 +178,12 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(PackArgs a, int R) 
     }
   }
   int base, rest;
-  block_scan(before, sums, &base);
-  block_scan(others, sums, &rest);
+  block_scan(before, sums, &base, kThreads / 32);
+  block_scan(others, sums, &rest, kThreads / 32);
   const int n = r0 + threadIdx.x;   // R is at most kThreads
   const bool c = n < r1 && counted(a, n);
   int total;
-  const int k = block_scan(c ? 1 : 0, sums, &total);
+  const int k = block_scan(c ? 1 : 0, sums, &total, kThreads / 32);
   if (n < r1) {
     a.pos[n] = c ? base + k : -1;
     if (!c) a.loss[n] = 0.f;
@@ -498,14 +507,15 @@ __global__ void __launch_bounds__(kThreads)
   hist[(long long)threadIdx.x * blocks + blockIdx.x] = h[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* __restrict__ hist, int total) {
+__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* __restrict__ hist, int total, int* __restrict__ list) {
   __shared__ int sums[32];
+  if (threadIdx.x == 0) list[0] = 0;
   int base = 0;
   for (int t0 = 0; t0 < total; t0 += 1024) {
     const int i = t0 + threadIdx.x;
     const int v = i < total ? (int)hist[i] : 0;
     int sum;
-    const int before = block_scan(v, sums, &sum);
+    const int before = block_scan(v, sums, &sum, 32);
     if (i < total) hist[i] = base + before;
     base += sum;
   }
@@ -583,7 +593,7 @@ PCB_DEVICE void write_zeros(char* p, long long bytes, int part, int parts) {
 template <int ITEMS>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThreads)
     cluster_sort_kernel(const void* __restrict__ tok, int tok64, int N, int V, int bits, uint32_t* __restrict__ keys_out,
-                        uint32_t* __restrict__ idx_out, char* zeros, long long zero_bytes) {
+                        uint32_t* __restrict__ idx_out, int* __restrict__ list, char* zeros, long long zero_bytes) {
   extern __shared__ __align__(16) uint32_t sm[];
   uint32_t* warp_count = sm;                                     // [warps][256]: keys of a digit, then its first place
   uint32_t* count = warp_count + kClusterWarps * 256;            // [blocks][256], the same in every block
@@ -597,6 +607,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
     return;
   }
   constexpr int PER = ITEMS * kClusterThreads;
+  if (blockIdx.x == 0 && threadIdx.x == 0) list[0] = 0;
   cluster_sync_all();   // every block of the cluster runs before another one writes to its shared memory
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int rank = (int)cluster_ctarank();
@@ -668,7 +679,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
         }
       }
       int total;
-      const int start = block_scan((int)all, sums, &total);
+      const int start = block_scan((int)all, sums, &total, 8);
       if (tid < 256) first[tid] = start + before;
     }
     __syncthreads();
@@ -699,10 +710,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
   }
 }
 
-// ---- sums over runs of equal tokens.  A block owns kChunk consecutive sorted entries and a slice of the columns;
-// a thread keeps VEC columns in registers over the run.  A run inside the chunk is written at once; the part of
-// a run that crosses a chunk's edge goes to a partial row, and join_kernel adds those in order.
-constexpr int kChunk = 16;
+// ---- sums over runs of equal tokens.  A warp owns kChunk consecutive sorted entries and 32 VEC of the columns.  A run of
+// up to kChunk entries is summed whole by the warp where it begins, which reads past its own entries for it.  A longer
+// one leaves a partial row in every chunk that it touches (slot 1 where it begins, slot 0 behind) and is put on a
+// list, and join_kernel adds its parts in order: however many tokens are the same, no warp sums more than two chunks.
+constexpr int kChunk = 8;
 
 template <typename TX, typename TW, int VEC>
 PCB_DEVICE void emit(TW* dw, uint32_t id, int D, int d0, float (&a)[VEC], float scale, int add) {
@@ -721,88 +733,150 @@ PCB_DEVICE void emit(TW* dw, uint32_t id, int D, int d0, float (&a)[VEC], float 
 template <typename TX, typename TW, int VEC>
 __global__ void __launch_bounds__(kThreads)
     run_sums_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ idx, const TX* __restrict__ dx,
-                    long long lddx, TW* __restrict__ dw, float* __restrict__ partial, int N, int V, int D, float scale,
-                    int add) {
-  __shared__ uint32_t s_key[kChunk + 2], s_idx[kChunk];
+                    long long lddx, TW* __restrict__ dw, float* __restrict__ partial, int* __restrict__ list, int N, int V,
+                    int D, float scale, int add) {
+  using R = typename Raw<TX, VEC>::type;
+  constexpr uint32_t kAll = 0xffffffffu;
   pdl_begin();
-  const int c0 = blockIdx.x * kChunk, cnt = min(kChunk, N - c0);
-  for (int i = threadIdx.x; i < cnt + 2; i += blockDim.x) {   // with both neighbours
-    const long long n = (long long)c0 + i - 1;
-    s_key[i] = n >= 0 && n < N ? keys[n] : 0xffffffffu;
-  }
-  for (int i = threadIdx.x; i < cnt; i += blockDim.x) s_idx[i] = idx[c0 + i];
-  __syncthreads();
-  const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (d0 >= D) return;
-  float acc[VEC] = {};
-  bool begun_before = s_key[0] == s_key[1];
-  constexpr int U = 8;
-  for (int i0 = 0; i0 < cnt; i0 += U) {
-    float r[U][VEC];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i0 + u < cnt && s_key[i0 + u + 1] < (uint32_t)V) load_vec<TX, VEC>(dx + s_idx[i0 + u] * lddx + d0, r[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      if (i >= cnt) break;
-      const uint32_t id = s_key[i + 1];
-      if (id >= (uint32_t)V) return;   // only tokens without a row follow
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += r[u][e];
-      const bool run_ends = s_key[i + 2] != id;
-      if (run_ends || i == cnt - 1) {
-        if (run_ends && !begun_before) {
-          emit<TX, TW, VEC>(dw, id, D, d0, acc, scale, add);
-        } else {
-          float* p = partial + ((long long)blockIdx.x * 2 + (begun_before ? 0 : 1)) * D + d0;
-          store_vec<float, VEC>(p, acc);
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-        begun_before = false;
-      }
+  const int lane = threadIdx.x & 31;
+  const int slices = (D + 32 * VEC - 1) / (32 * VEC);
+  const long long item = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const long long chunk = item / slices;
+  const int slice = (int)(item - chunk * slices);
+  if (chunk * kChunk >= N) return;   // whole warps
+  // lane l holds the key of entry l - kChunk of the chunk, with a chunk of keys on either side, and its place
+  const long long n = chunk * kChunk + lane - kChunk;
+  const bool in = lane < 3 * kChunk && n >= 0 && n < N;
+  const uint32_t key = in ? keys[n] : kAll - lane;   // outside: no two alike
+  const uint32_t place = in && lane >= kChunk ? idx[n] : 0u;
+  const uint32_t before = __shfl_up_sync(kAll, key, 1), behind8 = __shfl_down_sync(kAll, key, kChunk);
+  // per entry: the same token as the entry before; as the entry kChunk behind (of a run's first: it is a long run); a
+  // token with a row
+  const uint32_t same = __ballot_sync(kAll, lane > 0 && key == before);
+  const uint32_t longer = __ballot_sync(kAll, lane < 2 * kChunk && key == behind8);
+  const uint32_t live = __ballot_sync(kAll, in && key < (uint32_t)V);
+  // the chunk's first entry that is this warp's: behind a short run that began in the chunk before
+  int first = kChunk;
+  bool late = (same >> kChunk) & 1;   // the run at hand began in an earlier chunk
+  if (late) {
+    const int s = 31 - __clz(~same & ((2u << kChunk) - 1));   // its first entry in sight
+    if (!((longer >> s) & 1)) {
+      first = min(2 * kChunk, kChunk - 1 + __ffs(~(same >> kChunk)));
+      late = false;
     }
+  }
+  // entries of the next chunk that belong to a short run which begins here
+  int more = 0;
+  {
+    const int s = 31 - __clz(~same & ((1u << (2 * kChunk)) - 1));   // first entry of the chunk's last run
+    if (s >= first && !((longer >> s) & 1)) more = __ffs(~(same >> (2 * kChunk))) - 1;
+  }
+  const int d0 = (slice * 32 + lane) * VEC;
+  const bool mine = d0 < D;
+  // All rows are asked for at once: behind the zeros of a large matrix, which are still on their way to memory, a
+  // read takes microseconds.
+  constexpr int kAhead = 4;
+  R r[kChunk], ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) {
+    const uint32_t at = __shfl_sync(kAll, place, kChunk + i);
+    if (mine && kChunk + i >= first && ((live >> (kChunk + i)) & 1)) r[i] = *reinterpret_cast<const R*>(dx + at * lddx + d0);
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const uint32_t at = __shfl_sync(kAll, place, 2 * kChunk + i);
+    if (mine && i < more && ((live >> (2 * kChunk + i)) & 1)) ahead[i] = *reinterpret_cast<const R*>(dx + at * lddx + d0);
+  }
+  float acc[VEC] = {};
+  bool whole = false;   // the run at hand is summed here to its end
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) {
+    const int l = kChunk + i;
+    if (l < first) continue;
+    if (!((live >> l) & 1)) return;   // only tokens without a row follow
+    if (!late && (l == first || !((same >> l) & 1))) whole = !((longer >> l) & 1);
+    float v[VEC];
+    unpack<TX, VEC>(r[i], v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+    if (i < kChunk - 1 && ((same >> (l + 1)) & 1)) continue;
+    const uint32_t id = __shfl_sync(kAll, key, l);
+    if (late || !whole) {   // the run's part in this chunk
+      if (mine) store_vec<float, VEC>(partial + (chunk * 2 + (late ? 0 : 1)) * D + d0, acc);
+      if (!late && slice == 0 && lane == 0) list[1 + atomicAdd(list, 1)] = (int)chunk;   // in any order
+    } else {
+      if (i == kChunk - 1) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (j >= more) break;
+          unpack<TX, VEC>(ahead[j], v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+        }
+        for (int j = kAhead; j < more; ++j) {
+          const uint32_t at = __shfl_sync(kAll, place, 2 * kChunk + j);
+          if (mine) load_vec<TX, VEC>(dx + at * lddx + d0, v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+        }
+      }
+      if (mine) emit<TX, TW, VEC>(dw, id, D, d0, acc, scale, add);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    late = false;
   }
 }
 
-// The runs that begin in this block's chunk and go on behind it: their parts in order.
+// The long runs.  A block takes a run of the list and 32 VEC columns at a time; its warps share the run's parts, and the
+// first warp adds the warps' sums in order.
 template <typename TW, int VEC>
 __global__ void __launch_bounds__(kThreads)
-    join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, TW* __restrict__ dw, int N, int V,
-                int D, float scale, int add) {
+    join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ partial, const int* __restrict__ list,
+                TW* __restrict__ dw, int N, int V, int D, float scale, int add) {
+  constexpr int kWarps = kThreads / 32, U = 8;
+  __shared__ float s_sum[kWarps][32][VEC + 1];
   pdl_begin();
-  const long long c0 = (long long)blockIdx.x * kChunk, next = c0 + kChunk;
-  if (next >= N) return;
-  const uint32_t id = keys[next - 1];
-  if (id >= (uint32_t)V || keys[next] != id) return;
-  if (c0 > 0 && keys[c0 - 1] == id) return;   // begun in an earlier chunk
-  int parts = 0;                              // chunks behind this one that begin with the run
-  for (int more = blockDim.x; more == (int)blockDim.x;) {
-    const long long at = next + ((long long)parts + threadIdx.x) * kChunk;
-    more = __syncthreads_count(at < N && keys[at] == id);
-    parts += more;
-  }
-  const int d0 = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (d0 >= D) return;
-  float acc[VEC];
-  const float* p = partial + ((long long)blockIdx.x * 2 + 1) * D + d0;
-  load_vec<float, VEC>(p, acc);
-  p += D;
-  constexpr int U = 8;
-  for (int c = 0; c < parts; c += U) {
-    float r[U][VEC];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c + u < parts) load_vec<float, VEC>(p + (long long)(c + u) * 2 * D, r[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + u >= parts) break;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += r[u][e];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int slices = (D + 32 * VEC - 1) / (32 * VEC);
+  const long long items = (long long)list[0] * slices;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const int d0 = ((int)(item % slices) * 32 + lane) * VEC;
+    const long long c = list[1 + item / slices], next = (c + 1) * kChunk;
+    const uint32_t id = keys[next];
+    int parts = 1;   // chunks that the run touches
+    for (int more = blockDim.x; more == (int)blockDim.x;) {
+      const long long at = next + ((long long)parts - 1 + threadIdx.x) * kChunk;
+      more = __syncthreads_count(at < N && keys[at] == id);
+      parts += more;
     }
+    const int per = (parts + kWarps - 1) / kWarps, p0 = min(parts, w * per), p1 = min(parts, p0 + per);
+    float acc[VEC] = {};
+    if (d0 < D) {
+      for (int p = p0; p < p1; p += U) {
+        float r[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (p + u < p1) load_vec<float, VEC>(partial + ((c + p + u) * 2 + (p + u == 0 ? 1 : 0)) * D + d0, r[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (p + u < p1) acc[e] += r[u][e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s_sum[w][lane][e] = acc[e];
+    __syncthreads();
+    if (w == 0 && d0 < D) {
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += s_sum[k][lane][e];
+      emit<float, TW, VEC>(dw, id, D, d0, acc, scale, add);
+    }
+    __syncthreads();
   }
-  emit<float, TW, VEC>(dw, id, D, d0, acc, scale, add);
 }
 
 inline bool al(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -1055,11 +1129,11 @@ constexpr int kClusterKeys = 8 * kCluster * kClusterThreads;
 long long pcb_vocab_embed_bwd_bytes(int N, int V, int D) {
   const long long blocks = (N + kSortTile - 1) / kSortTile, chunks = (N + kChunk - 1) / kChunk;
   return (N <= kClusterKeys ? 2 : 4) * up256(4LL * N) + (N <= kClusterKeys ? 0 : up256(4LL * 256 * blocks)) +
-         up256(8LL * chunks * D);
+         up256(8LL * chunks * D) + up256(4LL * (chunks + 1));
 }
 
 template <int ITEMS>
-static int launch_cluster_sort(const void* tok, int tok64, int N, int V, int bits, uint32_t* keys, uint32_t* idx,
+static int launch_cluster_sort(const void* tok, int tok64, int N, int V, int bits, uint32_t* keys, uint32_t* idx, int* list,
                                void* zeros, long long zero_bytes, int num_sms, cudaStream_t s) {
   constexpr int smem = cluster_sort_smem<ITEMS>();
   static bool attr_done = false;
@@ -1068,11 +1142,12 @@ static int launch_cluster_sort(const void* tok, int tok64, int N, int V, int bit
       return -3;
     attr_done = true;
   }
-  // as many more clusters as there is for them to write, 64 KB a block at least
-  const int most = std::max(1, num_sms / kCluster - 2);
+  // as many more clusters as there is for them to write, 64 KB a block, up to 7 blocks an SM: of 131 MB (4096 tokens, V
+  // 32000, D 2048) 16 clusters made 55 us of the gradient, 34 made 44, 128 made 38 and 512 made 41
+  const int most = 7 * num_sms / kCluster;
   const int clusters = zero_bytes > 0 ? 1 + (int)std::min<long long>(most, (zero_bytes >> 19) + 1) : 1;
   return pdl_launch(cluster_sort_kernel<ITEMS>, dim3(clusters * kCluster), dim3(kClusterThreads), smem, s, tok, tok64, N,
-                    V, bits, keys, idx, (char*)zeros, zero_bytes) == cudaSuccess ? 0 : -3;
+                    V, bits, keys, idx, list, (char*)zeros, zero_bytes) == cudaSuccess ? 0 : -3;
 }
 
 int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16, long long lddx, void* dw, int dw_bf16,
@@ -1089,11 +1164,12 @@ int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16,
   int bits = 1;
   while (bits < 32 && (V >> bits) != 0) ++bits;   // keys run up to V
   const uint32_t *keys = nullptr, *idx = nullptr;
+  int* list = (int*)take(4LL * (chunks + 1));   // number of long runs, then the chunks where they begin; emptied by the sort
   int rc = 0;
   if (N <= kClusterKeys) {
     uint32_t *k = (uint32_t*)take(4LL * N), *i = (uint32_t*)take(4LL * N);
     auto sort = [&](auto items) {
-      return launch_cluster_sort<decltype(items)::value>(tok, tok64, N, V, bits, k, i, dw, zero_bytes, num_sms, s);
+      return launch_cluster_sort<decltype(items)::value>(tok, tok64, N, V, bits, k, i, list, dw, zero_bytes, num_sms, s);
     };
     if (N <= kClusterKeys / 8) rc = sort(std::integral_constant<int, 1>{});
     else if (N <= kClusterKeys / 4) rc = sort(std::integral_constant<int, 2>{});
@@ -1110,7 +1186,7 @@ int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16,
     int side = 0;
     for (int shift = 0; shift < bits; shift += 8) {
       sort_hist_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, N, V, shift, hist, blocks);
-      sort_scan_kernel<<<1, 1024, 0, s>>>(hist, 256 * blocks);
+      sort_scan_kernel<<<1, 1024, 0, s>>>(hist, 256 * blocks, list);
       sort_scatter_kernel<<<blocks, kThreads, 0, s>>>(tok, tok64, keys, idx, N, V, shift, hist, blocks, buf[2 * side],
                                                       buf[2 * side + 1]);
       if (launched()) return -3;
@@ -1126,13 +1202,14 @@ int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16,
     auto go = [&](auto v) {
       constexpr int VEC = decltype(v)::value;
       const int cols = (D + VEC - 1) / VEC;
-      const int threads = std::min(kThreads, (cols + 31) / 32 * 32);
-      const dim3 grid(chunks, (cols + threads - 1) / threads);
-      if (grid.y > 65535) { rc = -1; return; }
-      if (pdl_launch(run_sums_kernel<TX, TW, VEC>, grid, dim3(threads), 0, s, keys, idx, (const TX*)dx, lddx, (TW*)dw,
-                     partial, N, V, D, scale, add) != cudaSuccess ||
-          pdl_launch(join_kernel<TW, VEC>, grid, dim3(threads), 0, s, keys, (const float*)partial, (TW*)dw, N, V, D, scale,
-                     add) != cudaSuccess)
+      const int slices = (cols + 31) / 32;
+      const long long warps = (long long)chunks * slices, blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
+      if (blocks > 0x7fffffffLL) { rc = -1; return; }
+      const int joins = (int)std::min<long long>(4 * num_sms, warps);
+      if (pdl_launch(run_sums_kernel<TX, TW, VEC>, dim3((unsigned)blocks), dim3(kThreads), 0, s, keys, idx, (const TX*)dx, lddx, (TW*)dw,
+                     partial, list, N, V, D, scale, add) != cudaSuccess ||
+          pdl_launch(join_kernel<TW, VEC>, dim3(joins), dim3(kThreads), 0, s, keys, (const float*)partial, (const int*)list,
+                     (TW*)dw, N, V, D, scale, add) != cudaSuccess)
         rc = -3;
     };
     const bool wide = dx_bf16 && D % 8 == 0 && lddx % 8 == 0 && al(dx, 16) && al(dw, 16);
