@@ -1010,7 +1010,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   g.start = start;
   g.part = (float2*)part;
   g.z = z;
-  const int rc = pcb_head_gemm(HEAD_STAT, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, 0, num_sms, s);
+  const int rc = pcb_head_gemm(HEAD_STAT, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, num_sms, s);
   if (rc) return rc;
   return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, l.granules,
                     (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
@@ -1036,6 +1036,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   }
   g.lse = (const float*)at(sv, l.lse);
   g.g_low = (a.N + 255) / 256 * 256;
+  g.g_rows = (int)vocab_g_rows(a.N);
   g.plan = (int*)at(a.saved, l.count) + 2;
   g.want_dw = a.dw != nullptr;
   g.want_dx = a.dx != nullptr;
@@ -1057,7 +1058,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.dw = a.dw == nullptr ? nullptr : (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
     const __nv_bfloat16* w = (const __nv_bfloat16*)a.w + (long long)v0 * a.ldw;
     for (int mode : {HEAD_GRAD, HEAD_BWD}) {
-      const int rc = pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, a.plan.piece, num_sms, s);
+      const int rc = pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, num_sms, s);
       if (rc) return rc;
     }
   }

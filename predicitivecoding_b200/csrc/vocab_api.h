@@ -78,7 +78,7 @@ struct VocabGradArgs {
   int dw_f32;
   int dw_add;
   VocabPlan plan;
-  void* g;               // workspace: bf16 [vocab_g_rows(N), piece]
+  void* g;               // workspace: bf16, vocab_g_rows(N) * piece
   float* dx_slab;        // workspace: fp32 [slab_rows, ld_slab]
   float* dw_slab;        // workspace: fp32 [dw_max, V, ld_slab] when dw_max > 1
   long long ld_slab;

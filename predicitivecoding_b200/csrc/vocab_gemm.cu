@@ -198,7 +198,8 @@ PCB_DEVICE float pick32(const float (&v)[32], int o) {
 }
 
 // One packed row's part of the target list: the entries whose ids fall in this thread's 128 columns.  Its loads depend on
-// one another (row -> first entry -> id), so they are spread over the tile before the one that needs them.
+// one another (row -> first entry -> id): each of the three steps only asks, and the next one, 32 columns of
+// arithmetic later, uses the answer.
 struct RowTargets {
   bool live;        // a counted row
   float lse;
@@ -208,41 +209,54 @@ struct RowTargets {
   int next;         // its column relative to `lo`; past the 128 when none is left
 
   template <int MODE>
-  PCB_DEVICE void load_row(const HeadGemm& h, int packed, int col0, int rows) {
+  PCB_DEVICE void ask_row(const HeadGemm& h, int packed, int col0, int rows) {
     m = packed;
     lo = h.v0 + col0;
     live = packed < rows;
-    n = 0;
-    next = 1 << 30;
-    entry = left = 0;
-    lse = 0.f;
-    if (!live) return;
-    if (MODE == HEAD_GRAD) lse = h.lse[m];
-    if (h.start != nullptr) n = h.row[m];
-    else next = h.ids[m] - lo;   // class targets stand by packed row
+    const int at = max(min(packed, rows - 1), 0);
+    lse = MODE == HEAD_GRAD ? h.lse[at] : 0.f;
+    n = h.start != nullptr ? h.row[at] : h.ids[at];   // class targets stand by packed row
   }
-  PCB_DEVICE void load_entries(const HeadGemm& h) {
-    if (h.start != nullptr) {
-      if (!live) return;
-      const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
-      entry = s[0];
-      left = s[h.N] - entry;
+  PCB_DEVICE void ask_entries(const HeadGemm& h) {
+    if (h.start == nullptr) return;
+    if (!live) n = 0;   // with no row counted at all there is no first one either
+    const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
+    entry = s[0];
+    left = s[h.N];
+  }
+  PCB_DEVICE void ask_next(const HeadGemm& h) {
+    if (h.start == nullptr) {
+      const int t = n - lo;
+      left = live && t >= 0 && t < 128 ? 1 : 0;
+      entry = n = 0;
+      next = left > 0 ? t + lo : 0;
     } else {
-      left = next >= 0 && next < 128 ? 1 : 0;
-      if (left == 0) next = 1 << 30;
+      left = live ? left - entry : 0;
+      next = left > 0 ? h.ids[(long long)n * h.K + entry] : 0;
     }
   }
-  PCB_DEVICE void load_next(const HeadGemm& h) {
-    if (h.start != nullptr && left > 0) next = h.ids[(long long)n * h.K + entry] - lo;
-  }
+  PCB_DEVICE void settle() { next = left > 0 ? next - lo : 1 << 30; }
   PCB_DEVICE float weight(const HeadGemm& h) const { return h.q != nullptr ? h.q[(long long)n * h.K + entry] : 1.f; }
   PCB_DEVICE float* z(const HeadGemm& h) const { return h.z + (long long)m * h.K + entry; }
   PCB_DEVICE void advance(const HeadGemm& h) {
     ++entry;
-    next = 1 << 30;
-    if (--left > 0) load_next(h);
+    next = --left > 0 ? h.ids[(long long)n * h.K + entry] - lo : 1 << 30;
   }
 };
+
+PCB_DEVICE float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// (a0, a1) * b + (c, c)
+PCB_DEVICE void scale2(float& d0, float& d1, float a0, float a1, float b, float c) { ffma2v(d0, d1, a0, a1, b, c, c); }
+PCB_DEVICE void add2(float& d0, float& d1, float a0, float a1) {
+  asm("{\n\t.reg .b64 ra, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rd, {%0, %1};\n\t"
+      "add.rn.f32x2 rd, rd, ra;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1));
+}
 
 // tcgen05.wait::ld that names the registers it completes, so that no use of them moves above it while the next
 // load is in flight
@@ -285,15 +299,26 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
     }
     float cm[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = v[j];
+    for (int j = 0; j < 4; ++j) cm[j] = max3(v[8 * j], v[8 * j + 1], v[8 * j + 2]);
 #pragma unroll
-    for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], v[j]);
-    const float nm = fmaxf(mx, fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * a.c);
+    for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 3], v[8 * j + 4]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 5], v[8 * j + 6]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cm[j] = fmaxf(cm[j], v[8 * j + 7]);
+    const float nm = fmaxf(mx, max3(fmaxf(cm[0], cm[1]), cm[2], cm[3]) * a.c);
     const float ref = nm == -INFINITY ? 0.f : nm;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[8] = {};
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[j & 3] += ex2_approx(fmaf(v[j], a.c, -ref));
-    sum = sum * ex2_approx(mx - ref) + ((s[0] + s[1]) + (s[2] + s[3]));
+    for (int j = 0; j < 32; j += 2) {
+      float e0, e1;
+      scale2(e0, e1, v[j], v[j + 1], a.c, -ref);
+      add2(s[j & 7], s[(j & 7) + 1], ex2_approx(e0), ex2_approx(e1));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) add2(s[j], s[j + 1], s[j + 4], s[j + 5]);
+    add2(s[0], s[1], s[2], s[3]);
+    sum = fmaf(sum, ex2_approx(mx - ref), s[0] + s[1]);
     mx = nm;
     between(i);
   }
@@ -304,7 +329,7 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 // ones).  The factor 1 / count is applied in fp32 behind the products that read them: rounding a shared factor into
 // every entry would bias all of them alike.
 template <bool TWO, typename F, typename S>
-PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, F between, S store) {
+PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int col0, F between, S store) {
   const bool all = __all_sync(0xffffffffu, r.live);
   uint32_t buf[2][32];
   uint32_t hi[32], low[TWO ? 32 : 1];
@@ -315,10 +340,19 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, F betw
     if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = ex2_approx(fmaf(__uint_as_float(buf[i & 1][j]), a.c, -r.lse));
+    for (int j = 0; j < 32; j += 2) {
+      scale2(v[j], v[j + 1], __uint_as_float(buf[i & 1][j]), __uint_as_float(buf[i & 1][j + 1]), a.c, -r.lse);
+      v[j] = ex2_approx(v[j]);
+      v[j + 1] = ex2_approx(v[j + 1]);
+    }
     if (!all) {   // what stands in a row that is not counted may be anything
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = r.live ? v[j] : 0.f;
+    }
+    const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
+    if (nvalid < 32) {   // the rest of the last panel: K of dx's product
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : 0.f;
     }
     while (r.next < 32 * (i + 1)) {
       const int o = r.next - 32 * i;
@@ -471,8 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int low = sh.two && (kb & 1) ? a.g_low : 0;
 #pragma unroll
             for (int p = 0; p < kBM / 64; ++p) {
-              if (tile.dw) tma_load_2d_pair(sa + p * 8192, &tmA, &full[stage], m0 + 64 * p, k0 + low);
-              else tma_load_2d_pair(sa + p * 8192, &tmA, &full[stage], k0, m0 + 64 * p + low);
+              const int panel = tile.dw ? m0 / 64 + p : k0 / 64, at = tile.dw ? k0 : m0 + 64 * p;
+              tma_load_2d_pair(sa + p * 8192, &tmA, &full[stage], 0, panel * a.g_rows + at + low);
             }
 #pragma unroll
             for (int p = 0; p < BN / 128; ++p)
@@ -495,23 +529,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t acc_phase = 0;
       bool ok = true;
       for (int u = 0; ok && tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
+        // Shared-memory descriptors advance by additions to their low words (address / 16): the issue of one k-block has
+        // to take less than the 512 cycles that its matrix instructions do.
         const bool a_mn = MODE == HEAD_BWD && tile.dw;
         constexpr bool b_mn = MODE == HEAD_BWD;
         const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, a_mn, b_mn);
+        const uint64_t a0 = a_mn ? make_smem_desc(smem_u32(smem), 8192, 1024, 2) : make_smem_desc(smem_u32(smem), 16, 1024, 2);
+        const uint64_t b0 = make_smem_desc(smem_u32(smem) + C::A_BYTES, b_mn ? 8192 : 16, 1024, 2);
+        const uint32_t a_step = a_mn ? 2048 / 16 : 32 / 16;
+        constexpr uint32_t b_step = b_mn ? 2048 / 16 : 32 / 16;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, nullptr, kErrTimeoutTmemEmpty, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
         for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, nullptr, kErrTimeoutFull, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
-          const uint32_t sb = sa + C::A_BYTES;
+          const uint64_t ad = a0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
+          const uint64_t bd = b0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
+          umma_bf16_pair(d_tmem, ad, bd, idesc, kb > tile.kb0 ? 1u : 0u);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            const uint64_t ad = a_mn ? make_smem_desc(sa + k * 2048, 8192, 1024, 2) : make_smem_desc(sa + k * 32, 16, 1024, 2);
-            const uint64_t bd = b_mn ? make_smem_desc(sb + k * 2048, 8192, 1024, 2) : make_smem_desc(sb + k * 32, 16, 1024, 2);
-            umma_bf16_pair(d_tmem, ad, bd, idesc, (kb > tile.kb0 || k > 0) ? 1u : 0u);
-          }
+          for (int k = 1; k < kBK / 16; ++k) umma_bf16_pair(d_tmem, ad + k * a_step, bd + k * b_step, idesc, 1u);
           umma_commit_pair(&empty[stage], 0x3);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
@@ -539,15 +576,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     RowTargets ahead;
     if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, 0, tile)) {
-      ahead.template load_row<MODE>(a, tile.mb * 2 * kBM + rank * kBM + q * 32 + lane, tile.nb * BN + half * 128, sh.rows);
-      ahead.load_entries(a);
-      ahead.load_next(a);
+      ahead.template ask_row<MODE>(a, tile.mb * 2 * kBM + rank * kBM + q * 32 + lane, tile.nb * BN + half * 128, sh.rows);
+      ahead.ask_entries(a);
+      ahead.ask_next(a);
     }
     for (int u = 0; tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
       const int row0 = tile.mb * 2 * kBM + rank * kBM + q * 32;
       const int n0 = tile.nb * BN;
       // the next tile's rows and targets are fetched under this one's arithmetic
       RowTargets r = ahead;
+      if (MODE != HEAD_BWD) r.settle();
       int row0_next = 0, n0_next = 0, rows_next = 0;
       Tile after;
       if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, u + 1, after)) {
@@ -556,9 +594,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         rows_next = sh.rows;
       }
       auto between = [&](int i) {
-        if (i == 0) ahead.template load_row<MODE>(a, row0_next + lane, n0_next + half * 128, rows_next);
-        if (i == 1) ahead.load_entries(a);
-        if (i == 2) ahead.load_next(a);
+        if (i == 0) ahead.template ask_row<MODE>(a, row0_next + lane, n0_next + half * 128, rows_next);
+        if (i == 1) ahead.ask_entries(a);
+        if (i == 2) ahead.ask_next(a);
       };
       if (!mbar_wait(&tfull[acc], acc_phase, nullptr, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
@@ -568,10 +606,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else if (MODE == HEAD_GRAD) {
         auto store = [&](int b, const uint32_t (&pk)[32], bool low) {
           const int col = n0 + half * 128 + 64 * b;
-          if (col < a.cols) store_box64(&tmC, stg, box_at, pk, col, row0 + (low ? a.g_low : 0), lane);   // warp-uniform
+          if (col < a.cols)   // warp-uniform
+            store_box64(&tmC, stg, box_at, pk, 0, col / 64 * a.g_rows + row0 + (low ? a.g_low : 0), lane);
         };
-        if (sh.two) grad128<true>(a, r, tbase + half * 128, between, store);
-        else grad128<false>(a, r, tbase + half * 128, between, store);
+        if (sh.two) grad128<true>(a, r, tbase + half * 128, n0 + half * 128, between, store);
+        else grad128<false>(a, r, tbase + half * 128, n0 + half * 128, between, store);
       } else if (tile.dw && a.dw_tma && sh.dw_splits == 1) {
 #pragma unroll 1
         for (int c2 = half; c2 < BN / 64; c2 += 2) {
@@ -703,13 +742,15 @@ using namespace pcb;
 using namespace pcb::head;
 
 int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
-                  const void* w, long long ldw, void* g, long long ldg, int num_sms, cudaStream_t s) {
+                  const void* w, long long ldw, void* g, int num_sms, cudaStream_t s) {
   if (a.N < 1 || a.D < 1 || a.cols < 1 || num_sms < 2) return -1;
   a.bwd_pairs = num_sms / 2;   // tiles of the gradients are split until there are enough; a pair without one ends at once
   CUtensorMap t[5];
   memset(t, 0, sizeof(t));
   const int num_m = (a.N + 255) / 256;
   const bool bwd = mode == HEAD_BWD;
+  const long long panels = (a.cols + 63) / 64;
+  if (panels * a.g_rows > 0x7fffffffLL) return -1;   // rows of g's panels are addressed by an int
   const int xrows = bwd ? 64 : kBM;
   CUtensorMap& tx = t[bwd ? 3 : 0];
   if (!map2(&tx, x, a.D, a.N, ldx, xrows)) return -5;
@@ -718,13 +759,13 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
   else if (!map2(&t[4], x_all, a.D, a.N, ldx_all, xrows)) return -5;
   if (!bwd) {
     if (!map2(&t[1], w, a.D, a.cols, ldw, 128)) return -5;
-    if (mode == HEAD_GRAD && !map2(&t[2], g, a.cols, a.g_low + kTwoTermRows, ldg, 32)) return -5;
+    if (mode == HEAD_GRAD && !map2(&t[2], g, 64, panels * a.g_rows, 64, 32)) return -5;
     // the blocks that run side by side share the operand with the larger footprint
     a.row_blocks_last = a.N > a.cols;
     const int tiles = num_m * ((a.cols + 255) / 256);
     return mode == HEAD_STAT ? launch<HEAD_STAT, 256>(t, a, tiles, num_sms, s) : launch<HEAD_GRAD, 256>(t, a, tiles, num_sms, s);
   }
-  if (!map2(&t[0], g, a.cols, a.g_low + kTwoTermRows, ldg, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
+  if (!map2(&t[0], g, 64, panels * a.g_rows, 64, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
   a.dw_tma = a.want_dw && !a.dw_f32 && !a.dw_add && map2(&t[2], a.dw, a.D, a.cols, a.lddw, 32);
   if (!a.dw_tma) t[2] = t[0];
   const int bn = head_bn(a.D);

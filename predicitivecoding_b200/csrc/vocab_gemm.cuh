@@ -35,7 +35,10 @@ struct HeadGemm {
   float* z;               // [N, K] logits at the ids, by packed row
   // GRAD, BWD
   const float* lse;       // [N] base-2 log-sum-exp, by packed row
-  int g_low;              // row of g where the second terms begin (a multiple of 256, at least N)
+  // g: panels of 64 columns, each [g_rows, 64], so that every box that is stored or loaded (32 or 64 rows of a panel) is
+  // one run of memory, whichever of its two dimensions the product contracts
+  int g_rows;
+  int g_low;              // row of a panel where the second terms begin (a multiple of 256, at least N)
   // BWD.  The K splits of the two products depend on the number of counted rows: GRAD of the first
   // piece of the vocabulary works them out and leaves them in plan[0] (dw) and plan[1] (dx).
   int* plan;
@@ -61,7 +64,7 @@ __host__ __device__ inline int head_bn(int D) { return (D + 255) / 256 * 256 - (
 
 }  // namespace pcb
 
-// x: packed rows [N, ldx]; x_all: the batch itself (nullptr: cannot be read in place); w: [cols, D] rows v0..; g: [g_low +
-// kTwoTermRows, ldg].  Returns 0, -1 (operands), -3 (launch), -5 (tensor map).
+// x: packed rows [N, ldx]; x_all: the batch itself (nullptr: cannot be read in place); w: [cols, D] rows v0..; g: panels of 64
+// columns.  Returns 0, -1 (operands), -3 (launch), -5 (tensor map).
 int pcb_head_gemm(int mode, pcb::HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
-                  const void* w, long long ldw, void* g, long long ldg, int num_sms, cudaStream_t s);
+                  const void* w, long long ldw, void* g, int num_sms, cudaStream_t s);
