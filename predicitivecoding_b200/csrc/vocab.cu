@@ -218,27 +218,33 @@ __global__ void pad_rows_kernel(const __nv_bfloat16* __restrict__ src, long long
 
 // ---------------------------------------------------------------- the teacher's lists
 // One warp per row: the softmax of the entries present, and the entries in ascending id (rank = number of smaller
-// ids, ties by place), so that a thread of the GEMM's epilogue meets its row's targets in column order.
-__global__ void __launch_bounds__(kThreads)
+// ids, ties by place), so that a thread of the product's epilogue meets its row's targets in column order.  A lane
+// holds R entries; their ranks are counted together, four other entries at a time.
+constexpr int kSortRows = 4;   // rows (warps) per block
+
+template <int R>
+__global__ void __launch_bounds__(32 * kSortRows)
     sort_targets_kernel(const void* __restrict__ ids, int ids64, long long ld_ids, const void* __restrict__ logits,
                         int bf16, long long ld_logits, int N, int V, int K, float c, int* __restrict__ out_ids,
                         float* __restrict__ out_q, float* __restrict__ out_lq, int* __restrict__ out_len,
                         unsigned short* __restrict__ start, int granules) {
-  __shared__ int s_id[kThreads / 32][kMaxK];
-  __shared__ int s_sorted[kThreads / 32][kMaxK];
+  __shared__ __align__(16) int s_id[kSortRows][32 * R];
+  __shared__ int s_sorted[kSortRows][32 * R];
   pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = blockIdx.x * (kThreads / 32) + w;
+  const int n = blockIdx.x * kSortRows + w;
   if (n >= N) return;   // whole warps
-  int id[kMaxK / 32];
-  float y[kMaxK / 32];
+  constexpr int kAbsent = 0x7fffffff;   // behind every id
+  int id[R], rank[R];
+  float y[R];
   float mx = -INFINITY;
   int mine = 0;
 #pragma unroll
-  for (int r = 0; r < kMaxK / 32; ++r) {
+  for (int r = 0; r < R; ++r) {
     const int k = lane + 32 * r;
-    id[r] = -1;
+    id[r] = kAbsent;
     y[r] = -INFINITY;
+    rank[r] = 0;
     if (k < K) {
       const long long t = load_id(ids, ids64, n * ld_ids + k);
       const long long at = n * ld_logits + k;
@@ -249,51 +255,64 @@ __global__ void __launch_bounds__(kThreads)
         y[r] = l * c;
         ++mine;
       }
-      s_id[w][k] = id[r];
     }
+    s_id[w][k] = id[r];
     mx = fmaxf(mx, y[r]);
   }
   mx = warp_max(mx);
   float sum = 0.f;
 #pragma unroll
-  for (int r = 0; r < kMaxK / 32; ++r)
-    if (id[r] >= 0) sum += exp2f(y[r] - mx);
+  for (int r = 0; r < R; ++r)
+    if (id[r] != kAbsent) sum += exp2f(y[r] - mx);
   sum = warp_sum(sum);
   const int present = __reduce_add_sync(0xffffffffu, mine);
   const float ls = log2f(sum);
   __syncwarp();
+  for (int i = 0; i < K; i += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(&s_id[w][i]);
+    const int ov[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-  for (int r = 0; r < kMaxK / 32; ++r) {
-    if (id[r] < 0) continue;
-    const int k = lane + 32 * r;
-    int rank = 0;
-    for (int i = 0; i < K; ++i) {
-      const int o = s_id[w][i];
-      rank += o >= 0 && (o < id[r] || (o == id[r] && i < k)) ? 1 : 0;
-    }
-    s_sorted[w][rank] = id[r];
-    const long long at = (long long)n * K + rank;
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rank[r] += ov[e] < id[r] || (ov[e] == id[r] && i + e < lane + 32 * r) ? 1 : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (id[r] == kAbsent) continue;
+    s_sorted[w][rank[r]] = id[r];
+    const long long at = (long long)n * K + rank[r];
     out_ids[at] = id[r];
     out_q[at] = exp2f(y[r] - mx) / sum;
     out_lq[at] = y[r] - mx - ls;
   }
   __syncwarp();
   if (lane == 0) out_len[n] = present;
-  for (int g = lane; g <= granules; g += 32) {   // entries with an id below 128 g
-    int lo = 0, hi = present;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (s_sorted[w][mid] < g * 128LL) lo = mid + 1;
-      else hi = mid;
+  // entries with an id below 128 g, for every g: four searches at a time
+  for (int g0 = lane; g0 <= granules; g0 += 128) {
+    int lo[4] = {}, hi[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) hi[u] = present;
+    for (int span = present; span > 0; span >>= 1) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (lo[u] < hi[u]) {
+          const int mid = (lo[u] + hi[u]) >> 1;
+          if (s_sorted[w][mid] < (g0 + 32 * u) * 128LL) lo[u] = mid + 1;
+          else hi[u] = mid;
+        }
+      }
     }
-    start[(long long)g * N + n] = (unsigned short)lo;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (g0 + 32 * u <= granules) start[(long long)(g0 + 32 * u) * N + n] = (unsigned short)lo[u];
   }
 }
 
 // ---------------------------------------------------------------- row losses
-// 32 rows a block, 32 threads a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.
-// The last block to finish adds the losses up, in a fixed order and in 64 bits: scalars[0] = their sum or mean,
-// scalars[1] = 1 / counted rows (both 0 when there are none).
+// 32 rows a block, a warp a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.  The pairs
+// lie by row, so they are read with a row per lane and change hands through shared memory; the targets, which wait
+// for nothing, are read in the meantime.  The last block to finish adds the losses up, in a fixed order and in 64
+// bits: scalars[0] = their sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).
 constexpr int kLossParts = 32;
 
 __global__ void __launch_bounds__(32 * kLossParts)
@@ -301,55 +320,63 @@ __global__ void __launch_bounds__(32 * kLossParts)
                     const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
                     const int* __restrict__ len, int N, int K, float c, float factor, float* __restrict__ lse_out,
                     float* loss, int* count, int mean, float* __restrict__ scalars) {
-  __shared__ float sm[kLossParts][33], ss[kLossParts][33], sl[kLossParts][33];
+  __shared__ float sm[kLossParts][33], ss[kLossParts][33];
   __shared__ double sums[kLossParts];
   __shared__ int last;
   pdl_begin();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int j = blockIdx.x * 32 + tx;   // packed row
-  const bool live = j < min(count[0], N);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rows = min(count[0], N);
+  const int j = blockIdx.x * 32 + w;   // this warp's packed row
+  const bool live = j < rows;
   const int n = live ? row[j] : 0;
-  float m = -INFINITY, s = 0.f;
-  if (live) {
-#pragma unroll 4
-    for (int g = ty; g < granules; g += kLossParts) {
-      const float2 p = part[(long long)g * N + j];
-      const float nm = fmaxf(m, p.x);
-      const float ref = nm == -INFINITY ? 0.f : nm;
-      s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
-      m = nm;
-    }
+  // the first two targets of a lane: weight, and log2 q - c z
+  constexpr int kAhead = 2;
+  const int e = !live ? 0 : len != nullptr ? len[n] : 1;
+  const long long at_q = (long long)n * K, at_z = (long long)j * K;
+  float qk[kAhead], dk[kAhead];
+  auto target = [&](int k, float& weight, float& d) {
+    weight = q != nullptr ? q[at_q + k] : 1.f;
+    d = fmaf(-c, z[at_z + k], lq != nullptr ? lq[at_q + k] : 0.f);
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    qk[i] = dk[i] = 0.f;
+    if (lane + 32 * i < e) target(lane + 32 * i, qk[i], dk[i]);
   }
-  sm[ty][tx] = m;
-  ss[ty][tx] = s;
+  {
+    const int jl = blockIdx.x * 32 + lane;
+    float m = -INFINITY, s = 0.f;
+    if (jl < rows) {
+#pragma unroll 8
+      for (int g = w; g < granules; g += kLossParts) {
+        const float2 p = part[(long long)g * N + jl];
+        const float nm = fmaxf(m, p.x);
+        const float ref = nm == -INFINITY ? 0.f : nm;
+        s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+        m = nm;
+      }
+    }
+    sm[w][lane] = m;
+    ss[w][lane] = s;
+  }
   __syncthreads();
-  // warp ty joins the parts of column ty: lane = part
-  m = sm[tx][ty];
+  const float m = sm[lane][w];   // lane = part
   const float mm = warp_max(m);
   const float ref = mm == -INFINITY ? 0.f : mm;
-  const float tot = warp_sum(ss[tx][ty] * exp2f(m - ref));
-  __syncthreads();
-  if (tx == 0) sm[0][ty] = ref + log2f(tot);
-  __syncthreads();
-  const float lse = sm[0][tx];
-  // sum_k q_k (log2 q_k + lse - c z_k), term by term: each is a difference of logarithms of the same size
+  const float lse = ref + log2f(warp_sum(ss[lane][w] * exp2f(m - ref)));
+  // sum_k q_k (log2 q_k - c z_k + lse), term by term: each is a difference of logarithms of the same size
   float l = 0.f;
-  if (live) {
-    const long long at = (long long)n * K;
-    const int e = len != nullptr ? len[n] : 1;
-    for (int k = ty; k < e; k += kLossParts) {
-      const float d = fmaf(-c, z[(long long)j * K + k], lse);
-      if (q == nullptr) l += d;
-      else if (q[at + k] != 0.f) l += q[at + k] * (lq[at + k] + d);   // 0 log 0 = 0
-    }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (lane + 32 * i < e && qk[i] != 0.f) l += qk[i] * (dk[i] + lse);   // 0 log 0 = 0
+  for (int k = lane + 32 * kAhead; k < e; k += 32) {
+    float weight, d;
+    target(k, weight, d);
+    if (weight != 0.f) l += weight * (d + lse);
   }
-  sl[ty][tx] = l;
-  __syncthreads();
-  const float sum = warp_sum(sl[tx][ty]);
-  if (tx == 0) sl[0][ty] = sum;   // read by this warp only
-  __syncthreads();
-  if (ty == 0 && live) {
-    loss[n] = sl[0][tx] * factor;
+  l = warp_sum(l);
+  if (live && lane == 0) {
+    loss[n] = l * factor;
     lse_out[j] = lse;
   }
   if (scalars == nullptr) return;
@@ -363,14 +390,13 @@ __global__ void __launch_bounds__(32 * kLossParts)
   for (int i = threadIdx.x; i < N; i += 32 * kLossParts) t += __ldcg(loss + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (tx == 0) sums[ty] = t;
+  if (lane == 0) sums[w] = t;
   __syncthreads();
-  if (ty == 0) {
-    t = sums[tx];
+  if (w == 0) {
+    t = sums[lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (tx == 0) {
-      const int rows = count[0];
+    if (lane == 0) {
       scalars[0] = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
       scalars[1] = rows > 0 ? 1.f / (float)rows : 0.f;
     }
@@ -963,10 +989,18 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   unsigned short* start = distill ? (unsigned short*)at(saved, l.start) : nullptr;
   const float T = distill ? a.temperature : 1.f;
   const float c = 1.4426950408889634f / T;
-  if (distill &&
-      pdl_launch(sort_targets_kernel, dim3((a.N + 7) / 8), dim3(kThreads), 0, s, a.ids, a.ids64, a.ld_ids, a.logits,
-                 a.logits_bf16, a.ld_logits, a.N, a.V, a.K, c, ids, q, lq, len, start, l.granules) != cudaSuccess)
-    return -3;
+  if (distill) {
+    auto sort = [&](auto r) {
+      return pdl_launch(sort_targets_kernel<decltype(r)::value>, dim3((a.N + kSortRows - 1) / kSortRows),
+                        dim3(32 * kSortRows), 0, s, a.ids, a.ids64, a.ld_ids, a.logits, a.logits_bf16, a.ld_logits, a.N, a.V,
+                        a.K, c, ids, q, lq, len, start, l.granules);
+    };
+    const cudaError_t e = a.K <= 32    ? sort(std::integral_constant<int, 1>{})
+                          : a.K <= 64  ? sort(std::integral_constant<int, 2>{})
+                          : a.K <= 128 ? sort(std::integral_constant<int, 4>{})
+                                       : sort(std::integral_constant<int, 8>{});
+    if (e != cudaSuccess) return -3;
+  }
   PackArgs p{};
   p.tgt = a.tgt;
   p.tgt64 = a.tgt64;
