@@ -557,13 +557,11 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
   a.plan = pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), num_sms());
   a.ld_slab = (a.D + 3) / 4 * 4;
   const int64_t gbytes = (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
-  const int64_t dx_slab = dx ? (int64_t)a.plan.slab_rows * a.ld_slab : 0;
-  const int64_t dw_slab = dw && a.plan.dw_max > 1 ? (int64_t)a.plan.dw_max * st.V * a.ld_slab : 0;
-  at::Tensor ws = at::empty({gbytes + 4 * (dx_slab + dw_slab)}, st.saved.options());
+  const bool slabs = dx || a.plan.dw_max > 1;
+  at::Tensor ws = at::empty({gbytes + (slabs ? 4 * a.plan.all_rows * a.ld_slab : 0)}, st.saved.options());
   a.g = ws.data_ptr();
-  a.dx_slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
-  a.dw_slab = a.dx_slab + dx_slab;
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", 2 * a.plan.pieces + (dx || dw_slab ? 1 : 0));
+  if (slabs) a.slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", 2 * a.plan.pieces + (slabs ? 1 : 0));
   return {dx, dw};
 }
 

@@ -423,8 +423,8 @@ __global__ void __launch_bounds__(32 * kLossParts)
 constexpr int kFinishVecs = 4;
 
 struct FinishArgs {
-  const float* dx_slab;
-  const float* dw_slab;
+  const float* slab;
+  int slab_rows;         // of dx, dw's behind them
   const int* count;
   const int* plan;       // K splits of dw and dx
   const int* pos;
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a) {
   if (a.scale != nullptr) f *= *a.scale;
   if (a.scale2 != nullptr) f *= *a.scale2;
   const int d0 = (blockIdx.y * kFinishVecs * 32 + (threadIdx.x & 31)) * VEC;
-  const float* src = (w ? a.dw_slab : a.dx_slab) + (long long)max(j, 0) * a.ld_slab + d0;
-  const long long stride = (w ? a.V : (max(a.count[0], 1) + 255) / 256 * 256) * a.ld_slab;
+  const float* src = a.slab + ((long long)max(j, 0) + (w ? a.slab_rows : 0)) * a.ld_slab + d0;
+  const long long stride = ((w ? a.V : max(a.count[0], 1)) + 255) / 256 * 256 * a.ld_slab;
   float v[kFinishVecs][VEC] = {};
   if (j >= 0) {
     for (int k = 0; k < slabs; ++k, src += stride) {
@@ -970,6 +970,7 @@ VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms) {
   const long long tiles = p / 256 * ((D + bn - 1) / bn);
   r.dw_max = r.pieces == 1 ? (int)std::max(1LL, std::min(8LL, num_sms / 2 / tiles)) : 1;
   r.slab_rows = (int)std::min((N + 255LL) / 256 * 256 + 16 * 256, 1LL << 30);
+  r.all_rows = r.slab_rows + (r.dw_max > 1 ? r.dw_max * all : 0);
   return r;
 }
 
@@ -1096,8 +1097,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   g.alpha = a.gout * T;
   g.scale = a.mean ? a.scalars + 1 : nullptr;
   g.scale2 = a.gout_dev;
-  g.dx_slab = a.dx_slab;
-  g.dw_slab = a.dw_slab;
+  g.slab = a.slab;
   g.ld_slab = a.ld_slab;
   for (int v0 = 0; v0 < a.V; v0 += a.plan.piece) {
     g.v0 = v0;
@@ -1111,8 +1111,8 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     }
   }
   FinishArgs f{};
-  f.dx_slab = a.dx_slab;
-  f.dw_slab = a.dw_slab;
+  f.slab = a.slab;
+  f.slab_rows = a.plan.slab_rows;
   f.count = g.count;
   f.plan = g.plan;
   f.pos = (const int*)at(sv, l.pos);

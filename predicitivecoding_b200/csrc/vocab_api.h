@@ -53,7 +53,8 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill);
 struct VocabPlan {
   int piece, pieces;
   int dw_max;            // most K splits of the dw product
-  int slab_rows;         // rows of dx_slab
+  int slab_rows;         // rows of the fp32 slabs that dx takes
+  long long all_rows;    // with those of dw
 };
 VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms);
 
@@ -79,8 +80,7 @@ struct VocabGradArgs {
   int dw_add;
   VocabPlan plan;
   void* g;               // workspace: bf16, vocab_g_rows(N) * piece
-  float* dx_slab;        // workspace: fp32 [slab_rows, ld_slab]
-  float* dw_slab;        // workspace: fp32 [dw_max, V, ld_slab] when dw_max > 1
+  float* slab;           // workspace: fp32 [all_rows, ld_slab]
   long long ld_slab;
 };
 long long vocab_g_rows(int N);

@@ -99,14 +99,20 @@ PCB_DEVICE void plan_splits(const HeadGemm& a, int rows, int pairs, int* plan) {
 template <int MODE, int BN>
 PCB_DEVICE Shape shape_of(const HeadGemm& a, int pairs) {
   Shape s;
-  s.rows = min(*a.count, a.N);
+  const int count = *a.count;
+  int plan_dw = 0, plan_dx = 0;
+  if (MODE == HEAD_BWD) {   // asked for together
+    plan_dw = a.plan[0];
+    plan_dx = a.plan[1];
+  }
+  s.rows = min(count, a.N);
   const int r = max(s.rows, 1);   // one tile at least: gradients of a batch without counted rows are zeros
   s.num_m = (r + 2 * kBM - 1) / (2 * kBM);
   s.two = MODE != HEAD_STAT && s.rows <= kTwoTermRows;
   s.dw_tiles = s.kb_dw = s.dx_more = s.dx_least = s.catch_up = s.dw_splits = s.dx_splits = 0;
   if (MODE == HEAD_BWD) {
-    if (a.want_dw) s.dw_splits = a.plan[0];
-    if (a.want_dx) s.dx_splits = a.plan[1];
+    if (a.want_dw) s.dw_splits = plan_dw;
+    if (a.want_dx) s.dx_splits = plan_dx;
     s.num_n = (a.D + BN - 1) / BN;
     s.kb_dw = (r + kBK - 1) / kBK;
     s.kb_dx = (a.cols + kBK - 1) / kBK;
@@ -198,15 +204,19 @@ PCB_DEVICE float pick32(const float (&v)[32], int o) {
 }
 
 // One packed row's part of the target list: the entries whose ids fall in this thread's 128 columns.  Its loads depend on
-// one another (row -> first entry -> id): each of the three steps only asks, and the next one, 32 columns of
-// arithmetic later, uses the answer.
+// one another (row -> first entry -> ids): each of the three steps only asks, and the next one, 32 columns of
+// arithmetic later, uses the answer.  The next kAhead entries are kept in registers, so that one is asked for long
+// before it is met.
 struct RowTargets {
+  static constexpr int kAhead = 4;
+  static constexpr int kNone = 0x7fffffff;
   bool live;        // a counted row
   float lse;
   int n, m;         // the row's place in the batch and among the packed rows
   int lo;           // vocabulary id of the first of the 128 columns
-  int entry, left;  // next entry of the row's list, entries left in these columns
-  int next;         // its column relative to `lo`; past the 128 when none is left
+  int entry, end;   // next entry of the row's list, and the first behind these columns
+  int id[kAhead];   // its id and those behind it; kNone behind `end`
+  float q[kAhead];  // their weights (GRAD)
 
   template <int MODE>
   PCB_DEVICE void ask_row(const HeadGemm& h, int packed, int col0, int rows) {
@@ -222,25 +232,43 @@ struct RowTargets {
     if (!live) n = 0;   // with no row counted at all there is no first one either
     const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
     entry = s[0];
-    left = s[h.N];
+    end = s[h.N];
   }
-  PCB_DEVICE void ask_next(const HeadGemm& h) {
+  template <int MODE>
+  PCB_DEVICE void ask_ids(const HeadGemm& h) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      id[i] = kNone;
+      q[i] = 1.f;
+    }
     if (h.start == nullptr) {
-      const int t = n - lo;
-      left = live && t >= 0 && t < 128 ? 1 : 0;
-      entry = n = 0;
-      next = left > 0 ? t + lo : 0;
+      if (live && n >= lo && n < lo + 128) id[0] = n;
+      entry = n = end = 0;
     } else {
-      left = live ? left - entry : 0;
-      next = left > 0 ? h.ids[(long long)n * h.K + entry] : 0;
+      if (!live) end = entry;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fill<MODE>(h, i);
     }
   }
-  PCB_DEVICE void settle() { next = left > 0 ? next - lo : 1 << 30; }
-  PCB_DEVICE float weight(const HeadGemm& h) const { return h.q != nullptr ? h.q[(long long)n * h.K + entry] : 1.f; }
+  template <int MODE>
+  PCB_DEVICE void fill(const HeadGemm& h, int i) {   // slot i: entry + i
+    id[i] = kNone;
+    if (entry + i < end) {
+      const long long at = (long long)n * h.K + entry + i;
+      id[i] = h.ids[at];
+      if (MODE == HEAD_GRAD) q[i] = h.q[at];
+    }
+  }
   PCB_DEVICE float* z(const HeadGemm& h) const { return h.z + (long long)m * h.K + entry; }
+  template <int MODE>
   PCB_DEVICE void advance(const HeadGemm& h) {
     ++entry;
-    next = --left > 0 ? h.ids[(long long)n * h.K + entry] - lo : 1 << 30;
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) {
+      id[i] = id[i + 1];
+      q[i] = q[i + 1];
+    }
+    fill<MODE>(h, kAhead - 1);
   }
 };
 
@@ -280,16 +308,19 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
   float mx = -INFINITY, sum = 0.f;
   uint32_t buf[2][32];
   tmem_ld_32x32b_x32(taddr, buf[0]);
+#pragma unroll 1
+  for (int ii = 0; ii < 4; ii += 2)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    wait32(buf[i & 1]);
-    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
+  for (int i2 = 0; i2 < 2; ++i2) {
+    const int i = ii + i2;
+    wait32(buf[i2]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[i2 ^ 1]);
     float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[i & 1][j]);
-    while (r.next < 32 * (i + 1)) {
-      *r.z(a) = pick32(v, r.next - 32 * i);
-      r.advance(a);
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[i2][j]);
+    while (r.id[0] < r.lo + 32 * (i + 1)) {
+      *r.z(a) = pick32(v, r.id[0] - r.lo - 32 * i);
+      r.advance<HEAD_STAT>(a);
     }
     __syncwarp();
     const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
@@ -334,14 +365,17 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
   uint32_t buf[2][32];
   uint32_t hi[32], low[TWO ? 32 : 1];
   tmem_ld_32x32b_x32(taddr, buf[0]);
+#pragma unroll 1
+  for (int ii = 0; ii < 4; ii += 2)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    wait32(buf[i & 1]);
-    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
+  for (int i2 = 0; i2 < 2; ++i2) {
+    const int i = ii + i2;
+    wait32(buf[i2]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[i2 ^ 1]);
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      scale2(v[j], v[j + 1], __uint_as_float(buf[i & 1][j]), __uint_as_float(buf[i & 1][j + 1]), a.c, -r.lse);
+      scale2(v[j], v[j + 1], __uint_as_float(buf[i2][j]), __uint_as_float(buf[i2][j + 1]), a.c, -r.lse);
       v[j] = ex2_approx(v[j]);
       v[j + 1] = ex2_approx(v[j + 1]);
     }
@@ -354,21 +388,21 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : 0.f;
     }
-    while (r.next < 32 * (i + 1)) {
-      const int o = r.next - 32 * i;
-      const float q = r.weight(a);
+    while (r.id[0] < r.lo + 32 * (i + 1)) {
+      const int o = r.id[0] - r.lo - 32 * i;
+      const float q = r.q[0];
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] -= j == o ? q : 0.f;
-      r.advance(a);
+      r.advance<HEAD_GRAD>(a);
     }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const uint32_t p = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-      hi[16 * (i & 1) + j] = p;
-      if constexpr (TWO) low[16 * (i & 1) + j] = pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p));
+      hi[16 * i2 + j] = p;
+      if constexpr (TWO) low[16 * i2 + j] = pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p));
     }
-    if (i & 1) {
+    if (i2 == 1) {
       store(i >> 1, hi, false);
       if constexpr (TWO) store(i >> 1, low, true);
     }
@@ -377,6 +411,14 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 }
 
 // ---------------------------------------------------------------- stores
+// TMA store that adds the fp32 box to what is there; one launch adds to a place once
+PCB_DEVICE void tma_add_2d(const CUtensorMap* map, const void* smem_src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
 // a lane's 64 bf16 as its row of the 128-byte-swizzled [32 x 64] box, written by one TMA store; the two boxes of a warp
 // alternate
 PCB_DEVICE void store_box64(const CUtensorMap* map, uint8_t* stg, int& box_at, const uint32_t (&pk)[32], int col, int row,
@@ -429,12 +471,13 @@ PCB_DEVICE void store4(__nv_bfloat16* c, float (&o)[4], int nv, bool add) {
 }
 
 // ---------------------------------------------------------------- kernel
-// STAT, GRAD: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x.
+// STAT, GRAD: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x,
+// tmS = fp32 slabs.
 template <int MODE, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
-                const __grid_constant__ CUtensorMap tmX, const HeadGemm a) {
+                const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmS, const HeadGemm a) {
   using C = Cfg<MODE, BN>;
   constexpr int STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -469,7 +512,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
     if (MODE != HEAD_STAT) prefetch_tmap(&tmC);
-    if (MODE == HEAD_BWD) prefetch_tmap(&tmD);
+    if (MODE == HEAD_BWD) {
+      prefetch_tmap(&tmD);
+      prefetch_tmap(&tmS);
+    }
     prefetch_tmap(&tmX);
   }
   if (warp == 1) {
@@ -578,14 +624,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, 0, tile)) {
       ahead.template ask_row<MODE>(a, tile.mb * 2 * kBM + rank * kBM + q * 32 + lane, tile.nb * BN + half * 128, sh.rows);
       ahead.ask_entries(a);
-      ahead.ask_next(a);
+      ahead.template ask_ids<MODE>(a);
     }
     for (int u = 0; tile_at<MODE>(a, sh, pair_id, num_pairs, u, tile); ++u) {
       const int row0 = tile.mb * 2 * kBM + rank * kBM + q * 32;
       const int n0 = tile.nb * BN;
       // the next tile's rows and targets are fetched under this one's arithmetic
       RowTargets r = ahead;
-      if (MODE != HEAD_BWD) r.settle();
       int row0_next = 0, n0_next = 0, rows_next = 0;
       Tile after;
       if (MODE != HEAD_BWD && tile_at<MODE>(a, sh, pair_id, num_pairs, u + 1, after)) {
@@ -596,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto between = [&](int i) {
         if (i == 0) ahead.template ask_row<MODE>(a, row0_next + lane, n0_next + half * 128, rows_next);
         if (i == 1) ahead.ask_entries(a);
-        if (i == 2) ahead.ask_next(a);
+        if (i == 2) ahead.template ask_ids<MODE>(a);
       };
       if (!mbar_wait(&tfull[acc], acc_phase, nullptr, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
@@ -627,27 +672,46 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           store_box64(&tmC, stg, box_at, pk, col, row0, lane);
         }
-      } else {
-        // fp32 slabs, and the gradients of the weights that no TMA store takes: each 32 x 32 chunk goes through this
-        // warp's scratch (16-byte cells, XOR-swizzled by row), then 8 lanes write one row segment
-        float4* scr = reinterpret_cast<float4*>(stg);
+      } else if (!tile.dw || sh.dw_splits > 1) {
+        // fp32 slabs: [32 x 32] boxes of 128-byte rows, stored (or, behind the first piece of the vocabulary, added) by
+        // TMA; the rows up to the next multiple of 256 belong to the slab
+        const int at = tile.dw ? a.slab_rows + tile.split * ((a.cols + 255) / 256 * 256) : tile.split * (sh.num_m * 256);
         const bool none = tile.kb0 == tile.kb1;   // a split without k-blocks: nothing was accumulated
-        const int rows = tile.dw ? a.cols : sh.rows;
-        const bool slab = !tile.dw || sh.dw_splits > 1;
-        float* base = !tile.dw ? a.dx_slab + (long long)tile.split * (sh.num_m * 256) * a.ld_slab
-                      : slab   ? a.dw_slab + (long long)tile.split * a.cols * a.ld_slab
-                               : (float*)a.dw;
-        const long long ld = slab ? a.ld_slab : a.lddw;
-        const bool add = tile.dw ? !slab && a.dw_add : a.dx_add;
-        const float f = slab ? 1.f : scale;
+#pragma unroll 1
+        for (int c = half; c < BN / 32; c += 2) {
+          const int col = n0 + c * 32;
+          if (col >= a.D) break;   // warp-uniform
+          float v[32];
+          load32(tbase + c * 32, v);
+          uint8_t* box = stg + box_at * 4096;
+          box_at ^= 1;
+          if (lane == 0) bulk_group_wait_read<1>();   // the store that last read this box is done with it
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (!tile.dw && a.dx_add) tma_add_2d(&tmS, box, col, at + row0);
+            else tma_store_2d(&tmS, box, col, at + row0);
+            bulk_group_commit();
+          }
+        }
+      } else {
+        // gradients of the weights that no TMA store takes (fp32, added to, rows not 16-byte aligned): each 32 x 32 chunk
+        // goes through this warp's scratch (16-byte cells, XOR-swizzled by row), then 8 lanes write one row segment
+        float4* scr = reinterpret_cast<float4*>(stg);
+        if (lane == 0) bulk_group_wait_read<0>();   // TMA stores of earlier tiles read the same memory
+        __syncwarp();
 #pragma unroll 1
         for (int c = half; c < BN / 32; c += 2) {
           float v[32];
           load32(tbase + c * 32, v);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            scr[lane * 8 + (j ^ (lane & 7))] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                    : make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            scr[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           __syncwarp();
           const int c4 = lane & 7, col = n0 + c * 32 + c4 * 4;
           const int nv = min(4, a.D - col);
@@ -655,10 +719,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int it = 0; it < 8; ++it) {
             const int rr = it * 4 + (lane >> 3), m = row0 + rr;
             const float4 x = scr[rr * 8 + (c4 ^ (rr & 7))];
-            float e[4] = {f * x.x, f * x.y, f * x.z, f * x.w};
-            if (m < rows && nv > 0) {
-              if (slab || a.dw_f32) store4(base + m * ld + col, e, nv, add);
-              else store4(reinterpret_cast<__nv_bfloat16*>(a.dw) + m * ld + col, e, nv, add);
+            float e[4] = {scale * x.x, scale * x.y, scale * x.z, scale * x.w};
+            if (m < a.cols && nv > 0) {
+              if (a.dw_f32) store4(reinterpret_cast<float*>(a.dw) + m * a.lddw + col, e, nv, a.dw_add);
+              else store4(reinterpret_cast<__nv_bfloat16*>(a.dw) + m * a.lddw + col, e, nv, a.dw_add);
             }
           }
           __syncwarp();
@@ -696,21 +760,22 @@ static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// bf16 [outer, inner] rows of stride ld, boxes of [rows, 64] with the 128-byte swizzle
-static bool map2(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int rows) {
+// [outer, inner] rows of stride ld, bf16 in boxes of [rows, 64] or fp32 in boxes of [rows, 32], with the 128-byte swizzle
+static bool map2(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int rows,
+                 bool f32 = false) {
   auto fn = encoder();
-  if (fn == nullptr || !((reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % 8 == 0)) return false;
+  if (fn == nullptr || !((reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % (f32 ? 4 : 8) == 0)) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, (cuuint32_t)rows};   // 128 bytes wide
   const cuuint32_t es[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es,
+  return fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int MODE, int BN>
-static int launch(const CUtensorMap (&t)[5], const HeadGemm& a, int tiles, int num_sms, cudaStream_t s) {
+static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int num_sms, cudaStream_t s) {
   using C = Cfg<MODE, BN>;
   static bool attr_done = false;
   if (!attr_done) {
@@ -732,7 +797,7 @@ static int launch(const CUtensorMap (&t)[5], const HeadGemm& a, int tiles, int n
   attr[1].val.programmaticStreamSerializationAllowed = pdl_env_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, head_kernel<MODE, BN>, t[0], t[1], t[2], t[3], t[4], a) == cudaSuccess ? 0 : -3;
+  return cudaLaunchKernelEx(&cfg, head_kernel<MODE, BN>, t[0], t[1], t[2], t[3], t[4], t[5], a) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace head
@@ -745,7 +810,7 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
                   const void* w, long long ldw, void* g, int num_sms, cudaStream_t s) {
   if (a.N < 1 || a.D < 1 || a.cols < 1 || num_sms < 2) return -1;
   a.bwd_pairs = num_sms / 2;   // tiles of the gradients are split until there are enough; a pair without one ends at once
-  CUtensorMap t[5];
+  CUtensorMap t[6];
   memset(t, 0, sizeof(t));
   const int num_m = (a.N + 255) / 256;
   const bool bwd = mode == HEAD_BWD;
@@ -766,6 +831,9 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
     return mode == HEAD_STAT ? launch<HEAD_STAT, 256>(t, a, tiles, num_sms, s) : launch<HEAD_GRAD, 256>(t, a, tiles, num_sms, s);
   }
   if (!map2(&t[0], g, 64, panels * a.g_rows, 64, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
+  const long long slab_rows = a.slab_rows + (a.dw_max > 1 ? (long long)a.dw_max * ((a.cols + 255) / 256 * 256) : 0);
+  if (a.slab == nullptr) t[5] = t[0];
+  else if (!map2(&t[5], a.slab, a.D, slab_rows, a.ld_slab, 32, true)) return -5;
   a.dw_tma = a.want_dw && !a.dw_f32 && !a.dw_add && map2(&t[2], a.dw, a.D, a.cols, a.lddw, 32);
   if (!a.dw_tma) t[2] = t[0];
   const int bn = head_bn(a.D);

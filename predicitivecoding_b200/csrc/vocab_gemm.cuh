@@ -45,17 +45,18 @@ struct HeadGemm {
   int want_dw, want_dx;
   int bwd_pairs;          // pairs of CTAs of the BWD launch (set by pcb_head_gemm)
   int dw_max;             // most splits of dw
-  int slab_rows;          // rows of dx_slab: its splits times the counted rows, rounded up to 256, fit in
+  int slab_rows;          // rows of dx's slabs: its splits times the counted rows, rounded up to 256, fit in
   void* dw;               // [cols, D], row stride lddw (unsplit)
   long long lddw;
   int dw_f32, dw_add, dw_tma;
   float alpha;            // dw *= alpha * scale * scale2 (not the slabs)
   const float* scale;
   const float* scale2;
-  float* dx_slab;         // [splits][counted rows rounded up to 256, ld_slab], packed rows
-  int dx_add;
-  float* dw_slab;         // [splits][cols, ld_slab] when dw is split
+  // fp32 slabs, rows of ld_slab (nullptr: neither needs one): dx's, packed rows rounded up to 256 for each split; from row
+  // slab_rows on dw's, when it may be split, cols rounded up to 256 for each split
+  float* slab;
   long long ld_slab;
+  int dx_add;             // add to dx's slabs instead of writing them
 };
 
 // Columns of a tile of the gradients' products: 128 where 256 would leave an eighth or more of the columns empty.
