@@ -308,16 +308,13 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
   float mx = -INFINITY, sum = 0.f;
   uint32_t buf[2][32];
   tmem_ld_32x32b_x32(taddr, buf[0]);
-#pragma unroll 1
-  for (int ii = 0; ii < 4; ii += 2)
 #pragma unroll
-  for (int i2 = 0; i2 < 2; ++i2) {
-    const int i = ii + i2;
-    wait32(buf[i2]);
-    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[i2 ^ 1]);
+  for (int i = 0; i < 4; ++i) {
+    wait32(buf[i & 1]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[i2][j]);
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(buf[i & 1][j]);
     while (r.id[0] < r.lo + 32 * (i + 1)) {
       *r.z(a) = pick32(v, r.id[0] - r.lo - 32 * i);
       r.advance<HEAD_STAT>(a);
@@ -365,17 +362,14 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
   uint32_t buf[2][32];
   uint32_t hi[32], low[TWO ? 32 : 1];
   tmem_ld_32x32b_x32(taddr, buf[0]);
-#pragma unroll 1
-  for (int ii = 0; ii < 4; ii += 2)
 #pragma unroll
-  for (int i2 = 0; i2 < 2; ++i2) {
-    const int i = ii + i2;
-    wait32(buf[i2]);
-    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[i2 ^ 1]);
+  for (int i = 0; i < 4; ++i) {
+    wait32(buf[i & 1]);
+    if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      scale2(v[j], v[j + 1], __uint_as_float(buf[i2][j]), __uint_as_float(buf[i2][j + 1]), a.c, -r.lse);
+      scale2(v[j], v[j + 1], __uint_as_float(buf[i & 1][j]), __uint_as_float(buf[i & 1][j + 1]), a.c, -r.lse);
       v[j] = ex2_approx(v[j]);
       v[j + 1] = ex2_approx(v[j + 1]);
     }
@@ -399,10 +393,10 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const uint32_t p = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-      hi[16 * i2 + j] = p;
-      if constexpr (TWO) low[16 * i2 + j] = pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p));
+      hi[16 * (i & 1) + j] = p;
+      if constexpr (TWO) low[16 * (i & 1) + j] = pack_bf16x2(v[2 * j] - bf16_lo(p), v[2 * j + 1] - bf16_hi(p));
     }
-    if (i2 == 1) {
+    if (i & 1) {
       store(i >> 1, hi, false);
       if constexpr (TWO) store(i >> 1, low, true);
     }
