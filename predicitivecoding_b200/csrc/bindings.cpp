@@ -5,6 +5,7 @@
 // argument or a launch error.  No entry point allocates device memory except
 // where the docstring says so.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 #include <pybind11/stl.h>
@@ -386,7 +387,19 @@ struct HeadState {
   int64_t N, V, D, K;
   bool distill, mean, none;
   double temperature;
+  // 0, or the code of a bounded wait that ran out in a kernel of this loss (reads device memory: synchronises)
+  int64_t status() const {
+    if (N == 0) return 0;
+    const int64_t at = pcb::vocab_layout(N, V, D, K, distill).count / 4 + 4;
+    return saved.view(at::kInt)[at].item<int>();
+  }
 };
+
+// memory of `t` may be used by work on this stream until that is done, wherever it was allocated
+void used_here(const at::Tensor& t) {
+  if (t.defined())
+    c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), at::cuda::getCurrentCUDAStream());
+}
 
 // Loss of the vocabulary head: x [..., D], w [V, D] bf16; either targets [...] or ids, logits [..., K].  Allocates the
 // loss (a scalar, or one per row), what the gradients need, and w as the GEMMs read it when its rows are not 16-byte
@@ -530,6 +543,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     return {dx, dw};
   }
   if (!dx && !dw) return {dx, dw};
+  for (const at::Tensor& t : {st.saved, st.scalars, st.x, st.w}) used_here(t);
   a.x = st.x.data_ptr();
   a.ldx = rows_apart(st.x);
   a.w = st.w.data_ptr();
@@ -1259,7 +1273,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_readonly("D", &HeadState::D)
       .def_readonly("K", &HeadState::K)
       .def_readonly("distill", &HeadState::distill)
-      .def_readonly("temperature", &HeadState::temperature);
+      .def_readonly("temperature", &HeadState::temperature)
+      .def("status", &HeadState::status);
   m.def("vocab_ce_fwd", &vocab_ce_fwd);
   m.def("vocab_distill_fwd", &vocab_distill_fwd);
   m.def("vocab_head_bwd", &vocab_head_bwd);

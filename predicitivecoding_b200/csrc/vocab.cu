@@ -13,7 +13,7 @@
 // the products run over their number, known on the device only, and what stands in the other rows (NaN too) is
 // never read.  When all rows are counted the products read x itself.
 #include <algorithm>
-#include <cstdio>
+#include <type_traits>
 
 #include "common.cuh"
 #include "vocab_api.h"
@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(PackArgs a, int R) 
     if (threadIdx.x == 0) {
       a.count[0] = base;
       a.count[1] = 0;   // blocks of row_loss_kernel that are done
+      a.count[4] = 0;   // status
     }
     const int end = min(a.N, (max(base, 1) + 63) / 64 * 64);
     for (int j = base + (threadIdx.x >> 5); j < end; j += kThreads / 32) zero_or_copy(-1, j);
@@ -937,7 +938,7 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
   l.ldxc = (D + 7) / 8 * 8;
   l.granules = 2 * ((V + 255) / 256);
   l.xc = take((long long)N * l.ldxc * 2);
-  l.count = take(16);
+  l.count = take(32);
   l.row = take(4LL * N);
   l.pos = take(4LL * N);
   l.lse = take(4LL * N);
@@ -1052,6 +1053,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   g.D = a.D;
   g.cols = a.V;
   g.count = count;
+  g.err = count + 4;
   g.c = c;
   g.row = row;
   g.ids = ids;
@@ -1075,6 +1077,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   g.N = a.N;
   g.D = a.D;
   g.count = (const int*)at(sv, l.count);
+  g.err = (int*)at(sv, l.count) + 4;
   g.c = 1.4426950408889634f / T;
   g.row = (const int*)at(sv, l.row);
   g.ids = (const int*)at(sv, l.ids);
@@ -1185,12 +1188,8 @@ template <int ITEMS>
 static int launch_cluster_sort(const void* tok, int tok64, int N, int V, int bits, uint32_t* keys, uint32_t* idx, int* list,
                                void* zeros, long long zero_bytes, int num_sms, cudaStream_t s) {
   constexpr int smem = cluster_sort_smem<ITEMS>();
-  static bool attr_done = false;
-  if (!attr_done) {
-    if (cudaFuncSetAttribute(cluster_sort_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return -3;
-    attr_done = true;
-  }
+  static SmemLimit limit;
+  if (!limit.raise(cluster_sort_kernel<ITEMS>, smem)) return -3;
   // as many more clusters as there is for them to write, 64 KB a block, up to 7 blocks an SM: of 131 MB (4096 tokens, V
   // 32000, D 2048) 16 clusters made 55 us of the gradient, 34 made 44, 128 made 38 and 512 made 41
   const int most = 7 * num_sms / kCluster;

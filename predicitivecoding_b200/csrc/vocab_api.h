@@ -34,7 +34,7 @@ struct VocabHeadArgs {
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;
-  long long count;   // int [4]: counted rows, finished blocks of the loss kernel, K splits of dw and dx
+  long long count;   // int [5]: counted rows, finished blocks of the loss kernel, K splits of dw and dx, status of a wait
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
   long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature, by packed row

@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int m0 = tile.mb * 2 * kBM + rank * kBM;
         const int n0 = tile.nb * BN + rank * (BN / 2);
         for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, nullptr, kErrTimeoutEmpty, abort_flag)) { ok = false; break; }
+          if (!mbar_wait(&empty[stage], phase ^ 1u, a.err, kErrTimeoutEmpty, abort_flag)) { ok = false; break; }
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE_BYTES);
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
           uint8_t* sb = sa + C::A_BYTES;
@@ -578,11 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t b0 = make_smem_desc(smem_u32(smem) + C::A_BYTES, b_mn ? 8192 : 16, 1024, 2);
         const uint32_t a_step = a_mn ? 2048 / 16 : 32 / 16;
         constexpr uint32_t b_step = b_mn ? 2048 / 16 : 32 / 16;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, nullptr, kErrTimeoutTmemEmpty, abort_flag)) { ok = false; break; }
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, a.err, kErrTimeoutTmemEmpty, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
         for (int kb = tile.kb0; kb < tile.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, nullptr, kErrTimeoutFull, abort_flag)) { ok = false; break; }
+          if (!mbar_wait(&full[stage], phase, a.err, kErrTimeoutFull, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const uint64_t ad = a0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
           const uint64_t bd = b0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i == 1) ahead.ask_entries(a);
         if (i == 2) ahead.template ask_ids<MODE>(a);
       };
-      if (!mbar_wait(&tfull[acc], acc_phase, nullptr, kErrTimeoutTmemFull, abort_flag)) break;
+      if (!mbar_wait(&tfull[acc], acc_phase, a.err, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if (MODE == HEAD_STAT) {
@@ -771,12 +771,8 @@ static bool map2(CUtensorMap* m, const void* ptr, long long inner, long long out
 template <int MODE, int BN>
 static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int num_sms, cudaStream_t s) {
   using C = Cfg<MODE, BN>;
-  static bool attr_done = false;
-  if (!attr_done) {
-    if (cudaFuncSetAttribute(head_kernel<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) != cudaSuccess)
-      return -3;
-    attr_done = true;
-  }
+  static SmemLimit limit;
+  if (!limit.raise(head_kernel<MODE, BN>, C::SMEM_BYTES)) return -3;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * std::min(tiles, num_sms / 2), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);

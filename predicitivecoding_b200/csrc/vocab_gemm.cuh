@@ -1,5 +1,7 @@
 // Products of the vocabulary head (csrc/vocab_gemm.cu): what one launch reads and writes.
 #pragma once
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 namespace pcb {
@@ -9,6 +11,20 @@ namespace pcb {
 // one that the bf16 result takes anyway.  It is the rows of one tile: the second term costs one more pass of
 // matrix instructions over a tile that reading the weights bounds.
 constexpr int kTwoTermRows = 256;
+
+// Raises a kernel's limit of dynamic shared memory, once on each device.
+struct SmemLimit {
+  std::atomic<unsigned long long> done{0};
+  template <typename F>
+  bool raise(F* kernel, int bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return false;
+    if ((done.load(std::memory_order_relaxed) >> dev) & 1) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return true;
+  }
+};
 
 enum HeadMode : int {
   HEAD_STAT = 0,   // logits -> (max, sum) of every 128 of a row, and the logits at its targets
@@ -21,6 +37,7 @@ struct HeadGemm {
   int cols;               // columns of the vocabulary in this launch
   int v0;                 // the first of them (a multiple of 256)
   const int* count;       // device: counted rows, packed in front
+  int* err;               // device: status of a wait that ran out (0: none)
   int dense;              // x itself may be read in place of the packed rows when all are counted
   float c;                // log2(e) / temperature: exponents are taken to base 2
   int row_blocks_last;    // order of tiles: 1 = the column blocks of one row block run side by side

@@ -4,6 +4,10 @@ Reference: PredictiveCoding.LLM/Training/LmDistiller.cs:29-166.  ``build_dataset
 teacher for the completion of every prompt (optionally cached on disk as JSONL); ``step``
 trains on prompt + completion with the loss masked to the completion; ``on_policy_round``
 lets the student draft, asks the teacher for a corrected completion, and trains on it.
+
+``TopLogitDistiller`` is the token-level form, which the reference has not: the student learns the teacher's top
+logits at every position, next to the usual targets.  On a GPU neither loss holds the student's logits
+(:mod:`predicitivecoding_b200.ops.vocab`).
 """
 from __future__ import annotations
 
@@ -14,7 +18,9 @@ from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 
-from ..optim.adam import Adam
+from ..models.decoder_lm import DecoderLM
+from ..ops import vocab
+from ..optim.adam import Adam, clip_global_norm
 from .generation import greedy
 from .trainer import step as adam_step
 
@@ -68,3 +74,59 @@ def on_policy_round(model, tok, prompts: Sequence[str], teacher_correct: Callabl
         draft = tok.decode(out[len(ids):])
         data.append((p, teacher_correct(p, draft)))
     return step(model, tok, data, optimizer, lr, clip_norm)
+
+
+class TopLogitDistiller:
+    """Trains ``student`` on a teacher's top logits.
+
+    loss = alpha * T^2 KL(q || p_T) + (1 - alpha) * cross entropy, q the softmax of the teacher's ``top_k`` logits at
+    temperature T, p_T the student's softmax at T over its whole vocabulary.  Both means run over the positions whose
+    target is not ``ignore_index``.  ``embed_scale`` multiplies the student's embedding rows.
+    """
+
+    def __init__(self, student: DecoderLM, top_k: int = 32, temperature: float = 2.0, alpha: float = 0.5,
+                 embed_scale: float = 1.0, ignore_index: int = -1):
+        if not 1 <= top_k <= min(vocab.MAX_TOP_K, student.cfg.vocab):
+            raise ValueError(f"top_k must be between 1 and {min(vocab.MAX_TOP_K, student.cfg.vocab)}")
+        if temperature <= 0:
+            raise ValueError("temperature must be positive")
+        if not 0.0 <= alpha <= 1.0:
+            raise ValueError("alpha must be between 0 and 1")
+        self.student, self.top_k, self.temperature = student, top_k, float(temperature)
+        self.alpha, self.embed_scale, self.ignore_index = alpha, embed_scale, ignore_index
+
+    @torch.no_grad()
+    def ask(self, teacher: DecoderLM, tokens: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The teacher's top logits for tokens [..., S]: (ids int32, logits) [..., S, top_k], to keep or to pass on."""
+        top = teacher.forward(tokens).float().topk(self.top_k, dim=-1)
+        return top.indices.int(), top.values
+
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor,
+             training: bool = False) -> torch.Tensor:
+        m, on_gpu = self.student, tokens.is_cuda
+        embed = vocab.embedding if on_gpu else vocab.reference_embedding
+        x = m.hidden(tokens, training, embedded=embed(tokens, m.wemb, self.embed_scale))
+        ids = torch.where((targets != self.ignore_index)[..., None], ids, torch.full_like(ids, -1))
+        if on_gpu:
+            x, w = x.bfloat16(), m.wout.t().bfloat16().contiguous()
+            ce, kd = vocab.cross_entropy, vocab.distill
+        else:
+            w, ce, kd = m.wout.t(), vocab.reference_cross_entropy, vocab.reference_distill
+        total = x.new_zeros((), dtype=torch.float32)
+        if self.alpha < 1.0:
+            total = total + (1.0 - self.alpha) * ce(x, w, targets, self.ignore_index)
+        if self.alpha > 0.0:
+            total = total + self.alpha * kd(x, w, ids, logits, self.temperature)
+        return total
+
+    def step(self, tokens: torch.Tensor, targets: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor,
+             optimizer: Adam, lr: float, clip_norm: float = 1.0) -> float:
+        """One update on a batch [B, S]; returns its loss."""
+        params = list(self.student.parameters())
+        for p in params:
+            p.grad = None
+        loss = self.loss(tokens, targets, ids, logits, training=True)
+        loss.backward()
+        clip_global_norm(params, clip_norm)
+        optimizer.step(params, lr)
+        return float(loss.detach())

@@ -336,17 +336,20 @@ class DecoderLM(nn.Module):
 
     # ------------------------------------------------------------ forward
     def hidden(self, tokens: torch.Tensor, training: bool = False, probe=None,
-               aux_losses: Optional[list] = None, base_pos: int = 0) -> torch.Tensor:
-        """Embedding -> (looped) block stack -> final norm.  tokens: [B, S] or [S]."""
+               aux_losses: Optional[list] = None, base_pos: int = 0,
+               embedded: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Embedding -> (looped) block stack -> final norm.  tokens: [B, S] or [S].  ``embedded`` [.., S, D] replaces
+        the lookup of the tokens' rows."""
         c = self.cfg
         squeeze = tokens.dim() == 1
         if squeeze:
             tokens = tokens[None]
+            embedded = None if embedded is None else embedded[None]
         B, S = tokens.shape
         if S > c.max_seq:
             raise ValueError(f"Sequence length {S} exceeds MaxSeq {c.max_seq}.")
         self.forward_tokens += B * S
-        x = self.wemb[tokens]
+        x = self.wemb[tokens] if embedded is None else embedded
         dev = x.device
         rope = None
         if c.use_rope:

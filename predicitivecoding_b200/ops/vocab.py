@@ -19,7 +19,9 @@ Rows that are not counted - a target outside [0, V) or equal to ``ignore_index``
 have loss 0 and gradient 0, are not read and cost no products; the mean is over the counted rows, and 0 when there
 are none.  A teacher's entry is absent when its id is outside [0, V) or its logit is -inf.
 
-All results are the same from run to run: no sum depends on the order in which atomics arrive.
+The ids of a row's list are meant to differ; entries that repeat an id count as they stand in the loss, and together
+in the gradient.  All results are the same from run to run: no sum depends on the order in which atomics arrive.
+x and w are read again by ``head_bwd`` and must not change in between.
 Kernels: csrc/vocab.cu, csrc/vocab_epilogue.cuh, csrc/gemm2_tcgen05.cu.
 """
 from __future__ import annotations
@@ -90,8 +92,8 @@ def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optio
              piece: int = 0) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx [..., D], dw [V, D]) of a mean or summed loss times ``gout`` (a number, or an fp32 CUDA tensor with one
     value).  They are bf16, or go into ``dx`` / ``dw`` (bf16 or fp32; ``accumulate`` adds to ``dw``).  ``piece``: columns of
-    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of workspace take).  w must still
-    hold what the loss read."""
+    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of workspace take).  x and w must
+    still hold what the loss read."""
     if isinstance(gout, torch.Tensor):
         return ext().vocab_head_bwd(state, 1.0, gout, dx, dw, need_dx, need_dw, accumulate, piece)
     return ext().vocab_head_bwd(state, gout, None, dx, dw, need_dx, need_dw, accumulate, piece)
@@ -101,7 +103,7 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, kind, args, reduction):
         loss, ctx.state = (ce_fwd if kind == "ce" else distill_fwd)(x, w, *args, reduction)
-        ctx.save_for_backward(w)      # so that a change of w before the backward is noticed
+        ctx.save_for_backward(x, w)   # so that a change of either before the backward is noticed
         return loss
 
     @staticmethod
@@ -126,3 +128,39 @@ def distill(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, logits: torch.T
     if reduction == "none":
         return distill_fwd(x, w, ids, logits, temperature, reduction)[0]
     return _HeadLoss.apply(x, w, "distill", (ids, logits, temperature), reduction)
+
+
+# --------------------------------------------------------------------------- plain statements
+def reference_embedding(tok: torch.Tensor, w: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """:func:`embedding` in plain differentiable torch, on any device."""
+    live = (tok >= 0) & (tok < w.shape[0])
+    return torch.where(live[..., None], w[tok.long().clamp(0, w.shape[0] - 1)] * scale, torch.zeros((), device=w.device))
+
+
+def _mean_of_rows(rows: torch.Tensor, live: torch.Tensor, reduction: str) -> torch.Tensor:
+    rows = torch.where(live, rows, torch.zeros((), device=rows.device, dtype=rows.dtype))
+    if reduction == "none":
+        return rows
+    return rows.sum() / live.sum().clamp(min=1) if reduction == "mean" else rows.sum()
+
+
+def reference_cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -1,
+                            reduction: str = "mean") -> torch.Tensor:
+    """:func:`cross_entropy` in plain differentiable torch with the logits in memory, on any device."""
+    live = (targets >= 0) & (targets < w.shape[0]) & (targets != ignore_index)
+    logp = torch.log_softmax(x @ w.t(), -1)
+    at = torch.where(live, targets, torch.zeros_like(targets)).long()
+    return _mean_of_rows(-logp.gather(-1, at[..., None])[..., 0], live, reduction)
+
+
+def reference_distill(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor,
+                      temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """:func:`distill` in plain differentiable torch with the student's logits in memory, on any device."""
+    there = (ids >= 0) & (ids < w.shape[0]) & (logits != float("-inf"))
+    live = there.any(-1)
+    t = (logits.to(x.dtype) / temperature).masked_fill(~there, float("-inf"))
+    logq = torch.log_softmax(torch.where(live[..., None], t, torch.zeros_like(t)), -1)
+    q = torch.exp(logq) * there
+    logp = torch.log_softmax(x @ w.t() / temperature, -1).gather(-1, torch.where(there, ids, torch.zeros_like(ids)).long())
+    terms = torch.where(q > 0, q * (torch.where(q > 0, logq, torch.zeros_like(q)) - logp), torch.zeros_like(q))
+    return _mean_of_rows(temperature ** 2 * terms.sum(-1), live, reduction)

@@ -255,6 +255,55 @@ def test_pieces_and_outputs(piece):
     assert none is None and torch.equal(only_dw, vocab.head_bwd(state, piece=piece)[1])
 
 
+@pytest.mark.parametrize("rows,ignored", [(9000, 0.5), (8193, 0.99), (600, 0.0), (257, 0.0), (256, 0.0)])
+@pytest.mark.parametrize("V,piece", [(40, 0), (700, 256)])
+def test_long_batches_and_the_edge_of_two_terms(rows, ignored, V, piece):
+    """More rows than a block counts for itself; 256 counted rows (two-term gradients) and one more; pieces whose last
+    one is short."""
+    x, w, tgt, g = head(rows, V, 72, rows + V)
+    tgt = torch.where(torch.rand(rows, device=DEV, generator=g) < ignored, torch.full_like(tgt, -1), tgt)
+    q, live = targets64(V, tgt=tgt)
+    check_head(x, w, q, live, 1.0, lambda r: vocab.ce_fwd(x, w, tgt, reduction=r), "mean", piece=piece)
+    _, state = vocab.ce_fwd(x, w, tgt)
+    vocab.head_bwd(state, piece=piece)
+    assert state.status() == 0
+
+
+def test_few_rows_round_the_gradient_once():
+    """Up to 256 counted rows p - q has two terms: the bf16 result is off by its own rounding and 2^-14 more."""
+    x, w, tgt, g = head(5, 3000, 256, 21)
+    _, state = vocab.ce_fwd(x, w, tgt)
+    dx, dw = vocab.head_bwd(state)
+    q, live = targets64(3000, tgt=tgt)
+    G = (torch.softmax(x.double() @ w.double().T, 1) - q) / 5
+    for got, ref, size in ((dx, G @ w.double(), G.abs() @ w.double().abs()), (dw, G.T @ x.double(), G.T.abs() @ x.double().abs())):
+        assert bool(((got.double() - ref).abs() <= U * ref.abs() + 2.0 ** -14 * size).all())
+
+
+def test_top_logit_distiller_on_the_device():
+    """The distiller's loss and gradients on the device against the CPU's.  The device rounds the head's operands to
+    bf16 (2^-8 each, logits of size |x| |w|) and takes its matrix products in fp32."""
+    from predicitivecoding_b200.llm.distill import TopLogitDistiller
+    from predicitivecoding_b200.models.config import DecoderLmConfig
+    from predicitivecoding_b200.models.decoder_lm import DecoderLM
+    cfg = DecoderLmConfig(vocab=260, dim=64, num_blocks=2, num_heads=4, ff_dim=96, max_seq=32, use_rms_norm=True,
+                          use_rope=True, ffn="swiglu")
+    teacher, student = DecoderLM(cfg, seed=1), DecoderLM(cfg, seed=2)
+    tokens = torch.randint(0, 260, (3, 33), generator=torch.Generator().manual_seed(1))
+    x, y = tokens[:, :-1], tokens[:, 1:].clone()
+    y[0, :9] = -1
+    d = TopLogitDistiller(student, top_k=7, temperature=2.0, alpha=0.4, embed_scale=8.0)
+    ids, logits = d.ask(teacher, x)
+    want = d.loss(x, y, ids, logits)
+    grads = torch.autograd.grad(want, (student.wemb, student.wout))
+    size = float(student.hidden(x).norm(dim=-1).max() * student.wout.norm(dim=0).max())
+    student.to(DEV)
+    got = d.loss(x.to(DEV), y.to(DEV), ids.to(DEV), logits.to(DEV))
+    assert abs(float(got) - float(want)) <= 2 * 2 * U * size + 1e-4
+    for a, b in zip(torch.autograd.grad(got, (student.wemb, student.wout)), grads):
+        assert float((a.cpu() - b).norm() / b.norm()) <= 8 * U
+
+
 def test_strides_and_leading_shapes():
     x, w, tgt, g = head(96, 700, 48, 6)
     wide = torch.randn(700, 101, device=DEV, generator=g).bfloat16()
