@@ -340,10 +340,11 @@ __global__ void __launch_bounds__(32 * kLossParts)
   __shared__ int last;
   pdl_begin();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int rows = min(count[0], N);
   const int j = blockIdx.x * 32 + w;   // this warp's packed row
+  const int place = j < N ? row[j] : 0;   // asked for together with the count: a row behind it holds anything
+  const int rows = min(count[0], N);
   const bool live = j < rows;
-  const int n = live ? row[j] : 0;
+  const int n = live ? place : 0;
   // the first two targets of a lane: weight, and log2 q - c z
   constexpr int kAhead = 2;
   const int e = !live ? 0 : len != nullptr ? len[n] : 1;
@@ -402,6 +403,7 @@ __global__ void __launch_bounds__(32 * kLossParts)
   if (!last) return;
   __threadfence();
   double t = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < N; i += 32 * kLossParts) t += __ldcg(loss + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
