@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(32 * sort_rows(R))
 }
 
 // ---------------------------------------------------------------- row losses
-// 32 rows a block, a warp a row: the row's (max, sum) pairs become its log-sum-exp, its target list its loss.  The pairs
+// 32 rows a block, a warp a row: the row's (max, sum) pairs become one, its target list its loss.  The pairs
 // lie by row, so they are read with a row per lane and change hands through shared memory; the targets, which wait
 // for nothing, are read in the meantime.  The last block to finish adds the losses up, in a fixed order and in 64
 // bits: scalars[0] = their sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).
@@ -333,7 +333,7 @@ constexpr int kLossParts = 32;
 __global__ void __launch_bounds__(32 * kLossParts)
     row_loss_kernel(const float2* __restrict__ part, int granules, const int* __restrict__ row,
                     const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
-                    const int* __restrict__ len, int N, int K, float c, float factor, float* __restrict__ lse_out,
+                    const int* __restrict__ len, int N, int K, float c, float factor, float2* __restrict__ norm,
                     float* loss, int* count, int mean, float* __restrict__ scalars) {
   __shared__ float sm[kLossParts][33], ss[kLossParts][33];
   __shared__ double sums[kLossParts];
@@ -345,19 +345,20 @@ __global__ void __launch_bounds__(32 * kLossParts)
   const int rows = min(count[0], N);
   const bool live = j < rows;
   const int n = live ? place : 0;
-  // the first two targets of a lane: weight, and log2 q - c z
+  // the first two targets of a lane: weight, its logarithm, logit
   constexpr int kAhead = 2;
   const int e = !live ? 0 : len != nullptr ? len[n] : 1;
   const long long at_q = (long long)n * K, at_z = (long long)j * K;
-  float qk[kAhead], dk[kAhead];
-  auto target = [&](int k, float& weight, float& d) {
+  float qk[kAhead], lk[kAhead], zk[kAhead];
+  auto target = [&](int k, float& weight, float& lw, float& logit) {
     weight = q != nullptr ? q[at_q + k] : 1.f;
-    d = fmaf(-c, z[at_z + k], lq != nullptr ? lq[at_q + k] : 0.f);
+    lw = lq != nullptr ? lq[at_q + k] : 0.f;
+    logit = z[at_z + k];
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    qk[i] = dk[i] = 0.f;
-    if (lane + 32 * i < e) target(lane + 32 * i, qk[i], dk[i]);
+    qk[i] = lk[i] = zk[i] = 0.f;
+    if (lane + 32 * i < e) target(lane + 32 * i, qk[i], lk[i], zk[i]);
   }
   {
     const int jl = blockIdx.x * 32 + lane;
@@ -379,21 +380,24 @@ __global__ void __launch_bounds__(32 * kLossParts)
   const float m = sm[lane][w];   // lane = part
   const float mm = warp_max(m);
   const float ref = mm == -INFINITY ? 0.f : mm;
-  const float lse = ref + log2f(warp_sum(ss[lane][w] * exp2f(m - ref)));
-  // sum_k q_k (log2 q_k - c z_k + lse), term by term: each is a difference of logarithms of the same size
+  const float tot = warp_sum(ss[lane][w] * exp2f(m - ref));
+  const float lt = log2f(tot);
+  // sum_k q_k (log2 q_k - log2 p_k), log2 p_k = (c z_k - ref) - log2(tot).  The difference of the two large numbers is
+  // taken first and in one rounding: what ref itself was rounded by is in tot, so a row that is sure of its target
+  // keeps the digits of its small loss.
   float l = 0.f;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
-    if (lane + 32 * i < e && qk[i] != 0.f) l += qk[i] * (dk[i] + lse);   // 0 log 0 = 0
+    if (lane + 32 * i < e && qk[i] != 0.f) l += qk[i] * (lk[i] + (fmaf(-c, zk[i], ref) + lt));   // 0 log 0 = 0
   for (int k = lane + 32 * kAhead; k < e; k += 32) {
-    float weight, d;
-    target(k, weight, d);
-    if (weight != 0.f) l += weight * (d + lse);
+    float weight, lw, logit;
+    target(k, weight, lw, logit);
+    if (weight != 0.f) l += weight * (lw + (fmaf(-c, logit, ref) + lt));
   }
   l = warp_sum(l);
   if (live && lane == 0) {
     loss[n] = l * factor;
-    lse_out[j] = lse;
+    norm[j] = make_float2(ref, 1.f / tot);
   }
   if (scalars == nullptr) return;
   __threadfence();
@@ -943,7 +947,7 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
   l.count = take(32);
   l.row = take(4LL * N);
   l.pos = take(4LL * N);
-  l.lse = take(4LL * N);
+  l.norm = take(8LL * N);
   l.z = take(4LL * N * K);
   l.ids = take(4LL * N * K);
   if (distill) {
@@ -1001,7 +1005,8 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   if (a.N < 1 || a.V < 1 || a.D < 1 || a.K < 1 || a.K > kMaxK) return -1;
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, distill);
   int *row = (int*)at(saved, l.row), *ids = (int*)at(saved, l.ids), *count = (int*)at(saved, l.count);
-  float *lse = (float*)at(saved, l.lse), *z = (float*)at(saved, l.z);
+  float2* norm = (float2*)at(saved, l.norm);
+  float* z = (float*)at(saved, l.z);
   float *q = distill ? (float*)at(saved, l.q) : nullptr, *lq = distill ? (float*)at(saved, l.lq) : nullptr;
   int* len = distill ? (int*)at(saved, l.len) : nullptr;
   unsigned short* start = distill ? (unsigned short*)at(saved, l.start) : nullptr;
@@ -1067,7 +1072,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   if (rc) return rc;
   return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, l.granules,
                     (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
-                    0.6931471805599453f * T * T, lse, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+                    0.6931471805599453f * T * T, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
 }
 
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
@@ -1088,7 +1093,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.q = (const float*)at(sv, l.q);
     g.start = (const unsigned short*)at(sv, l.start);
   }
-  g.lse = (const float*)at(sv, l.lse);
+  g.norm = (const float2*)at(sv, l.norm);
   g.g_low = (a.N + 255) / 256 * 256;
   g.g_rows = (int)vocab_g_rows(a.N);
   g.plan = (int*)at(a.saved, l.count) + 2;

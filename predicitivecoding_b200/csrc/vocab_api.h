@@ -37,7 +37,7 @@ struct VocabLayout {
   long long count;   // int [5]: counted rows, finished blocks of the loss kernel, K splits of dw and dx, status of a wait
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
-  long long lse;     // float [N]: base-2 log-sum-exp of logit * log2(e) / temperature, by packed row
+  long long norm;    // float2 [N], by packed row: r and 1 / s, the sum of 2^(logit log2(e) / temperature - r)
   long long z;       // float [N, K]: logits at the target ids, by packed row
   long long ids;     // int [N, K] ascending ids (cross entropy: the targets by packed row)
   long long q;       // float [N, K] weights (distillation)

@@ -211,7 +211,7 @@ struct RowTargets {
   static constexpr int kAhead = 4;
   static constexpr int kNone = 0x7fffffff;
   bool live;        // a counted row
-  float lse;
+  float2 norm;      // GRAD: p = 2^(c l - x) y
   int n, m;         // the row's place in the batch and among the packed rows
   int lo;           // vocabulary id of the first of the 128 columns
   int entry, end;   // next entry of the row's list, and the first behind these columns
@@ -224,7 +224,7 @@ struct RowTargets {
     lo = h.v0 + col0;
     live = packed < rows;
     const int at = max(min(packed, rows - 1), 0);
-    lse = MODE == HEAD_GRAD ? h.lse[at] : 0.f;
+    norm = MODE == HEAD_GRAD ? h.norm[at] : make_float2(0.f, 0.f);
     n = h.start != nullptr ? h.row[at] : h.ids[at];   // class targets stand by packed row
   }
   PCB_DEVICE void ask_entries(const HeadGemm& h) {
@@ -284,6 +284,13 @@ PCB_DEVICE void add2(float& d0, float& d1, float a0, float a1) {
       "add.rn.f32x2 rd, rd, ra;\n\tmov.b64 {%0, %1}, rd;\n\t}"
       : "+f"(d0), "+f"(d1)
       : "f"(a0), "f"(a1));
+}
+
+PCB_DEVICE void mul2(float& d0, float& d1, float a0, float a1, float b) {
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b));
 }
 
 // tcgen05.wait::ld that names the registers it completes, so that no use of them moves above it while the next
@@ -369,9 +376,9 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      scale2(v[j], v[j + 1], __uint_as_float(buf[i & 1][j]), __uint_as_float(buf[i & 1][j + 1]), a.c, -r.lse);
-      v[j] = ex2_approx(v[j]);
-      v[j + 1] = ex2_approx(v[j + 1]);
+      float e0, e1;
+      scale2(e0, e1, __uint_as_float(buf[i & 1][j]), __uint_as_float(buf[i & 1][j + 1]), a.c, -r.norm.x);
+      mul2(v[j], v[j + 1], ex2_approx(e0), ex2_approx(e1), r.norm.y);
     }
     if (!all) {   // what stands in a row that is not counted may be anything
 #pragma unroll

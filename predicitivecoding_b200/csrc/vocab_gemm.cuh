@@ -51,7 +51,7 @@ struct HeadGemm {
   float2* part;           // [2 ceil(V / 256), N] (max, sum), by packed row
   float* z;               // [N, K] logits at the ids, by packed row
   // GRAD, BWD
-  const float* lse;       // [N] base-2 log-sum-exp, by packed row
+  const float2* norm;     // [N] (r, 1 / sum of 2^(c l - r)), by packed row
   // g: panels of 64 columns, each [g_rows, 64], so that every box that is stored or loaded (32 or 64 rows of a panel) is
   // one run of memory, whichever of its two dimensions the product contracts
   int g_rows;
