@@ -323,6 +323,164 @@ __global__ void __launch_bounds__(32 * sort_rows(R))
   }
 }
 
+// ---------------------------------------------------------------- logits of a few rows
+// What the STAT and GRAD products do, for up to kFewRows rows on the FMA units: such a call reads the weights once and has
+// nothing else to do, so it is bound by that; sums in fp32 rounded to nearest keep digits that the tensor cores'
+// accumulation, cut off at each of its D / 16 steps, loses (one row, D 1600: a loss 7e-6 off), and which the loss of
+// few rows does not average out.  Both modes make the same logits, bit for bit: a row that is sure of its target has
+// the sum of its other probabilities in p - q.  A block takes 128 rows of w, a warp four of them at a time, its lanes
+// 8 columns each in turn; x stands in shared memory.  Scoring 1, 2, 4 and 8 rows of 2048 against 32000: 36, 35, 41 and
+// 57 us, on the tensor cores 43, 39, 41 and 39, where the losses are 0.2 to 0.7e-6 off instead of 0.05e-6.
+constexpr int kFewRows = 4;
+constexpr int few_threads(int rows) { return rows <= 2 ? 1024 : 512; }   // as many as registers allow: a small w has few blocks
+constexpr int kFewColumns = 24 * 1024;   // of x in shared memory
+
+struct FewRowsArgs {
+  const __nv_bfloat16* x;      // the batch, read in place when all rows are counted (nullptr: never)
+  long long ldx;
+  const __nv_bfloat16* xc;     // packed rows
+  long long ldxc;
+  const __nv_bfloat16* w;      // [cols, D]
+  long long ldw;
+  __nv_bfloat16* g;            // GRAD
+  HeadGemm h;
+};
+
+// (c0, c1) += (a0, a1) * (b0, b1)
+PCB_DEVICE void fma2(float (&c)[2], float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%0, %1};\n\t"
+      "fma.rn.f32x2 rc, ra, rb, rc;\n\tmov.b64 {%0, %1}, rc;\n\t}"
+      : "+f"(c[0]), "+f"(c[1])
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+template <int NR, bool GRAD>
+__global__ void __launch_bounds__(few_threads(NR)) few_rows_kernel(FewRowsArgs a) {
+  constexpr int kThreads = few_threads(NR), kPerWarp = 128 / (kThreads / 32);
+  extern __shared__ __align__(16) __nv_bfloat16 xs[];   // [NR][ld]
+  __shared__ float logits[NR][128];
+  pdl_begin();
+  const HeadGemm& h = a.h;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int nvec = (h.D + 7) / 8, ld = nvec * 8, whole = h.D / 8;
+  const int rows = min(h.count[0], h.N);
+  const bool direct = a.x != nullptr && rows == h.N;
+  const __nv_bfloat16* src = direct ? a.x : a.xc;
+  const long long lds = direct ? a.ldx : a.ldxc;
+  for (int i = threadIdx.x; i < NR * nvec; i += kThreads) {   // rows of either are 16-byte aligned, packed ones padded
+    const int n = i / nvec, v = i - n * nvec;
+    reinterpret_cast<uint4*>(xs)[i] = n < rows ? *reinterpret_cast<const uint4*>(src + n * lds + v * 8) : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  const int col0 = blockIdx.x * 128;
+#pragma unroll 1
+  for (int r0 = 0; r0 < kPerWarp; r0 += 4) {
+    const int v0 = col0 + w * kPerWarp + r0;
+    if (v0 < h.cols) {   // warp-uniform
+      const __nv_bfloat16* p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[r] = a.w + (long long)min(v0 + r, h.cols - 1) * a.ldw;
+      float acc[4][NR][2] = {};   // even and odd columns: products and sums are taken in pairs
+#pragma unroll 2
+      for (int v = lane; v < whole; v += 32) {
+        float f[4][8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_vec<__nv_bfloat16, 8>(p[r] + v * 8, f[r]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          float xv[8];
+          load_vec<__nv_bfloat16, 8>(xs + n * ld + v * 8, xv);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) fma2(acc[r][n], f[r][e], f[r][e + 1], xv[e], xv[e + 1]);
+        }
+      }
+      if (whole * 8 + lane < h.D) {   // the columns that fill no vector
+        const int d = whole * 8 + lane;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+            acc[r][n][0] = fmaf(__bfloat162float(p[r][d]), __bfloat162float(xs[n * ld + d]), acc[r][n][0]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const float s = warp_sum(acc[r][n][0] + acc[r][n][1]);
+          if (lane == 0) logits[n][w * kPerWarp + r0 + r] = s;
+        }
+    }
+  }
+  __syncthreads();
+  const int lo = h.v0 + col0;   // vocabulary id of the first column
+  const bool mine = w < NR && w < rows;   // a warp per row
+  int e0 = 0, e1 = 0;           // this row's entries in these columns
+  const int* ids = nullptr;
+  const float* q = nullptr;
+  if (mine) {
+    if (h.start != nullptr) {
+      const int n = h.row[w];
+      const unsigned short* s = h.start + (long long)(lo >> 7) * h.N + n;
+      e0 = s[0];
+      e1 = s[h.N];
+      ids = h.ids + (long long)n * h.K;
+      if (GRAD) q = h.q + (long long)n * h.K;
+    } else {
+      ids = h.ids + w;
+      e1 = ids[0] >= lo && ids[0] < lo + 128 ? 1 : 0;
+    }
+  }
+  if constexpr (!GRAD) {
+    if (!mine) return;
+    float v[4], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = col0 + lane + 32 * i < h.cols ? logits[w][lane + 32 * i] : -INFINITY;
+      mx = fmaxf(mx, v[i]);
+    }
+    mx = warp_max(mx) * h.c;
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += exp2f(fmaf(v[i], h.c, -ref));
+    sum = warp_sum(sum);
+    if (lane == 0) h.part[(long long)(lo >> 7) * h.N + w] = make_float2(mx, sum);
+    for (int e = e0 + lane; e < e1; e += 32) h.z[(long long)w * h.K + e] = logits[w][ids[e] - lo];
+  } else {
+    if (mine) {
+      const float2 norm = h.norm[w];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = lane + 32 * i;
+        logits[w][c] = col0 + c < h.cols ? exp2f(fmaf(logits[w][c], h.c, -norm.x)) * norm.y : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0)
+        for (int e = e0; e < e1; ++e) logits[w][ids[e] - lo] -= q != nullptr ? q[e] : 1.f;   // in order: ids may repeat
+    }
+    __syncthreads();
+    // the two panels' rows up to the first k-block of dw's product, in both terms: 8 columns a thread and turn
+    for (int i = threadIdx.x; i < 2 * 64 * 8; i += kThreads) {
+      const int c = (i & 7) * 8, n = (i >> 3) & 63, panel = i >> 9;
+      if (col0 + panel * 64 >= h.cols) break;
+      uint32_t hi[4] = {}, low[4] = {};
+      if (n < rows) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x0 = logits[n % NR][panel * 64 + c + 2 * j], x1 = logits[n % NR][panel * 64 + c + 2 * j + 1];
+          hi[j] = pack_bf16x2(x0, x1);
+          low[j] = pack_bf16x2(x0 - bf16_lo(hi[j]), x1 - bf16_hi(hi[j]));
+        }
+      }
+      __nv_bfloat16* g = a.g + ((long long)(col0 / 64 + panel) * h.g_rows + n) * 64 + c;
+      *reinterpret_cast<uint4*>(g) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(g + (long long)h.g_low * 64) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && h.v0 == 0) plan_splits(h, rows, h.bwd_pairs, h.plan);
+  }
+}
+
 // ---------------------------------------------------------------- row losses
 // 32 rows a block, a warp a row: the row's (max, sum) pairs become one, its target list its loss.  The pairs
 // lie by row, so they are read with a row per lane and change hands through shared memory; the targets, which wait
@@ -1000,6 +1158,32 @@ static bool readable(const void* x, long long ldx, int D) {
   return D % 8 == 0 && ldx % 8 == 0 && ldx >= D && al(x, 16);
 }
 
+static bool few_rows(int N, int D) { return N <= kFewRows && D <= kFewColumns; }
+
+template <bool GRAD>
+static int launch_few_rows(const HeadGemm& h, const void* xc, long long ldxc, const void* x, long long ldx, const void* w,
+                           long long ldw, void* g, cudaStream_t s) {
+  FewRowsArgs f{};
+  f.x = (const __nv_bfloat16*)x;
+  f.ldx = ldx;
+  f.xc = (const __nv_bfloat16*)xc;
+  f.ldxc = ldxc;
+  f.w = (const __nv_bfloat16*)w;
+  f.ldw = ldw;
+  f.g = (__nv_bfloat16*)g;
+  f.h = h;
+  auto go = [&](auto nr) {
+    constexpr int NR = decltype(nr)::value;
+    static SmemLimit limit;
+    if (!limit.raise(few_rows_kernel<NR, GRAD>, NR * kFewColumns * 2)) return cudaErrorInvalidValue;
+    return pdl_launch(few_rows_kernel<NR, GRAD>, dim3((h.cols + 127) / 128), dim3(few_threads(NR)), (size_t)(NR * ldxc * 2), s, f);
+  };
+  const cudaError_t e = h.N == 1   ? go(std::integral_constant<int, 1>{})
+                        : h.N == 2 ? go(std::integral_constant<int, 2>{})
+                                   : go(std::integral_constant<int, 4>{});
+  return e == cudaSuccess ? 0 : -3;
+}
+
 int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s) {
   const bool distill = a.tgt == nullptr;
   if (a.N < 1 || a.V < 1 || a.D < 1 || a.K < 1 || a.K > kMaxK) return -1;
@@ -1055,6 +1239,11 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
     R = (a.N + blocks - 1) / blocks;
   }
   if (pdl_launch(pack_rows_kernel, dim3(blocks), dim3(kThreads), 0, s, p, R) != cudaSuccess) return -3;
+  auto finish = [&](const VocabLayout& l, int pairs) {   // row losses from `pairs` (max, sum) pairs a row
+    return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, pairs,
+                      (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
+                      0.6931471805599453f * T * T, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+  };
   HeadGemm g{};
   g.N = a.N;
   g.D = a.D;
@@ -1068,11 +1257,13 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   g.start = start;
   g.part = (float2*)part;
   g.z = z;
+  if (few_rows(a.N, a.D)) {
+    const int rc = launch_few_rows<false>(g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, s);
+    return rc ? rc : finish(l, (a.V + 127) / 128);
+  }
   const int rc = pcb_head_gemm(HEAD_STAT, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, num_sms, s);
   if (rc) return rc;
-  return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, l.granules,
-                    (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
-                    0.6931471805599453f * T * T, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+  return finish(l, l.granules);
 }
 
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
@@ -1108,6 +1299,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   g.scale = a.mean ? a.scalars + 1 : nullptr;
   g.scale2 = a.gout_dev;
   g.slab = a.slab;
+  g.bwd_pairs = num_sms / 2;
   g.ld_slab = a.ld_slab;
   for (int v0 = 0; v0 < a.V; v0 += a.plan.piece) {
     g.v0 = v0;
@@ -1116,7 +1308,9 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.dw = a.dw == nullptr ? nullptr : (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
     const __nv_bfloat16* w = (const __nv_bfloat16*)a.w + (long long)v0 * a.ldw;
     for (int mode : {HEAD_GRAD, HEAD_BWD}) {
-      const int rc = pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, num_sms, s);
+      const int rc = mode == HEAD_GRAD && few_rows(a.N, a.D)
+                         ? launch_few_rows<true>(g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, s)
+                         : pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, num_sms, s);
       if (rc) return rc;
     }
   }

@@ -83,6 +83,37 @@ struct HeadGemm {
 constexpr int kMaxDxSplits = 16;
 __host__ __device__ inline int head_bn(int D) { return D <= 128 ? 128 : 256; }
 
+// k-blocks that a tile costs besides its own
+constexpr int kTileOverhead = 4;
+
+// K splits of dw and dx.  With the schedule below all pairs of SMs are busy for the mean of the work and half a tile of
+// dw, unless either product has too few tiles; slabs cost their bytes, written and read once, of which the time of
+// one k-block of a 256-column tile moves 2.4 MB.  As if both were wanted, so that a gradient is the same with and
+// without the other.
+__device__ inline void plan_splits(const HeadGemm& a, int rows, int pairs, int* plan) {
+  const int bn = head_bn(a.D), num_n = (a.D + bn - 1) / bn;
+  const int r = max(rows, 1), two = rows <= kTwoTermRows ? 2 : 1;
+  const float kb_dw = two * ((r + 63) / 64), kb_dx = two * ((a.cols + 63) / 64);
+  const int dw = (a.cols + 255) / 256 * num_n, dx = (r + 255) / 256 * num_n;
+  const float slab = 8.f * a.D / 2.4e6f * (256 / bn);   // per row
+  const int dx_max = min(kMaxDxSplits, a.slab_rows / ((r + 255) / 256 * 256));
+  float best = INFINITY;
+  for (int s1 = 1; s1 <= a.dw_max && (s1 == 1 || kb_dw >= 4 * s1); s1 *= 2) {
+    const float c1 = kb_dw / s1 + kTileOverhead;
+    const float alone = (dw * s1 + pairs - 1) / pairs * c1;
+    for (int s2 = 1; s2 <= dx_max && (s2 == 1 || kb_dx >= 4 * s2); ++s2) {
+      const float c2 = kb_dx / s2 + kTileOverhead;
+      const float even = (dw * s1 * c1 + dx * s2 * c2) / pairs + 0.5f * c1;
+      const float c = fmaxf(fmaxf(even, alone), (dx * s2 + pairs - 1) / pairs * c2) + slab * ((s1 > 1 ? s1 * a.cols : 0) + s2 * r);
+      if (c < best) {
+        best = c;
+        plan[0] = s1;
+        plan[1] = s2;
+      }
+    }
+  }
+}
+
 }  // namespace pcb
 
 // x: packed rows [N, ldx]; x_all: the batch itself (nullptr: cannot be read in place); w: [cols, D] rows v0..; g: panels of 64
