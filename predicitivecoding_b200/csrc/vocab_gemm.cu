@@ -275,11 +275,20 @@ PCB_DEVICE void wait32(uint32_t (&r)[32]) {
       : "memory");
 }
 
+// the other accumulator's part of 32 logits
+PCB_DEVICE void add_half(uint32_t taddr, uint32_t (&v)[32]) {
+  uint32_t o[32];
+  tmem_ld_32x32b_x32(taddr + 256, o);
+  wait32(o);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[j]));
+}
+
 // (max, sum 2^(c l - max)) of this thread's 128 logits, in one pass with a running maximum, and the logits at the
 // row's targets.  The maximum stays in units of c l, and the sum is taken against that rounded value, so the
 // log-sum-exp made of the pair carries no error of the product c * max.  The next 32 columns come from TMEM while
 // these are worked on; `between(i)` runs after 32 columns.
-template <typename F>
+template <bool HALVES, typename F>
 PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int col0, F between) {
   float mx = -INFINITY, sum = 0.f;
   uint32_t buf[2][32];
@@ -287,6 +296,7 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     wait32(buf[i & 1]);
+    if constexpr (HALVES) add_half(taddr + 32 * i, buf[i & 1]);
     if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
 #pragma unroll
@@ -332,7 +342,7 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 // 128 columns of softmax - target distribution as bf16, 64 at a time handed to `store` (high terms, and with TWO the low
 // ones).  The factor 1 / count is applied in fp32 behind the products that read them: rounding a shared factor into
 // every entry would bias all of them alike.
-template <bool TWO, typename F, typename S>
+template <bool TWO, bool HALVES, typename F, typename S>
 PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int col0, F between, S store) {
   const bool all = __all_sync(0xffffffffu, r.live);
   uint32_t buf[2][32];
@@ -341,6 +351,7 @@ PCB_DEVICE void grad128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     wait32(buf[i & 1]);
+    if constexpr (HALVES) add_half(taddr + 32 * i, buf[i & 1]);
     if (i < 3) tmem_ld_32x32b_x32(taddr + 32 * (i + 1), buf[(i + 1) & 1]);
     float v[32];
 #pragma unroll
@@ -440,10 +451,17 @@ PCB_DEVICE void store4(__nv_bfloat16* c, float (&o)[4], int nv, bool add) {
   }
 }
 
+// The tensor cores cut a sum off at every step, which takes D / 16 units of its last digit from a logit.  A batch of one
+// row block is bound by reading w and needs no second accumulator to work ahead: with HALVES the two take half of the
+// sum each, and the losses come out at half of the error (32 rows of 2048 against 32000: 4e-7 in 38 us, 9e-7 in 36
+// with the tiles overlapped; below 1024 columns the error is under half of that and the overlap stays).  Both logits'
+// modes go by the same rule: what a row that is sure of its target has in p - q is the sum of its other entries.
+static bool in_halves(int N, int D) { return N <= kTwoTermRows && D >= 1024; }
+
 // ---------------------------------------------------------------- kernel
 // STAT, GRAD: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x,
 // tmS = fp32 slabs.
-template <int MODE, int BN>
+template <int MODE, int BN, bool HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
     head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
@@ -562,15 +580,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint64_t ad = a0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
           const uint64_t bd = b0 + static_cast<uint32_t>(stage) * (C::STAGE_BYTES / 16);
-          umma_bf16_pair(d_tmem, ad, bd, idesc, kb > tile.kb0 ? 1u : 0u);
+          uint32_t d = d_tmem;
+          bool fresh = kb == tile.kb0;
+          if (HALVES && kb >= sh.kb_dx / 2) {
+            d += BN;
+            fresh = kb == sh.kb_dx / 2;
+          }
+          umma_bf16_pair(d, ad, bd, idesc, fresh ? 0u : 1u);
 #pragma unroll
-          for (int k = 1; k < kBK / 16; ++k) umma_bf16_pair(d_tmem, ad + k * a_step, bd + k * b_step, idesc, 1u);
+          for (int k = 1; k < kBK / 16; ++k) umma_bf16_pair(d, ad + k * a_step, bd + k * b_step, idesc, 1u);
           umma_commit_pair(&empty[stage], 0x3);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         umma_commit_pair(&tfull[acc], 0x3);
-        acc ^= 1;
+        if (!HALVES) acc ^= 1;   // two halves: always the same pair of accumulators
         if (acc == 0) acc_phase ^= 1u;
       }
     }
@@ -617,15 +641,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if (MODE == HEAD_STAT) {
-        stat128(a, r, tbase + half * 128, n0 + half * 128, between);
+        stat128<HALVES>(a, r, tbase + half * 128, n0 + half * 128, between);
       } else if (MODE == HEAD_GRAD) {
         auto store = [&](int b, const uint32_t (&pk)[32], bool low) {
           const int col = n0 + half * 128 + 64 * b;
           if (col < a.cols)   // warp-uniform
             store_box64(&tmC, stg, box_at, pk, 0, col / 64 * a.g_rows + row0 + (low ? a.g_low : 0), lane);
         };
-        if (sh.two) grad128<true>(a, r, tbase + half * 128, n0 + half * 128, between, store);
-        else grad128<false>(a, r, tbase + half * 128, n0 + half * 128, between, store);
+        if (HALVES || sh.two) grad128<true, HALVES>(a, r, tbase + half * 128, n0 + half * 128, between, store);
+        else grad128<false, false>(a, r, tbase + half * 128, n0 + half * 128, between, store);
       } else if (tile.dw && a.dw_tma && sh.dw_splits == 1) {
 #pragma unroll 1
         for (int c2 = half; c2 < BN / 64; c2 += 2) {
@@ -704,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader) mbar_arrive(&tempty[acc]);
         else mbar_arrive_remote(acc ? tempty_leader1 : tempty_leader0);
       }
-      acc ^= 1;
+      if (!HALVES) acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
     if (MODE != HEAD_STAT && lane == 0) bulk_group_wait_all();   // every TMA store has landed
@@ -744,11 +768,11 @@ static bool map2(CUtensorMap* m, const void* ptr, long long inner, long long out
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE, int BN>
+template <int MODE, int BN, bool HALVES = false>
 static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int num_sms, cudaStream_t s) {
   using C = Cfg<MODE, BN>;
   static SmemLimit limit;
-  if (!limit.raise(head_kernel<MODE, BN>, C::SMEM_BYTES)) return -3;
+  if (!limit.raise(head_kernel<MODE, BN, HALVES>, C::SMEM_BYTES)) return -3;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * std::min(tiles, num_sms / 2), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
@@ -763,7 +787,7 @@ static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int n
   attr[1].val.programmaticStreamSerializationAllowed = pdl_env_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, head_kernel<MODE, BN>, t[0], t[1], t[2], t[3], t[4], t[5], a) == cudaSuccess ? 0 : -3;
+  return cudaLaunchKernelEx(&cfg, head_kernel<MODE, BN, HALVES>, t[0], t[1], t[2], t[3], t[4], t[5], a) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace head
@@ -794,6 +818,9 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
     // the blocks that run side by side share the operand with the larger footprint
     a.row_blocks_last = a.N > a.cols;
     const int tiles = num_m * ((a.cols + 255) / 256);
+    if (in_halves(a.N, a.D))
+      return mode == HEAD_STAT ? launch<HEAD_STAT, 256, true>(t, a, tiles, num_sms, s)
+                               : launch<HEAD_GRAD, 256, true>(t, a, tiles, num_sms, s);
     return mode == HEAD_STAT ? launch<HEAD_STAT, 256>(t, a, tiles, num_sms, s) : launch<HEAD_GRAD, 256>(t, a, tiles, num_sms, s);
   }
   if (!map2(&t[0], g, 64, panels * a.g_rows, 64, 64) || !map2(&t[1], w, a.D, a.cols, ldw, 64)) return -5;
