@@ -18,7 +18,7 @@ from . import (ext, gemm, gemm_pc, attn_fwd, attn_bwd, EPI_BF16, EPI_F32, EPI_RE
 
 CASES = ("gemm_swiglu", "gemm_lmhead", "gemm_dw", "pc_pred", "pc_state", "attn_fwd", "attn_fwd_mma", "attn_bwd",
          "attn_fwd_d128", "attn_fwd_mma_d128", "attn_bwd_d128", "moe_fwd", "moe_layer", "skinny_qkv",
-         "decode_attn_b32")
+         "decode_attn_b32", "vocab_ce", "vocab_distill", "embed_grad")
 
 
 def build(which: str, dev: str = "cuda"):
@@ -112,6 +112,24 @@ def build(which: str, dev: str = "cuda"):
         kc, vc = rn(B, H, cap, hd).to(bf), rn(B, H, cap, hd).to(bf)
         lens = torch.full((B,), L, dtype=torch.int32, device=dev)
         return (lambda: decode_attn(q, kc, vc, lens, hd ** -0.5)), 4 * B * H * L * hd
+    if which in ("vocab_ce", "vocab_distill"):   # loss and gradients of the head without its logits, 4 x 1024 tokens
+        from . import vocab
+        N, D, V, K = 4096, 768, 32000, 64
+        x, w = rn(N, D).to(bf), rn(V, D, scale=0.05).to(bf)
+        tgt = torch.randint(0, V, (N,), device=dev, generator=g)
+        ids = torch.randint(0, V, (N, K), device=dev, generator=g)
+        top = rn(N, K, scale=2.0)
+
+        def step():
+            loss, state = (vocab.ce_fwd(x, w, tgt) if which == "vocab_ce" else vocab.distill_fwd(x, w, ids, top, 2.0))
+            return vocab.head_bwd(state)
+        return step, 8 * N * V * D
+    if which == "embed_grad":           # gradient of the embedding, 16 x 1024 tokens that fall off as 1 / rank
+        from . import vocab
+        N, D, V = 16384, 768, 32000
+        tok = (torch.exp(torch.rand(N, device=dev, generator=g) * torch.log(torch.tensor(float(V)))) - 1).long()
+        dx = rn(N, D)
+        return (lambda: vocab.embed_bwd(tok, dx, V, 27.7)), N * D
     raise ValueError(f"unknown case {which!r}; one of {CASES}")
 
 
