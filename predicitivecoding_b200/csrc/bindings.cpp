@@ -383,9 +383,11 @@ at::Tensor flat(const at::Tensor& t) { return t.is_contiguous() ? t : t.contiguo
 // What a loss of the vocabulary head keeps for its gradients.
 struct HeadState {
   at::Tensor saved, scalars, x, w;
+  at::Tensor g;   // gradient of the logits, where the forward made it
+  pcb::VocabPlan plan;
   std::vector<int64_t> lead;
   int64_t N, V, D, K;
-  bool distill, mean, none;
+  bool distill, mean, none, gradient;
   double temperature;
   // 0, or the code of a bounded wait that ran out in a kernel of this loss (reads device memory: synchronises)
   int64_t status() const {
@@ -406,7 +408,8 @@ void used_here(const at::Tensor& t) {
 // aligned.
 std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x, const at::Tensor& w,
                                           const at::Tensor* tgt, int64_t ignore, const at::Tensor* ids,
-                                          const at::Tensor* logits, double temperature, const std::string& reduction) {
+                                          const at::Tensor* logits, double temperature, const std::string& reduction,
+                                          bool gradient) {
   PCB_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16, what, ": x must be a bf16 CUDA tensor");
   PCB_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16, what, ": w must be a bf16 CUDA tensor");
   PCB_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.numel() > 0 &&
@@ -420,6 +423,7 @@ std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x,
   st.lead.assign(x.sizes().begin(), x.sizes().end() - 1);
   st.mean = reduction == "mean";
   st.none = reduction == "none";
+  st.gradient = gradient && !st.none;
   st.distill = tgt == nullptr;
   st.D = x.size(-1);
   st.N = x.numel() / st.D;
@@ -479,21 +483,24 @@ std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x,
     a.loss = part.data_ptr<float>() + pairs;
     loss = st.scalars.select(0, 0);
   }
-  check(pcb_vocab_fwd(a, st.saved.data_ptr(), part.data_ptr(), st.mean ? 1 : 0, num_sms(), cur_stream()), what,
-        st.distill ? 4 : 3);
+  st.plan = pcb::vocab_plan(a.N, a.V, a.D, 0, st.gradient, num_sms());
+  if (st.plan.whole) st.g = at::empty({pcb::vocab_g_rows(a.N) * st.plan.piece}, x.options());
+  check(pcb_vocab_fwd(a, st.plan, st.saved.data_ptr(), part.data_ptr(), st.g.defined() ? st.g.data_ptr() : nullptr,
+                      st.mean ? 1 : 0, num_sms(), cur_stream()),
+        what, (st.distill ? 2 : 1) + (st.plan.whole ? 1 : 2));
   return {loss, st};
 }
 
 std::pair<at::Tensor, HeadState> vocab_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
-                                              int64_t ignore, const std::string& reduction) {
+                                              int64_t ignore, const std::string& reduction, bool gradient) {
   is64(targets, "ce_fwd: targets");
   PCB_CHECK(x.dim() >= 1 && same_lead(targets, x, 0), "ce_fwd: targets must have x's leading shape");
-  return head_fwd("ce_fwd", x, w, &targets, ignore, nullptr, nullptr, 1.0, reduction);
+  return head_fwd("ce_fwd", x, w, &targets, ignore, nullptr, nullptr, 1.0, reduction, gradient);
 }
 
 std::pair<at::Tensor, HeadState> vocab_distill_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& ids,
                                                    const at::Tensor& logits, double temperature,
-                                                   const std::string& reduction) {
+                                                   const std::string& reduction, bool gradient) {
   is64(ids, "distill_fwd: ids");
   is_bf16(logits, "distill_fwd: logits");
   PCB_CHECK(x.dim() >= 1 && same_lead(ids, x, 1) && ids.sizes() == logits.sizes(),
@@ -502,7 +509,7 @@ std::pair<at::Tensor, HeadState> vocab_distill_fwd(const at::Tensor& x, const at
             pcb::kVocabMaxEntries, " entries per row");
   PCB_CHECK(temperature > 0 && temperature < std::numeric_limits<float>::infinity(),
             "distill_fwd: temperature must be positive and finite");
-  return head_fwd("distill_fwd", x, w, nullptr, -1, &ids, &logits, temperature, reduction);
+  return head_fwd("distill_fwd", x, w, nullptr, -1, &ids, &logits, temperature, reduction, gradient);
 }
 
 // Gradients of a mean or summed loss, into dx [..., D] and dw [V, D] where given, else into new bf16 tensors.  Allocates
@@ -511,6 +518,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     const HeadState& st, double gout, const c10::optional<at::Tensor>& gout_dev, c10::optional<at::Tensor> dx,
     c10::optional<at::Tensor> dw, bool need_dx, bool need_dw, bool accumulate, int64_t piece) {
   PCB_CHECK(!st.none, "head_bwd: the gradient is of a mean or summed loss");
+  PCB_CHECK(st.gradient, "head_bwd: the loss was taken without its gradient");
   PCB_CHECK(!accumulate || dw, "head_bwd: accumulate needs dw");
   PCB_CHECK(piece >= 0, "head_bwd: piece must not be negative");
   pcb::VocabGradArgs a{};
@@ -543,7 +551,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     return {dx, dw};
   }
   if (!dx && !dw) return {dx, dw};
-  for (const at::Tensor& t : {st.saved, st.scalars, st.x, st.w}) used_here(t);
+  for (const at::Tensor& t : {st.saved, st.scalars, st.x, st.w, st.g}) used_here(t);
   a.x = st.x.data_ptr();
   a.ldx = rows_apart(st.x);
   a.w = st.w.data_ptr();
@@ -568,14 +576,15 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     a.lddw = rows_apart(*dw);
   }
   a.dw_add = accumulate;
-  a.plan = pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), num_sms());
+  a.plan = st.plan.whole ? st.plan
+                         : pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), false, num_sms());
   a.ld_slab = (a.D + 3) / 4 * 4;
-  const int64_t gbytes = (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
+  const int64_t gbytes = a.plan.whole ? 0 : (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
   const bool slabs = dx || a.plan.dw_max > 1;
   at::Tensor ws = at::empty({gbytes + (slabs ? 4 * a.plan.all_rows * a.ld_slab : 0)}, st.saved.options());
-  a.g = ws.data_ptr();
+  a.g = a.plan.whole ? st.g.data_ptr() : ws.data_ptr();
   if (slabs) a.slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", 2 * a.plan.pieces + (slabs ? 1 : 0));
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", (a.plan.whole ? 1 : 2) * a.plan.pieces + (slabs ? 1 : 0));
   return {dx, dw};
 }
 

@@ -564,22 +564,7 @@ __global__ void __launch_bounds__(32 * kLossParts)
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double t = 0.0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < N; i += 32 * kLossParts) t += __ldcg(loss + i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (lane == 0) sums[w] = t;
-  __syncthreads();
-  if (w == 0) {
-    t = sums[lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) {
-      scalars[0] = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
-      scalars[1] = rows > 0 ? 1.f / (float)rows : 0.f;
-    }
-  }
+  add_losses<32 * kLossParts>(loss, N, rows, mean, scalars, sums, threadIdx.x, [] { __syncthreads(); });
 }
 
 // Gradients from their fp32 slabs: the sum in slab order, times the gradient's factor.  The first N rows are dx's, found
@@ -1120,7 +1105,9 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
 
 long long vocab_g_rows(int N) { return (N + 255LL) / 256 * 256 + kTwoTermRows; }
 
-VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms) {
+static bool few_rows(int N, int D) { return N <= kFewRows && D <= kFewColumns; }
+
+VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num_sms) {
   VocabPlan r{};
   const long long all = (V + 255LL) / 256 * 256;
   long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2LL * N) / 256 * 256;
@@ -1136,6 +1123,8 @@ VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms) {
   r.dw_max = r.pieces == 1 ? (int)std::max(1LL, std::min(8LL, num_sms / 2 / tiles)) : 1;
   r.slab_rows = (int)std::min((N + 255LL) / 256 * 256 + 16 * 256, 1LL << 30);
   r.all_rows = r.slab_rows + (r.dw_max > 1 ? r.dw_max * all : 0);
+  // g then lives as long as the forward's state, so it is bounded as a piece is
+  r.whole = gradient && r.pieces == 1 && !few_rows(N, D) && pcb_head_whole(N, V, D);
   return r;
 }
 
@@ -1157,8 +1146,6 @@ static char* at(void* base, long long off) { return (char*)base + off; }
 static bool readable(const void* x, long long ldx, int D) {
   return D % 8 == 0 && ldx % 8 == 0 && ldx >= D && al(x, 16);
 }
-
-static bool few_rows(int N, int D) { return N <= kFewRows && D <= kFewColumns; }
 
 template <bool GRAD>
 static int launch_few_rows(const HeadGemm& h, const void* xc, long long ldxc, const void* x, long long ldx, const void* w,
@@ -1184,7 +1171,18 @@ static int launch_few_rows(const HeadGemm& h, const void* xc, long long ldxc, co
   return e == cudaSuccess ? 0 : -3;
 }
 
-int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s) {
+// what the backward's launches, and the forward's where it makes g, know of the gradients' products
+static void plan_products(HeadGemm& g, const VocabPlan& plan, int N, int* count, int num_sms) {
+  g.g_low = (N + 255) / 256 * 256;
+  g.g_rows = (int)vocab_g_rows(N);
+  g.plan = count + 2;
+  g.dw_max = plan.dw_max;
+  g.slab_rows = plan.slab_rows;
+  g.bwd_pairs = num_sms / 2;
+}
+
+int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, void* part, void* dlogits, int mean,
+                  int num_sms, cudaStream_t s) {
   const bool distill = a.tgt == nullptr;
   if (a.N < 1 || a.V < 1 || a.D < 1 || a.K < 1 || a.K > kMaxK) return -1;
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, distill);
@@ -1195,7 +1193,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   int* len = distill ? (int*)at(saved, l.len) : nullptr;
   unsigned short* start = distill ? (unsigned short*)at(saved, l.start) : nullptr;
   const float T = distill ? a.temperature : 1.f;
-  const float c = 1.4426950408889634f / T;
+  const float c = 1.4426950408889634f / T, factor = 0.6931471805599453f * T * T;
   if (distill) {
     auto sort = [&](auto r) {
       constexpr int R = decltype(r)::value, rows = sort_rows(R);
@@ -1242,7 +1240,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   auto finish = [&](const VocabLayout& l, int pairs) {   // row losses from `pairs` (max, sum) pairs a row
     return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, pairs,
                       (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
-                      0.6931471805599453f * T * T, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+                      factor, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
   };
   HeadGemm g{};
   g.N = a.N;
@@ -1260,6 +1258,16 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, void* saved, void* part, int mean, int
   if (few_rows(a.N, a.D)) {
     const int rc = launch_few_rows<false>(g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, s);
     return rc ? rc : finish(l, (a.V + 127) / 128);
+  }
+  if (plan.whole) {
+    plan_products(g, plan, a.N, count, num_sms);
+    g.q = q;
+    g.loss = a.loss;
+    g.factor = factor;
+    g.scalars = a.scalars;
+    g.mean = mean;
+    g.done = count + 1;
+    return pcb_head_gemm(HEAD_WHOLE, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, dlogits, num_sms, s);
   }
   const int rc = pcb_head_gemm(HEAD_STAT, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, num_sms, s);
   if (rc) return rc;
@@ -1285,13 +1293,9 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.start = (const unsigned short*)at(sv, l.start);
   }
   g.norm = (const float2*)at(sv, l.norm);
-  g.g_low = (a.N + 255) / 256 * 256;
-  g.g_rows = (int)vocab_g_rows(a.N);
-  g.plan = (int*)at(a.saved, l.count) + 2;
+  plan_products(g, a.plan, a.N, (int*)at(sv, l.count), num_sms);
   g.want_dw = a.dw != nullptr;
   g.want_dx = a.dx != nullptr;
-  g.dw_max = a.plan.dw_max;
-  g.slab_rows = a.plan.slab_rows;
   g.lddw = a.lddw;
   g.dw_f32 = a.dw_f32;
   g.dw_add = a.dw_add;
@@ -1299,7 +1303,6 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   g.scale = a.mean ? a.scalars + 1 : nullptr;
   g.scale2 = a.gout_dev;
   g.slab = a.slab;
-  g.bwd_pairs = num_sms / 2;
   g.ld_slab = a.ld_slab;
   for (int v0 = 0; v0 < a.V; v0 += a.plan.piece) {
     g.v0 = v0;
@@ -1308,6 +1311,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.dw = a.dw == nullptr ? nullptr : (char*)a.dw + (long long)v0 * a.lddw * (a.dw_f32 ? 4 : 2);
     const __nv_bfloat16* w = (const __nv_bfloat16*)a.w + (long long)v0 * a.ldw;
     for (int mode : {HEAD_GRAD, HEAD_BWD}) {
+      if (mode == HEAD_GRAD && a.plan.whole) continue;   // the forward made g
       const int rc = mode == HEAD_GRAD && few_rows(a.N, a.D)
                          ? launch_few_rows<true>(g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, s)
                          : pcb_head_gemm(mode, g, at(sv, l.xc), l.ldxc, x_all, a.ldx, w, a.ldw, a.g, num_sms, s);

@@ -30,6 +30,17 @@ struct VocabHeadArgs {
   float* scalars;       // [2]: sum or mean of the row losses, 1 / counted rows (nullptr: not wanted)
 };
 
+// Workspaces of the backward.  The vocabulary is taken `piece` columns at a time.
+struct VocabPlan {
+  int piece, pieces;
+  int dw_max;            // most K splits of the dw product
+  int slab_rows;         // rows of the fp32 slabs that dx takes
+  long long all_rows;    // with those of dw
+  bool whole;            // a small vocabulary: the forward makes the gradient of the logits, g, along with the loss
+};
+// `gradient`: for a forward that a backward follows
+VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num_sms);
+
 // Where the forward keeps what the backward reads: byte offsets into one buffer.
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
@@ -48,15 +59,6 @@ struct VocabLayout {
   long long bytes;
 };
 VocabLayout vocab_layout(int N, int V, int D, int K, bool distill);
-
-// Workspaces of the backward.  The vocabulary is taken `piece` columns at a time.
-struct VocabPlan {
-  int piece, pieces;
-  int dw_max;            // most K splits of the dw product
-  int slab_rows;         // rows of the fp32 slabs that dx takes
-  long long all_rows;    // with those of dw
-};
-VocabPlan vocab_plan(int N, int V, int D, int want_piece, int num_sms);
 
 struct VocabGradArgs {
   const void* x;         // as the forward read it
@@ -79,7 +81,7 @@ struct VocabGradArgs {
   int dw_f32;
   int dw_add;
   VocabPlan plan;
-  void* g;               // workspace: bf16, vocab_g_rows(N) * piece
+  void* g;               // bf16, vocab_g_rows(N) * piece: workspace, or as the forward left it
   float* slab;           // workspace: fp32 [all_rows, ld_slab]
   long long ld_slab;
 };
@@ -88,8 +90,9 @@ long long vocab_g_rows(int N);
 }  // namespace pcb
 
 int pcb_vocab_pad_rows(const void* src, long long ld, void* dst, long long ldd, int rows, int D, cudaStream_t s);
-// `part`: [granules, N] float2 workspace
-int pcb_vocab_fwd(const pcb::VocabHeadArgs& a, void* saved, void* part, int mean, int num_sms, cudaStream_t s);
+// `part`: [granules, N] float2 workspace; `g`: bf16 [vocab_g_rows(N) * piece] where plan.whole
+int pcb_vocab_fwd(const pcb::VocabHeadArgs& a, const pcb::VocabPlan& plan, void* saved, void* part, void* g, int mean,
+                  int num_sms, cudaStream_t s);
 int pcb_vocab_bwd(const pcb::VocabGradArgs& a, int num_sms, cudaStream_t s);
 
 // x[n] = scale * w[tok[n]]; rows of tokens outside [0, V) are zero

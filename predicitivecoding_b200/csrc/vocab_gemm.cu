@@ -5,6 +5,11 @@
 //   STAT, GRAD   logits tile = x w^T; a thread of the epilogue owns one row (a TMEM lane) and 128 of its logits, so
 //                the softmax statistics need no exchange between threads, and the row's few targets in those
 //                columns are met by walking its ascending list
+//   WHOLE        the same of a vocabulary of up to two tiles, whose logits stay in TMEM until the row's softmax is known:
+//                a second pass over them makes the row's loss and its gradient.  One launch in place of three and 2 of
+//                the 8 N V D operations less: loss and gradients of 2048 rows of 256 against 256 take 28.8 us,
+//                37.1 the other way; of 131072 rows of 768 against 512, 527 and 617.  A loss alone is
+//                quicker without g (2048 rows of 768 against 512: 18 us, 26), so this is for losses with a backward
 //   BWD          dw = g^T x (rows = vocabulary, K = counted rows) and dx = g w (rows = counted rows, K = vocabulary)
 //                as one list of tiles: neither product fills whole waves of 74 pairs by itself, the two share g in
 //                L2, and a small batch saves a launch.  K is split where there are few tiles; the parts go to fp32
@@ -37,10 +42,13 @@ struct Cfg {
   static constexpr int TMEM_COLS = 2 * BN;
   // per epilogue warp: two [32 x 64] bf16 boxes for TMA stores, of which the fp32 path uses one as scratch
   static constexpr int EPI_WARP_BYTES = MODE == HEAD_STAT ? 0 : 8192;
-  static constexpr int STAGES_FIT = (232448 - 2048 - kEpiWarps * EPI_WARP_BYTES) / STAGE_BYTES;
+  // WHOLE: (max, sum) of both halves of a row, losses of one, partial sums of the losses
+  static constexpr int ROW_BYTES = MODE == HEAD_WHOLE ? kBM * 20 + 8 * kEpiWarps + 8 : 0;
+  static constexpr int STAGES_FIT = (232448 - 2048 - kEpiWarps * EPI_WARP_BYTES - ROW_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES + 1024;
-  static constexpr int SMEM_BYTES = EPI_OFF + kEpiWarps * EPI_WARP_BYTES + 1024;
+  static constexpr int ROW_OFF = EPI_OFF + kEpiWarps * EPI_WARP_BYTES;
+  static constexpr int SMEM_BYTES = ROW_OFF + ROW_BYTES + 1024;
   static_assert(SMEM_BYTES <= 232448, "dynamic shared memory above the 227 KB per-block limit");
   static_assert(8 * (2 * STAGES + 4) + 8 <= 1024, "barriers do not fit behind the ring");
 };
@@ -108,6 +116,15 @@ PCB_DEVICE Shape shape_of(const HeadGemm& a, int pairs) {
 // share their operands in L2, and the pairs end within about one of its tiles of one another.
 template <int MODE>
 PCB_DEVICE bool tile_at(const HeadGemm& a, const Shape& s, int pair, int pairs, int u, Tile& r) {
+  if (MODE == HEAD_WHOLE) {   // a pair takes all columns of its rows
+    r.mb = pair + (s.num_n == 2 ? u >> 1 : u) * pairs;
+    r.nb = s.num_n == 2 ? u & 1 : 0;
+    r.dw = false;
+    r.split = 0;
+    r.kb0 = 0;
+    r.kb1 = s.kb_dx;
+    return r.mb < s.num_m;
+  }
   if (MODE != HEAD_BWD) {
     const int t = pair + u * pairs;
     if (t >= s.tiles) return false;
@@ -225,7 +242,7 @@ struct RowTargets {
     if (entry + i < end) {
       const long long at = (long long)n * h.K + entry + i;
       id[i] = h.ids[at];
-      if (MODE == HEAD_GRAD) q[i] = h.q[at];
+      if (MODE != HEAD_STAT) q[i] = h.q[at];
     }
   }
   PCB_DEVICE float* z(const HeadGemm& h) const { return h.z + (long long)m * h.K + entry; }
@@ -284,6 +301,37 @@ PCB_DEVICE void add_half(uint32_t taddr, uint32_t (&v)[32]) {
   for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[j]));
 }
 
+// 32 logits, `nvalid` of them in the vocabulary, joined to a running (max, sum 2^(c l - max))
+PCB_DEVICE void join32(float c, float (&v)[32], int nvalid, float& mx, float& sum) {
+  if (nvalid < 32) {   // warp-uniform
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : -INFINITY;
+  }
+  float cm[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cm[j] = max3(v[8 * j], v[8 * j + 1], v[8 * j + 2]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 3], v[8 * j + 4]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 5], v[8 * j + 6]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cm[j] = fmaxf(cm[j], v[8 * j + 7]);
+  const float nm = fmaxf(mx, max3(fmaxf(cm[0], cm[1]), cm[2], cm[3]) * c);
+  const float ref = nm == -INFINITY ? 0.f : nm;
+  float s[8] = {};
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float e0, e1;
+    scale2(e0, e1, v[j], v[j + 1], c, -ref);
+    add2(s[j & 7], s[(j & 7) + 1], ex2_approx(e0), ex2_approx(e1));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) add2(s[j], s[j + 1], s[j + 4], s[j + 5]);
+  add2(s[0], s[1], s[2], s[3]);
+  sum = fmaf(sum, ex2_approx(mx - ref), s[0] + s[1]);
+  mx = nm;
+}
+
 // (max, sum 2^(c l - max)) of this thread's 128 logits, in one pass with a running maximum, and the logits at the
 // row's targets.  The maximum stays in units of c l, and the sum is taken against that rounded value, so the
 // log-sum-exp made of the pair carries no error of the product c * max.  The next 32 columns come from TMEM while
@@ -306,34 +354,7 @@ PCB_DEVICE void stat128(const HeadGemm& a, RowTargets& r, uint32_t taddr, int co
       r.advance<HEAD_STAT>(a);
     }
     __syncwarp();
-    const int nvalid = a.cols - (col0 + 32 * i);   // warp-uniform
-    if (nvalid < 32) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : -INFINITY;
-    }
-    float cm[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = max3(v[8 * j], v[8 * j + 1], v[8 * j + 2]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 3], v[8 * j + 4]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = max3(cm[j], v[8 * j + 5], v[8 * j + 6]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) cm[j] = fmaxf(cm[j], v[8 * j + 7]);
-    const float nm = fmaxf(mx, max3(fmaxf(cm[0], cm[1]), cm[2], cm[3]) * a.c);
-    const float ref = nm == -INFINITY ? 0.f : nm;
-    float s[8] = {};
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      float e0, e1;
-      scale2(e0, e1, v[j], v[j + 1], a.c, -ref);
-      add2(s[j & 7], s[(j & 7) + 1], ex2_approx(e0), ex2_approx(e1));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) add2(s[j], s[j + 1], s[j + 4], s[j + 5]);
-    add2(s[0], s[1], s[2], s[3]);
-    sum = fmaf(sum, ex2_approx(mx - ref), s[0] + s[1]);
-    mx = nm;
+    join32(a.c, v, a.cols - (col0 + 32 * i), mx, sum);
     between(i);
   }
   if (r.live) a.part[(long long)(r.lo >> 7) * a.N + r.m] = make_float2(mx, sum);
@@ -420,6 +441,178 @@ PCB_DEVICE void store_box64(const CUtensorMap* map, uint8_t* stg, int& box_at, c
   }
 }
 
+PCB_DEVICE void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// whether `p` holds for all of them
+PCB_DEVICE bool bar_and(int id, int threads, bool p) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %1, 0;\n\tbar.red.and.pred b, %2, %3, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+      : "=r"(r)
+      : "r"((int)p), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+// ---------------------------------------------------------------- WHOLE's epilogue
+// Two threads share a row: each owns 128 columns of every tile.  The first pass makes their softmax statistics, which
+// the two exchange; the second the row's entries of g and, where it meets a target, the loss.  Both go through 32 columns
+// at a time in a loop that is not unrolled: most launches run this code once on an SM, and fetching it counts (2048
+// rows, 256 x 256: 13.1 us for the launch, 14.3 with the four steps written out; 512 rows, 260 x 256, 16 targets
+// each: 19.2, 22.6).
+PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, uint8_t* stg, const CUtensorMap* tmC,
+                           uint32_t tmem_base, uint64_t* tfull, const uint32_t (&tempty_leader)[2], int pair, int pairs,
+                           uint32_t rank, volatile int* abort_flag) {
+  constexpr int kEpi = 32 * kEpiWarps;
+  float2* stats = reinterpret_cast<float2*>(smem);                          // [2][kBM]
+  float* losses = reinterpret_cast<float*>(smem + kBM * 16);                // [kBM]
+  double* sums = reinterpret_cast<double*>(smem + kBM * 20);
+  volatile int* last = reinterpret_cast<volatile int*>(sums + kEpiWarps);
+  const int tid = threadIdx.x - 64, lane = tid & 31, q = (threadIdx.x >> 5) & 3, half = tid >> 7;
+  const int mine = q * 32 + lane;
+  Tile tile;
+  RowTargets ahead;
+  auto row_of = [&](const Tile& t) { return t.mb * 2 * kBM + (int)rank * kBM + q * 32; };
+  if (tile_at<HEAD_WHOLE>(a, sh, pair, pairs, 0, tile)) {
+    ahead.ask_row<HEAD_WHOLE>(a, row_of(tile) + lane, half * 128, sh.rows);
+    ahead.ask_entries(a);
+    ahead.ask_ids<HEAD_WHOLE>(a);
+  }
+  for (int u = 0; tile_at<HEAD_WHOLE>(a, sh, pair, pairs, u, tile); u += sh.num_n) {
+    const int row0 = row_of(tile);
+    const bool live = row0 + lane < sh.rows;
+    const int place = live ? a.row[row0 + lane] : 0;
+    float mx = -INFINITY, sum = 0.f;
+    bool ok = true;
+#pragma unroll 1
+    for (int nb = 0; nb < sh.num_n; ++nb) {
+      const int acc = (u + nb) & 1, col0 = nb * 256 + half * 128;
+      // behind a wait that ran out the barriers below are still met, and both threads of a row leave together
+      ok = mbar_wait(&tfull[acc], ((u + nb) >> 1) & 1, a.err, kErrTimeoutTmemFull, abort_flag) && ok;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + half * 128;
+#pragma unroll 1
+      for (int i = 0; i < 4 && col0 + 32 * i < a.cols; ++i) {
+        float v[32];
+        load32(taddr + 32 * i, v);
+        join32(a.c, v, a.cols - (col0 + 32 * i), mx, sum);
+      }
+    }
+    stats[half * kBM + mine] = make_float2(mx, sum);
+    ok = bar_and(1 + q, 64, ok);
+    const float2 s0 = stats[mine], s1 = stats[kBM + mine];
+    const float m = fmaxf(s0.x, s1.x), ref = m == -INFINITY ? 0.f : m;
+    const float tot = s0.y * exp2f(s0.x - ref) + s1.y * exp2f(s1.x - ref);
+    const float lt = log2f(tot), over = 1.f / tot;
+    float l = 0.f;
+#pragma unroll 1
+    for (int nb = 0; nb < sh.num_n; ++nb) {
+      const int acc = (u + nb) & 1, col0 = nb * 256 + half * 128;
+      RowTargets r = ahead;
+      Tile after;
+      const bool more = tile_at<HEAD_WHOLE>(a, sh, pair, pairs, u + nb + 1, after);
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + half * 128;
+      uint4 low[4];   // of the panel's first half
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        if (more) {   // the next tile's targets, under this one's arithmetic
+          if (i == 0) ahead.ask_row<HEAD_WHOLE>(a, row_of(after) + lane, after.nb * 256 + half * 128, sh.rows);
+          if (i == 1) ahead.ask_entries(a);
+          if (i == 2) ahead.ask_ids<HEAD_WHOLE>(a);
+        }
+        const int col = col0 + 32 * i, panel = col / 64;
+        if (64 * panel >= a.cols) continue;   // warp-uniform
+        float z[32], v[32];
+        load32(taddr + 32 * i, z);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          float e0, e1;
+          scale2(e0, e1, z[j], z[j + 1], a.c, -ref);
+          mul2(v[j], v[j + 1], ex2_approx(e0), ex2_approx(e1), over);
+        }
+        const int nvalid = live ? a.cols - col : 0;   // what stands in a row that is not counted may be anything
+        if (!__all_sync(0xffffffffu, nvalid >= 32)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = j < nvalid ? v[j] : 0.f;
+        }
+        // a panel's box of high terms and one of low terms, as TMA stores them; until the latter is filled, each lane's row of
+        // it holds its 32 entries while the targets are taken off
+        if ((i & 1) == 0) {
+          if (lane == 0) bulk_group_wait_read<0>();   // the last panel's stores are done with the boxes
+          __syncwarp();
+        }
+        uint8_t* box = stg + lane * 128;
+        float4* cells = reinterpret_cast<float4*>(box + 4096);
+        const int end = r.lo + 32 * (i + 1);
+        if (r.id[0] < end) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            cells[j ^ (lane & 7)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          do {
+            const int o = r.id[0] - r.lo - 32 * i;
+            const float w = r.q[0];
+            // sum_k q_k (log2 q_k - log2 p_k); the difference of the logit and ref first, in one rounding; 0 log 0 = 0
+            if (w != 0.f) l += w * (log2f(w) + (fmaf(-a.c, pick32(z, o), ref) + lt));
+            reinterpret_cast<float*>(cells + ((o >> 2) ^ (lane & 7)))[o & 3] -= w;
+            r.advance<HEAD_WHOLE>(a);
+          } while (r.id[0] < end);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = cells[j ^ (lane & 7)];
+            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[k] = pack_bf16x2(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
+          const int at = (4 * (i & 1) + j) ^ (lane & 7);
+          reinterpret_cast<uint4*>(box)[at] = make_uint4(p[0], p[1], p[2], p[3]);
+          if (sh.two) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              p[k] = pack_bf16x2(v[8 * j + 2 * k] - bf16_lo(p[k]), v[8 * j + 2 * k + 1] - bf16_hi(p[k]));
+            if (i & 1) {
+              reinterpret_cast<uint4*>(cells)[j ^ (lane & 7)] = low[j];
+              reinterpret_cast<uint4*>(cells)[at] = make_uint4(p[0], p[1], p[2], p[3]);
+            } else {
+              low[j] = make_uint4(p[0], p[1], p[2], p[3]);
+            }
+          }
+        }
+        if (i & 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(tmC, stg, 0, panel * a.g_rows + row0);
+            if (sh.two) tma_store_2d(tmC, stg + 4096, 0, panel * a.g_rows + row0 + a.g_low);
+            bulk_group_commit();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(tempty_leader[acc]);
+    }
+    if (half) losses[mine] = l;
+    bar_sync(1 + q, 64);
+    if (!half && live) a.loss[place] = (l + losses[mine]) * a.factor;
+    if (!ok) break;
+  }
+  if (lane == 0) bulk_group_wait_all();   // every TMA store has landed
+  if (a.scalars == nullptr) return;
+  bar_sync(5, kEpi);
+  if (tid == 0) {   // one fence for what all of these threads wrote before the barrier, and will read after the next
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.done) : "memory");
+    *last = before == (int)gridDim.x - 1;
+  }
+  bar_sync(5, kEpi);
+  if (!*last) return;
+  add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.scalars, sums, tid, [] { bar_sync(5, kEpi); });
+}
+
 PCB_DEVICE bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 PCB_DEVICE void store4(float* c, float (&o)[4], int nv, bool add) {
@@ -459,7 +652,7 @@ PCB_DEVICE void store4(__nv_bfloat16* c, float (&o)[4], int nv, bool add) {
 static bool in_halves(int N, int D) { return N <= kTwoTermRows && D >= 1024; }
 
 // ---------------------------------------------------------------- kernel
-// STAT, GRAD: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x,
+// STAT, GRAD, WHOLE: tmA = packed x, tmX = x, tmB = w, tmC = g.   BWD: tmA = g, tmB = w, tmC = dw, tmD = packed x, tmX = x,
 // tmS = fp32 slabs.
 template <int MODE, int BN, bool HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -554,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (MODE == HEAD_GRAD && lane == 0 && !leader && pair_id == 0 && a.v0 == 0) plan_splits(a, sh.rows, a.bwd_pairs, a.plan);
+    if ((MODE == HEAD_GRAD || MODE == HEAD_WHOLE) && lane == 0 && !leader && pair_id == 0 && a.v0 == 0) plan_splits(a, sh.rows, a.bwd_pairs, a.plan);
     if (lane == 0 && leader) {
       // ---------------- MMA issuer (leader only) ----------------
       int stage = 0;
@@ -598,6 +791,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (acc == 0) acc_phase ^= 1u;
       }
     }
+  } else if (MODE == HEAD_WHOLE) {
+    const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
+    whole_rows(a, sh, smem + C::ROW_OFF, smem + C::EPI_OFF + (warp - 2) * C::EPI_WARP_BYTES, &tmC, tmem_base, tfull,
+               tempty_leader, pair_id, num_pairs, rank, abort_flag);
   } else {
     // ---------------- epilogue warps (both CTAs, 128 rows each) ----------------
     const int q = warp & 3;
@@ -796,6 +993,8 @@ static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int n
 using namespace pcb;
 using namespace pcb::head;
 
+bool pcb_head_whole(int N, int V, int D) { return V <= kWholeColumns && !in_halves(N, D); }
+
 int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
                   const void* w, long long ldw, void* g, int num_sms, cudaStream_t s) {
   if (a.N < 1 || a.D < 1 || a.cols < 1 || num_sms < 2) return -1;
@@ -814,7 +1013,11 @@ int pcb_head_gemm(int mode, HeadGemm a, const void* x, long long ldx, const void
   else if (!map2(&t[4], x_all, a.D, a.N, ldx_all, xrows)) return -5;
   if (!bwd) {
     if (!map2(&t[1], w, a.D, a.cols, ldw, 128)) return -5;
-    if (mode == HEAD_GRAD && !map2(&t[2], g, 64, panels * a.g_rows, 64, 32)) return -5;
+    if (mode != HEAD_STAT && !map2(&t[2], g, 64, panels * a.g_rows, 64, 32)) return -5;
+    if (mode == HEAD_WHOLE) {
+      if (!pcb_head_whole(a.N, a.cols, a.D)) return -1;
+      return launch<HEAD_WHOLE, 256>(t, a, num_m, num_sms, s);
+    }
     // the blocks that run side by side share the operand with the larger footprint
     a.row_blocks_last = a.N > a.cols;
     const int tiles = num_m * ((a.cols + 255) / 256);

@@ -30,7 +30,12 @@ enum HeadMode : int {
   HEAD_STAT = 0,   // logits -> (max, sum) of every 128 of a row, and the logits at its targets
   HEAD_GRAD = 1,   // logits -> g = softmax - target distribution, bf16
   HEAD_BWD = 2,    // dw = g^T x and dx = g w in one launch
+  HEAD_WHOLE = 3,  // a vocabulary of up to kWholeColumns: logits -> row losses, their sum and g
 };
+
+// Columns of logits that the accumulators of a tile row hold together: up to there the softmax of a row is known before
+// its logits are gone, and they need not be made again for the gradient.
+constexpr int kWholeColumns = 512;
 
 struct HeadGemm {
   int N, D;               // rows of the batch, width
@@ -50,6 +55,12 @@ struct HeadGemm {
   // STAT
   float2* part;           // [2 ceil(V / 256), N] (max, sum), by packed row
   float* z;               // [N, K] logits at the ids, by packed row
+  // WHOLE
+  float* loss;            // [N] by batch row: factor * the divergence in bits
+  float factor;
+  float* scalars;         // as row_loss_kernel leaves them (nullptr: not wanted)
+  int mean;
+  int* done;              // CTAs that are done, 0 before the launch
   // GRAD, BWD
   const float2* norm;     // [N] (r, 1 / sum of 2^(c l - r)), by packed row
   // g: panels of 64 columns, each [g_rows, 64], so that every box that is stored or loaded (32 or 64 rows of a panel) is
@@ -114,9 +125,33 @@ __device__ inline void plan_splits(const HeadGemm& a, int rows, int pairs, int* 
   }
 }
 
+// The last step of a loss: the rows' losses added up by THREADS threads in a fixed order and in 64 bits.  scalars[0] = their
+// sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).  `sync` joins the threads.
+template <int THREADS, typename F>
+__device__ inline void add_losses(const float* loss, int N, int rows, int mean, float* scalars, double* sums, int tid, F sync) {
+  double t = 0.0;
+#pragma unroll 8
+  for (int i = tid; i < N; i += THREADS) t += __ldcg(loss + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((tid & 31) == 0) sums[tid >> 5] = t;
+  sync();
+  if (tid < 32) {
+    t = tid < THREADS / 32 ? sums[tid] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (tid == 0) {
+      scalars[0] = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
+      scalars[1] = rows > 0 ? 1.f / (float)rows : 0.f;
+    }
+  }
+}
+
 }  // namespace pcb
 
 // x: packed rows [N, ldx]; x_all: the batch itself (nullptr: cannot be read in place); w: [cols, D] rows v0..; g: panels of 64
 // columns.  Returns 0, -1 (operands), -3 (launch), -5 (tensor map).
 int pcb_head_gemm(int mode, pcb::HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all,
                   const void* w, long long ldw, void* g, int num_sms, cudaStream_t s);
+// whether HEAD_WHOLE takes these sizes
+bool pcb_head_whole(int N, int V, int D);

@@ -13,7 +13,8 @@ Shapes: tokens and targets [...] int32 or int64, w [V, D] (nn.Linear layout, the
 The losses take bf16 x and w, multiply on the tensor cores and hold the logits, the softmax statistics and every sum
 in fp32; the logits themselves are never stored.  ``head_bwd`` makes them again, ``piece`` columns of the vocabulary
 at a time, which costs 8 N V D operations for a step instead of 6 and needs N * piece * 2 bytes (256 MiB by default)
-instead of N * V * 2.  softmax - target is rounded to bf16 once, as an operand of the two gradient products.
+instead of N * V * 2.  A vocabulary of up to 512 whose N * V * 2 bytes stay within that bound is the exception: its loss
+is taken together with the gradient of its logits, which the state then keeps.  softmax - target is rounded to bf16 once, as an operand of the two gradient products.
 
 Rows that are not counted - a target outside [0, V) or equal to ``ignore_index``, a teacher's list without entries -
 have loss 0 and gradient 0, are not read and cost no products; the mean is over the counted rows, and 0 when there
@@ -22,7 +23,7 @@ are none.  A teacher's entry is absent when its id is outside [0, V) or its logi
 The ids of a row's list are meant to differ; entries that repeat an id count as they stand in the loss, and together
 in the gradient.  All results are the same from run to run: no sum depends on the order in which atomics arrive.
 x and w are read again by ``head_bwd`` and must not change in between.
-Kernels: csrc/vocab.cu, csrc/vocab_epilogue.cuh, csrc/gemm2_tcgen05.cu.
+Kernels: csrc/vocab.cu, csrc/vocab_gemm.cu.
 """
 from __future__ import annotations
 
@@ -75,16 +76,18 @@ def embedding(tok: torch.Tensor, w: torch.Tensor, scale: float = 1.0,
 
 # --------------------------------------------------------------------------- head losses
 def ce_fwd(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -1,
-           reduction: str = "mean") -> Tuple[torch.Tensor, HeadState]:
-    """Softmax cross entropy of the head x w^T without its logits: (fp32 loss, state for :func:`head_bwd`)."""
-    return ext().vocab_ce_fwd(x, w, targets, ignore_index, reduction)
+           reduction: str = "mean", gradient: bool = True) -> Tuple[torch.Tensor, HeadState]:
+    """Softmax cross entropy of the head x w^T without its logits: (fp32 loss, state for :func:`head_bwd`).
+    ``gradient=False``: no backward will follow."""
+    return ext().vocab_ce_fwd(x, w, targets, ignore_index, reduction, gradient)
 
 
 def distill_fwd(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, temperature: float = 1.0,
-                reduction: str = "mean") -> Tuple[torch.Tensor, HeadState]:
+                reduction: str = "mean", gradient: bool = True) -> Tuple[torch.Tensor, HeadState]:
     """Divergence of the student's softmax from the teacher's, which is known by its top logits: ids (int) and logits
-    (fp32 or bf16) [..., K], in any order, K <= 256; (fp32 loss, state for :func:`head_bwd`)."""
-    return ext().vocab_distill_fwd(x, w, ids, logits, temperature, reduction)
+    (fp32 or bf16) [..., K], in any order, K <= 256; (fp32 loss, state for :func:`head_bwd`).
+    ``gradient=False``: no backward will follow."""
+    return ext().vocab_distill_fwd(x, w, ids, logits, temperature, reduction, gradient)
 
 
 def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optional[torch.Tensor] = None,
@@ -92,7 +95,8 @@ def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optio
              piece: int = 0) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx [..., D], dw [V, D]) of a mean or summed loss times ``gout`` (a number, or an fp32 CUDA tensor with one
     value).  They are bf16, or go into ``dx`` / ``dw`` (bf16 or fp32; ``accumulate`` adds to ``dw``).  ``piece``: columns of
-    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of workspace take).  x and w must
+    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of workspace take; a vocabulary of up
+    to 512 may be taken whole).  x and w must
     still hold what the loss read."""
     if isinstance(gout, torch.Tensor):
         return ext().vocab_head_bwd(state, 1.0, gout, dx, dw, need_dx, need_dw, accumulate, piece)
@@ -114,19 +118,23 @@ class _HeadLoss(torch.autograd.Function):
         return dx, dw, None, None, None
 
 
+def _differentiated(x: torch.Tensor, w: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+
+
 def cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -1,
                   reduction: str = "mean") -> torch.Tensor:
     """Differentiable :func:`ce_fwd` (mean or sum; ``none`` has no gradient)."""
-    if reduction == "none":
-        return ce_fwd(x, w, targets, ignore_index, reduction)[0]
+    if reduction == "none" or not _differentiated(x, w):
+        return ce_fwd(x, w, targets, ignore_index, reduction, gradient=False)[0]
     return _HeadLoss.apply(x, w, "ce", (targets, ignore_index), reduction)
 
 
 def distill(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, temperature: float = 1.0,
             reduction: str = "mean") -> torch.Tensor:
     """Differentiable :func:`distill_fwd` by x and w (mean or sum); the teacher's logits get no gradient."""
-    if reduction == "none":
-        return distill_fwd(x, w, ids, logits, temperature, reduction)[0]
+    if reduction == "none" or not _differentiated(x, w):
+        return distill_fwd(x, w, ids, logits, temperature, reduction, gradient=False)[0]
     return _HeadLoss.apply(x, w, "distill", (ids, logits, temperature), reduction)
 
 

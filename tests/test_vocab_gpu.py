@@ -255,6 +255,47 @@ def test_pieces_and_outputs(piece):
     assert none is None and torch.equal(only_dw, vocab.head_bwd(state, piece=piece)[1])
 
 
+@pytest.mark.parametrize("N,V", [(256, 512), (255, 511), (257, 385), (513, 512), (900, 320), (40000, 257), (5, 33)])
+@pytest.mark.parametrize("K", [0, 5, 33])
+def test_vocabularies_taken_whole(N, V, K):
+    """Row blocks that end inside a tile, columns that end in each of its parts, one and several blocks a pair of SMs,
+    one and two terms; more targets in 32 columns than are held ahead; the loss without its gradient is the same."""
+    x, w, own, g = head(N, V, 48, N + V + K)
+    if K:
+        ids, t = teacher(N, V, K, own, g, torch.float32)
+        q, live = targets64(V, ids=ids, t=t, T=1.5)
+        T, fwd = 1.5, lambda r, **k: vocab.distill_fwd(x, w, ids, t, 1.5, r, **k)
+    else:
+        own[1::7] = -1
+        q, live = targets64(V, tgt=own)
+        T, fwd = 1.0, lambda r, **k: vocab.ce_fwd(x, w, own, reduction=r, **k)
+    x[~live] = float("nan")
+    check_head(x, w, q, live, T, fwd, "mean", gout=1.5)
+    loss, state = fwd("sum")
+    first = vocab.head_bwd(state)
+    for a, b in zip(first, vocab.head_bwd(state, piece=256)):   # again, from the same state
+        assert torch.equal(a, b)
+    alone, refused = fwd("sum", gradient=False)
+    rows = fwd("none")[0].double()
+    assert abs(float(alone) - float(loss)) <= 2.0 ** -19 * float(rows.abs().sum()) + 1e-5 * N
+    with pytest.raises(ValueError):
+        vocab.head_bwd(refused)
+    assert state.status() == 0
+
+
+def test_a_whole_vocabulary_with_infinities():
+    """Logits of -inf and +inf in one row reach that row's loss and gradient, and no other row's."""
+    x, w, tgt, g = head(300, 300, 64, 3)
+    clean_loss = vocab.ce_fwd(x, w, tgt, reduction="none")[0]
+    dx = vocab.head_bwd(vocab.ce_fwd(x, w, tgt, reduction="sum")[1], need_dw=False)[0]
+    x[17] = float("inf")
+    loss, state = vocab.ce_fwd(x, w, tgt, reduction="sum")
+    bad = vocab.head_bwd(state, need_dw=False)[0]
+    keep = torch.arange(300, device=DEV) != 17
+    assert not bool(torch.isfinite(loss)) and not bool(torch.isfinite(bad[17].float()).all())
+    assert torch.equal(bad[keep], dx[keep]) and bool(torch.isfinite(clean_loss).all())
+
+
 @pytest.mark.parametrize("rows,ignored", [(9000, 0.5), (8193, 0.99), (600, 0.0), (257, 0.0), (256, 0.0)])
 @pytest.mark.parametrize("V,piece", [(40, 0), (700, 256)])
 def test_long_batches_and_the_edge_of_two_terms(rows, ignored, V, piece):
