@@ -644,7 +644,7 @@ at::Tensor vocab_embed_bwd(const at::Tensor& tok, const at::Tensor& dx, int64_t 
   check(pcb_vocab_embed_bwd(t.data_ptr(), t64, d2.data_ptr(), xb, rows_apart(d2), out->data_ptr(),
                             out->scalar_type() == at::kBFloat16, N, V, D, (float)scale, accumulate ? 1 : 0, ws.data_ptr(),
                             num_sms(), cur_stream()),
-        "embed_bwd", 3);
+        "embed_bwd", pcb_vocab_embed_bwd_launches(N, V, D, out->scalar_type() == at::kBFloat16, accumulate ? 1 : 0));
   return *out;
 }
 

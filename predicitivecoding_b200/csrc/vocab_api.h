@@ -100,6 +100,8 @@ int pcb_vocab_embed_fwd(const void* tok, int tok64, const void* w, int w_bf16, l
                         int N, int V, int D, float scale, cudaStream_t s);
 // bytes of workspace of the embedding gradient
 long long pcb_vocab_embed_bwd_bytes(int N, int V, int D);
+// kernels that the gradient launches
+int pcb_vocab_embed_bwd_launches(int N, int V, int D, int dw_bf16, int add);
 // dw[v] (+)= scale * sum of dx[n] over tok[n] == v in ascending n
 int pcb_vocab_embed_bwd(const void* tok, int tok64, const void* dx, int dx_bf16, long long lddx, void* dw, int dw_bf16,
                         int N, int V, int D, float scale, int add, void* ws, int num_sms, cudaStream_t s);

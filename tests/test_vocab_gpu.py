@@ -80,6 +80,37 @@ def test_embedding(N, V, D, kind, wt, xt, idt):
     assert torch.equal(acc[untouched], start[untouched])
 
 
+def check_embedding_grad(tok, V, dx, wt, scale=0.6):
+    exact = torch.zeros(V, dx.shape[1], device=DEV, dtype=torch.float64)
+    at = torch.nonzero((tok >= 0) & (tok < V))[:, 0]
+    exact.index_add_(0, tok[at], dx[at].double() * scale)
+    size = torch.zeros_like(exact).index_add_(0, tok[at], dx[at].double().abs() * scale)
+    n = torch.bincount(tok[at], minlength=V)[:, None]
+    out = torch.full((V, dx.shape[1]), float("nan"), device=DEV, dtype=wt)    # every element is written
+    dw = vocab.embed_bwd(tok, dx, V, scale, out=out)
+    bound = (n + 2) * E * size + (U * exact.abs() if wt == torch.bfloat16 else 0)
+    assert bool(((dw.double() - exact).abs() <= bound).all())
+    assert torch.equal(dw, vocab.embed_bwd(tok, dx, V, scale, dtype=wt))
+    return dw
+
+
+@pytest.mark.parametrize("N", [15, 16, 17, 511, 512, 513, 1023, 1024, 1025])
+@pytest.mark.parametrize("V,D", [(3, 129), (2500, 40), (40000, 210)])
+def test_embedding_gradient_of_few_tokens(N, V, D):
+    """Either side of the sizes up to which nothing is sorted (1024 tokens, 512 into a large matrix); tokens of 16 and 17
+    places, of a whole batch, met first in one part of the batch."""
+    g = gen(N + V)
+    dx = torch.randn(N, D, device=DEV, generator=g)
+    for kind in ("zipf", "one", "pad"):
+        check_embedding_grad(tokens(N, V, kind, g), V, dx, torch.float32)
+    tok = torch.arange(N, device=DEV) // 17 % V                              # runs of 17, the last one shorter
+    fp32 = check_embedding_grad(tok, V, dx, torch.float32)
+    check_embedding_grad((torch.arange(N, device=DEV) * 7) % min(V, N // 16 + 1), V, dx.bfloat16(), torch.bfloat16)
+    base = torch.randn(V, D, device=DEV, generator=g)
+    both = vocab.embed_bwd(tok, dx, V, 0.6, out=base.clone(), accumulate=True)
+    assert float((both - (base + fp32)).abs().max()) <= 4 * E * float((base.abs() + fp32.abs()).max())
+
+
 def test_embedding_strides_and_shapes():
     g = gen(3)
     w = torch.randn(50, 80, device=DEV, generator=g)[:, 3:40]           # rows apart, unaligned
