@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(32 * sort_rows(R))
 // accumulation, cut off at each of its D / 16 steps, loses (one row, D 1600: a loss 7e-6 off), and which the loss of
 // few rows does not average out.  Both modes make the same logits, bit for bit: a row that is sure of its target has
 // the sum of its other probabilities in p - q.  A block takes 128 rows of w, a warp four of them at a time, its lanes
-// 8 columns each in turn; x stands in shared memory.  Scoring 1, 2, 4 and 8 rows of 2048 against 32000: 36, 35, 41 and
-// 57 us, on the tensor cores 43, 39, 41 and 39, where the losses are 0.2 to 0.7e-6 off instead of 0.05e-6.
+// 8 columns each in turn; x stands in shared memory.  Losses of 1, 2, 4 and 8 rows of 2048 against 32000: 36, 35, 41 and
+// 57 us, on the tensor cores 43, 39, 41 and 39, where they are 0.2 to 0.7e-6 off instead of 0.05e-6.  (A loss without
+// gradient over many columns is score_kernel's: 31.5, 33.0, 31.9 us, at most 0.15e-6 off.)
 constexpr int kFewRows = 4;
 constexpr int few_threads(int rows) { return rows <= 2 ? 1024 : 512; }   // as many as registers allow: a small w has few blocks
 constexpr int kFewColumns = 24 * 1024;   // of x in shared memory
@@ -1264,6 +1265,9 @@ VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num
   r.dw_max = r.pieces == 1 ? (int)std::max(1LL, std::min(8LL, num_sms / 2 / tiles)) : 1;
   r.slab_rows = (int)std::min((N + 255LL) / 256 * 256 + 16 * 256, 1LL << 30);
   r.all_rows = r.slab_rows + (r.dw_max > 1 ? r.dw_max * all : 0);
+  // a block of 128 columns an SM at least, or the FMA units are quicker: one row of 1600 against 300 takes 12.4 us, 16.2
+  // by score_kernel; one of 2048 against 32000 35.8 and 31.5
+  r.score = !gradient && N <= kScoreRows && !(few_rows(N, D) && V <= 128LL * num_sms);
   // g then lives as long as the forward's state, so it is bounded as a piece is
   r.whole = gradient && r.pieces == 1 && !few_rows(N, D) && pcb_head_whole(N, V, D);
   return r;
@@ -1396,6 +1400,10 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
   g.start = start;
   g.part = (float2*)part;
   g.z = z;
+  if (plan.score) {
+    const int rc = pcb_head_score(g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, s);
+    return rc ? rc : finish(l, (a.V + 127) / 128);
+  }
   if (few_rows(a.N, a.D)) {
     const int rc = launch_few_rows<false>(g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, nullptr, s);
     return rc ? rc : finish(l, (a.V + 127) / 128);

@@ -36,6 +36,7 @@ struct VocabPlan {
   int dw_max;            // most K splits of the dw product
   int slab_rows;         // rows of the fp32 slabs that dx takes
   long long all_rows;    // with those of dw
+  bool score;            // a few rows' loss alone
   bool whole;            // a small vocabulary: the forward makes the gradient of the logits, g, along with the loss
 };
 // `gradient`: for a forward that a backward follows

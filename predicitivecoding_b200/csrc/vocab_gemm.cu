@@ -5,6 +5,7 @@
 //   STAT, GRAD   logits tile = x w^T; a thread of the epilogue owns one row (a TMEM lane) and 128 of its logits, so
 //                the softmax statistics need no exchange between threads, and the row's few targets in those
 //                columns are met by walking its ascending list
+//   (the loss of a few rows without gradient has a kernel of its own, below)
 //   WHOLE        the same of a vocabulary of up to two tiles, whose logits stay in TMEM until the row's softmax is known:
 //                a second pass over them makes the row's loss and its gradient.  One launch in place of three and 2 of
 //                the 8 N V D operations less: loss and gradients of 2048 rows of 256 against 256 take 28.8 us,
@@ -937,6 +938,161 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
 }
 
+// ---------------------------------------------------------------- the loss of a few rows
+// STAT for up to kScoreRows rows of which only the loss is wanted.  Reading w bounds it, so the product is turned round: 128
+// rows of w are the matrix instruction's M and the batch its N, no operand is padded to 256 rows, and a block of 100
+// KB of stages leaves room for another one on the SM, whose loads go on while this one is in its epilogue.  Nothing
+// before the launch in this stream writes w that has not ended (the kernel that packs the rows waited for it), so the
+// first stages of w are asked for before the wait for the packed rows.  The sum over D is taken in up to eight parts,
+// each in an accumulator of its own: the tensor cores cut off what D / 16 / 8 steps lose, not D / 16.
+// 32 rows of 2048 against 32000: 31.7 us for the call and losses 1e-7 off, 38 and 4e-7 by tiles of 256 rows; 64 rows 33
+// against 42 to 49, 128 rows 40 against 50; this kernel alone 25.8 us at 32 rows, of which 131 MB take 20.  The gradient
+// has to make the same logits again, bit for bit, so a loss that it follows is not taken here.
+constexpr int kScoreThreads = 128;
+
+template <int NB>   // rows of a block
+struct Score {
+  static constexpr int W = 128 * kBK * 2, X = NB * kBK * 2, STAGE = W + X;
+  static constexpr int STAGES = 110 * 1024 / STAGE;   // 5, 4, 3
+  static constexpr int PARTS = 256 / NB;
+  static constexpr int SMEM = STAGES * STAGE + 256 + 1024;
+  static constexpr int LD = 132;   // floats between the rows of the logits in shared memory
+  static_assert(NB * LD * 4 <= STAGES * STAGE, "logits do not fit in the ring");
+  static_assert(2 * (SMEM + 1024) <= 233472, "two blocks on an SM");
+};
+
+template <int NB>
+__global__ void __launch_bounds__(kScoreThreads, 2)
+    score_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
+                 const __grid_constant__ CUtensorMap tmX, const HeadGemm a) {
+  using C = Score<NB>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* done = empty + C::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int lo = blockIdx.x * 128;
+  const int kbs = (a.D + kBK - 1) / kBK, parts = min(kbs, C::PARTS), pre = min(kbs, C::STAGES);
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    for (int i = 0; i < pre; ++i) {
+      mbar_arrive_expect_tx(&full[i], C::STAGE);
+      tma_load_2d(smem + i * C::STAGE, &tmW, &full[i], i * kBK, lo);
+    }
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+  // behind the product a few threads have a row: what they need of it
+  constexpr int kPer = kScoreThreads / NB;
+  const int m = tid / kPer, first = tid % kPer;
+  const int rows = min(*a.count, a.N);
+  const bool live = m < rows;
+  const int n = !live ? 0 : a.start != nullptr ? a.row[m] : a.ids[m];   // batch row, or the class
+  int entry = 0, end = 0;
+  if (live && a.start != nullptr) {
+    const unsigned short* s = a.start + (long long)blockIdx.x * a.N + n;
+    entry = s[0];
+    end = s[a.N];
+  }
+  if (warp == 0 && lane == 0) {
+    const CUtensorMap* x = a.dense && rows == a.N ? &tmX : &tmA;
+    for (int i = 0; i < pre; ++i) tma_load_2d(smem + i * C::STAGE + C::W, x, &full[i], i * kBK, 0);
+    for (int i = pre; i < kbs; ++i) {
+      const int s = i % C::STAGES;
+      if (!mbar_wait(&empty[s], ((i / C::STAGES) & 1) ^ 1u, a.err, kErrTimeoutEmpty, abort_flag)) break;
+      mbar_arrive_expect_tx(&full[s], C::STAGE);
+      tma_load_2d(smem + s * C::STAGE, &tmW, &full[s], i * kBK, lo);
+      tma_load_2d(smem + s * C::STAGE + C::W, x, &full[s], i * kBK, 0);
+    }
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = make_idesc_bf16(128, NB, 0, 0);
+    int part = -1, next = 0;   // k-block at which the next part begins
+    for (int i = 0; i < kbs; ++i) {
+      const int s = i % C::STAGES;
+      const bool fresh = i == next;
+      if (fresh) {
+        ++part;
+        next = kbs * (part + 1) / parts;
+      }
+      if (!mbar_wait(&full[s], (i / C::STAGES) & 1, a.err, kErrTimeoutFull, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t sw = smem_u32(smem + s * C::STAGE);
+#pragma unroll
+      for (int k = 0; k < kBK / 16; ++k)
+        umma_bf16(tmem + part * NB, make_smem_desc(sw + k * 32, 16, 1024, 2),
+                  make_smem_desc(sw + C::W + k * 32, 16, 1024, 2), idesc, fresh && k == 0 ? 0u : 1u);
+      umma_commit(&empty[s]);
+    }
+    umma_commit(done);
+  }
+  __syncwarp();
+  // all lanes leave together, before the warp-wide loads; a wait that ran out has recorded its error
+  __all_sync(0xffffffffu, mbar_wait(done, 0, a.err, kErrTimeoutTmemFull, abort_flag));
+  tc_fence_after();
+  __syncthreads();   // every warp is past the wait: no copy or product uses the ring
+  float* logits = reinterpret_cast<float*>(smem);   // [NB][LD]
+#pragma unroll 1
+  for (int b = 0; b < NB; b += 32) {
+    const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16) + b;
+    float v[32];
+    load32(at, v);
+#pragma unroll 1
+    for (int p = 1; p < parts; ++p) {
+      float o[32];
+      load32(at + p * NB, o);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += o[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) logits[(b + j) * C::LD + tid] = v[j];
+  }
+  __syncthreads();
+  const float* mine = logits + m * C::LD;
+  const int nvalid = min(128, a.cols - lo);
+  float mx = -INFINITY;
+#pragma unroll 8
+  for (int j = first; j < nvalid; j += kPer) mx = fmaxf(mx, mine[j]);
+#pragma unroll
+  for (int o = 1; o < kPer; o *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  mx *= a.c;
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float t = 0.f;
+#pragma unroll 8
+  for (int j = first; j < nvalid; j += kPer) t += ex2_approx(fmaf(mine[j], a.c, -ref));
+#pragma unroll
+  for (int o = 1; o < kPer; o *= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (live) {
+    if (first == 0) a.part[(long long)blockIdx.x * a.N + m] = make_float2(mx, t);
+    if (a.start == nullptr) {
+      if (first == 0 && n >= lo && n < lo + 128) a.z[m] = mine[n - lo];
+    } else {
+      for (int e = entry + first; e < end; e += kPer) a.z[(long long)m * a.K + e] = mine[a.ids[(long long)n * a.K + e] - lo];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 256);
+}
+
 // ---------------------------------------------------------------- host
 static PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -992,6 +1148,27 @@ static int launch(const CUtensorMap (&t)[6], const HeadGemm& a, int tiles, int n
 
 using namespace pcb;
 using namespace pcb::head;
+
+template <int NB>
+static int launch_score(HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all, const void* w,
+                        long long ldw, cudaStream_t s) {
+  CUtensorMap tw, ta, tx;
+  if (!map2(&tw, w, a.D, a.cols, ldw, 128) || !map2(&ta, x, a.D, a.N, ldx, NB)) return -5;
+  a.dense = x_all != nullptr;
+  if (!a.dense) tx = ta;
+  else if (!map2(&tx, x_all, a.D, a.N, ldx_all, NB)) return -5;
+  static SmemLimit limit;
+  if (!limit.raise(score_kernel<NB>, Score<NB>::SMEM)) return -3;
+  return pdl_launch(score_kernel<NB>, dim3((a.cols + 127) / 128), dim3(kScoreThreads), Score<NB>::SMEM, s, tw, ta, tx, a) == cudaSuccess ? 0 : -3;
+}
+
+int pcb_head_score(HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all, const void* w, long long ldw,
+                   cudaStream_t s) {
+  if (a.N < 1 || a.N > kScoreRows || a.D < 1 || a.cols < 1) return -1;
+  return a.N <= 32   ? launch_score<32>(a, x, ldx, x_all, ldx_all, w, ldw, s)
+         : a.N <= 64 ? launch_score<64>(a, x, ldx, x_all, ldx_all, w, ldw, s)
+                     : launch_score<128>(a, x, ldx, x_all, ldx_all, w, ldw, s);
+}
 
 bool pcb_head_whole(int N, int V, int D) { return V <= kWholeColumns && !in_halves(N, D); }
 

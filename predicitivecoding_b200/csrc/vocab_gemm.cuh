@@ -12,6 +12,9 @@ namespace pcb {
 // matrix instructions over a tile that reading the weights bounds.
 constexpr int kTwoTermRows = 256;
 
+// Up to this many rows, a loss without gradient is made by a product with the vocabulary as its rows.
+constexpr int kScoreRows = 128;
+
 // Raises a kernel's limit of dynamic shared memory, once on each device.
 struct SmemLimit {
   std::atomic<unsigned long long> done{0};
@@ -155,3 +158,6 @@ int pcb_head_gemm(int mode, pcb::HeadGemm a, const void* x, long long ldx, const
                   const void* w, long long ldw, void* g, int num_sms, cudaStream_t s);
 // whether HEAD_WHOLE takes these sizes
 bool pcb_head_whole(int N, int V, int D);
+// STAT of up to kScoreRows rows; operands as in pcb_head_gemm
+int pcb_head_score(pcb::HeadGemm a, const void* x, long long ldx, const void* x_all, long long ldx_all, const void* w,
+                   long long ldw, cudaStream_t s);

@@ -314,6 +314,34 @@ def test_vocabularies_taken_whole(N, V, K):
     assert state.status() == 0
 
 
+@pytest.mark.parametrize("N", [5, 17, 32, 33])
+@pytest.mark.parametrize("V,D", [(1, 8), (127, 64), (128, 72), (129, 33), (1000, 448), (4099, 520), (300, 2112)])
+@pytest.mark.parametrize("K", [0, 3, 70])
+def test_scoring_a_few_rows(N, V, D, K):
+    """The loss of a few rows without its gradient: one to more k-blocks than a ring holds, fewer k-blocks than partial
+    sums, columns that end inside a block, rows not counted, in place and from rows apart."""
+    x, w, own, g = head(N, V, D, N + V + D + K)
+    K = min(K, V)
+    if K:
+        ids, t = teacher(N, V, K, own, g, torch.float32)
+        q, live = targets64(V, ids=ids, t=t, T=0.7)
+        T, fwd = 0.7, lambda x, **k: vocab.distill_fwd(x, w, ids, t, 0.7, **k)
+    else:
+        own[1::5] = -1
+        q, live = targets64(V, tgt=own)
+        T, fwd = 1.0, lambda x, **k: vocab.ce_fwd(x, w, own, **k)
+    x[~live] = float("nan")
+    apart = torch.full((N, D + 24), float("nan"), device=DEV).bfloat16()
+    apart[:, 8:8 + D] = x
+    for v in (x, apart[:, 8:8 + D]):
+        check_head(v, w, q, live, T, lambda r: fwd(v, reduction=r), "none")
+    rows, state = fwd(x, reduction="none")
+    mean, alone = fwd(x, gradient=False)
+    assert state.status() == 0 and alone.status() == 0
+    assert abs(float(mean) - float(rows.double().sum()) / max(int(live.sum()), 1)) <= 2.0 ** -22 * float(rows.abs().max())
+    assert torch.equal(rows, fwd(x, reduction="none")[0])
+
+
 def test_a_whole_vocabulary_with_infinities():
     """Logits of -inf and +inf in one row reach that row's loss and gradient, and no other row's."""
     x, w, tgt, g = head(300, 300, 64, 3)
