@@ -454,6 +454,14 @@ PCB_DEVICE bool bar_and(int id, int threads, bool p) {
   return r != 0;
 }
 
+// The accumulator of this warp is free again, at the leader's barrier.  Relaxed: what the leader waits for is that the loads
+// from TMEM are complete, which tcgen05.wait::ld and the fence before this see to; a release at cluster scope would also wait
+// for this thread's own loads and stores in global memory, 1500 cycles in the other CTA at every tile (epilogues of
+// 128 columns of statistics 3300 cycles in the leader, 4800 in the other).
+PCB_DEVICE void arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // ---------------------------------------------------------------- WHOLE's epilogue
 // Two threads share a row: each owns 128 columns of every tile.  The first pass makes their softmax statistics, which
 // the two exchange; the second the row's entries of g and, where it meets a target, the loss.  Both go through 32 columns
@@ -594,7 +602,7 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(tempty_leader[acc]);
+      if (lane == 0) arrive_leader(tempty_leader[acc]);
     }
     if (half) losses[mine] = l;
     bar_sync(1 + q, 64);
@@ -924,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         if (leader) mbar_arrive(&tempty[acc]);
-        else mbar_arrive_remote(acc ? tempty_leader1 : tempty_leader0);
+        else arrive_leader(acc ? tempty_leader1 : tempty_leader0);
       }
       if (!HALVES) acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
