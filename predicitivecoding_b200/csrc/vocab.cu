@@ -559,12 +559,10 @@ __global__ void __launch_bounds__(32 * kLossParts)
     norm[j] = make_float2(ref, 1.f / tot);
   }
   if (scalars == nullptr) return;
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(&count[1], 1) == (int)gridDim.x - 1;
+  if (threadIdx.x == 0) last = arrive_last(&count[1], (int)gridDim.x);
   __syncthreads();
   if (!last) return;
-  __threadfence();
   add_losses<32 * kLossParts>(loss, N, rows, mean, scalars, sums, threadIdx.x, [] { __syncthreads(); });
 }
 

@@ -612,11 +612,7 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
   if (lane == 0) bulk_group_wait_all();   // every TMA store has landed
   if (a.scalars == nullptr) return;
   bar_sync(5, kEpi);
-  if (tid == 0) {   // one fence for what all of these threads wrote before the barrier, and will read after the next
-    int before;
-    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.done) : "memory");
-    *last = before == (int)gridDim.x - 1;
-  }
+  if (tid == 0) *last = arrive_last(a.done, (int)gridDim.x);
   bar_sync(5, kEpi);
   if (!*last) return;
   add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.scalars, sums, tid, [] { bar_sync(5, kEpi); });

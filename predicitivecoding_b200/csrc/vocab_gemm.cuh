@@ -128,6 +128,14 @@ __device__ inline void plan_splits(const HeadGemm& a, int rows, int pairs, int* 
   }
 }
 
+// Whether this block is the last of `blocks` to come here, called by one thread between two barriers of the block: its
+// release covers what all of the block's threads wrote before the first, its acquire what they read after the second.
+__device__ inline bool arrive_last(int* done, int blocks) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(done) : "memory");
+  return before == blocks - 1;
+}
+
 // The last step of a loss: the rows' losses added up by THREADS threads in a fixed order and in 64 bits.  scalars[0] = their
 // sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).  `sync` joins the threads.
 template <int THREADS, typename F>
