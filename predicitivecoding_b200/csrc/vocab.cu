@@ -9,6 +9,7 @@
 // sum) and picks the logits at the targets; the backward makes the logits again, a piece of the vocabulary at a
 // time, and turns them into bf16 p - q, which two more products read: dw of the piece is finished there, dx is
 // accumulated over the pieces in fp32.  8 N V D operations instead of 6, for N * piece * 2 bytes of workspace.
+// (A vocabulary of up to 512 columns is taken whole where a gradient follows: its loss and p - q come of one product.)
 // Rows without a target (masked prompts, padding) are taken out first: the counted rows are packed in order,
 // the products run over their number, known on the device only, and what stands in the other rows (NaN too) is
 // never read.  When all rows are counted the products read x itself.

@@ -8,7 +8,7 @@
 //   (the loss of a few rows without gradient has a kernel of its own, below)
 //   WHOLE        the same of a vocabulary of up to two tiles, whose logits stay in TMEM until the row's softmax is known:
 //                a second pass over them makes the row's loss and its gradient.  One launch in place of three and 2 of
-//                the 8 N V D operations less: loss and gradients of 2048 rows of 256 against 256 take 28.8 us,
+//                the 8 N V D operations less: loss and gradients of 2048 rows of 256 against 256 take 28.2 us,
 //                37.1 the other way; of 131072 rows of 768 against 512, 527 and 617.  A loss alone is
 //                quicker without g (2048 rows of 768 against 512: 18 us, 26), so this is for losses with a backward
 //   BWD          dw = g^T x (rows = vocabulary, K = counted rows) and dx = g w (rows = counted rows, K = vocabulary)
