@@ -30,6 +30,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ext
 
@@ -54,7 +55,7 @@ def embed_bwd(tok: torch.Tensor, dx: torch.Tensor, vocab: int, scale: float = 1.
 
 
 class Embed(torch.autograd.Function):
-    """Autograd form of the lookup; the gradient has w's type."""
+    """Autograd form of the lookup; the gradient has w's type, and none of its own (differentiating it raises)."""
 
     @staticmethod
     def forward(ctx, tok, w, scale, dtype):
@@ -63,6 +64,7 @@ class Embed(torch.autograd.Function):
         return embed_fwd(tok, w, scale, dtype=dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx):
         tok, = ctx.saved_tensors
         return None, embed_bwd(tok, dx, ctx.w[0], ctx.scale, dtype=ctx.w[1]), None, None
@@ -104,6 +106,8 @@ def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optio
 
 
 class _HeadLoss(torch.autograd.Function):
+    """Autograd form of a mean or summed loss; its gradients have none of their own (differentiating them raises)."""
+
     @staticmethod
     def forward(ctx, x, w, kind, args, reduction):
         loss, ctx.state = (ce_fwd if kind == "ce" else distill_fwd)(x, w, *args, reduction)
@@ -111,6 +115,7 @@ class _HeadLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         ctx.saved_tensors
         dx, dw = head_bwd(ctx.state, g.float().contiguous(), need_dx=ctx.needs_input_grad[0],
