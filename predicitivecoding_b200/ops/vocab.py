@@ -105,6 +105,18 @@ def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optio
     return ext().vocab_head_bwd(state, gout, None, dx, dw, need_dx, need_dw, accumulate, piece)
 
 
+class _Final(torch.autograd.Function):
+    """A gradient made by kernels, as a function of what it depends on that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("the gradients of the vocabulary head's losses cannot be differentiated")
+
+
 class _HeadLoss(torch.autograd.Function):
     """Autograd form of a mean or summed loss; its gradients have none of their own (differentiating them raises)."""
 
@@ -115,12 +127,15 @@ class _HeadLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        ctx.saved_tensors
-        dx, dw = head_bwd(ctx.state, g.float().contiguous(), need_dx=ctx.needs_input_grad[0],
-                          need_dw=ctx.needs_input_grad[1])
-        return dx, dw, None, None, None
+        sources = ctx.saved_tensors
+        with torch.no_grad():
+            grads = head_bwd(ctx.state, g.float().contiguous(), need_dx=ctx.needs_input_grad[0],
+                             need_dw=ctx.needs_input_grad[1])
+        # once_differentiable would not do: it lets a gradient by way of a constant g pass, which yet depends on x and w
+        if torch.is_grad_enabled():
+            grads = tuple(d if d is None else _Final.apply(d, *sources, g) for d in grads)
+        return *grads, None, None, None
 
 
 def _differentiated(x: torch.Tensor, w: torch.Tensor) -> bool:

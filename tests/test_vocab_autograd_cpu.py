@@ -56,5 +56,5 @@ def test_a_gradient_of_a_gradient_is_refused(plain, form):
     first, = torch.autograd.grad(f(), w)
     graph, = torch.autograd.grad(f(), w, create_graph=True)
     assert torch.equal(first, graph)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
+    with pytest.raises(RuntimeError, match="differentia"):
         ((graph ** 2).sum() + (w ** 2).sum()).backward()
