@@ -138,24 +138,41 @@ class _HeadLoss(torch.autograd.Function):
         return *grads, None, None, None
 
 
+class _RowLosses(torch.autograd.Function):
+    """Per-row losses.  Their gradient does not exist; asking for it raises, where a detached result would train nothing."""
+
+    @staticmethod
+    def forward(ctx, x, w, kind, args):
+        return (ce_fwd if kind == "ce" else distill_fwd)(x, w, *args, "none", gradient=False)[0]
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("losses with reduction 'none' have no gradient: take the mean or the sum")
+
+
 def _differentiated(x: torch.Tensor, w: torch.Tensor) -> bool:
     return torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
 
 
+def _head_loss(kind: str, x: torch.Tensor, w: torch.Tensor, args: tuple, reduction: str) -> torch.Tensor:
+    if not _differentiated(x, w):
+        return (ce_fwd if kind == "ce" else distill_fwd)(x, w, *args, reduction, gradient=False)[0]
+    if reduction == "none":
+        return _RowLosses.apply(x, w, kind, args)
+    return _HeadLoss.apply(x, w, kind, args, reduction)
+
+
 def cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -1,
                   reduction: str = "mean") -> torch.Tensor:
-    """Differentiable :func:`ce_fwd` (mean or sum; ``none`` has no gradient)."""
-    if reduction == "none" or not _differentiated(x, w):
-        return ce_fwd(x, w, targets, ignore_index, reduction, gradient=False)[0]
-    return _HeadLoss.apply(x, w, "ce", (targets, ignore_index), reduction)
+    """Differentiable :func:`ce_fwd` (mean or sum; a backward through ``none`` raises)."""
+    return _head_loss("ce", x, w, (targets, ignore_index), reduction)
 
 
 def distill(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor, temperature: float = 1.0,
             reduction: str = "mean") -> torch.Tensor:
-    """Differentiable :func:`distill_fwd` by x and w (mean or sum); the teacher's logits get no gradient."""
-    if reduction == "none" or not _differentiated(x, w):
-        return distill_fwd(x, w, ids, logits, temperature, reduction, gradient=False)[0]
-    return _HeadLoss.apply(x, w, "distill", (ids, logits, temperature), reduction)
+    """Differentiable :func:`distill_fwd` by x and w (mean or sum; a backward through ``none`` raises); the teacher's
+    logits get no gradient."""
+    return _head_loss("distill", x, w, (ids, logits, temperature), reduction)
 
 
 # --------------------------------------------------------------------------- plain statements

@@ -58,3 +58,19 @@ def test_a_gradient_of_a_gradient_is_refused(plain, form):
     assert torch.equal(first, graph)
     with pytest.raises(RuntimeError, match="differentia"):
         ((graph ** 2).sum() + (w ** 2).sum()).backward()
+
+
+@pytest.mark.parametrize("form", ["cross_entropy", "distill"])
+def test_a_gradient_of_row_losses_is_refused(plain, form):
+    """Per-row losses have no gradient: weighted rows in a sum with another loss raise instead of training nothing.
+    Without a gradient wanted they are plain values."""
+    x, w, tgt, ids, logits = operands()
+    f = ((lambda: vocab.cross_entropy(x, w, tgt, reduction="none")) if form == "cross_entropy" else
+         (lambda: vocab.distill(x, w, ids, logits, 2.0, "none")))
+    rows = f()
+    weights = torch.arange(6.0)
+    with pytest.raises(RuntimeError, match="none"):
+        ((rows * weights).sum() + (x ** 2).sum()).backward()
+    with torch.no_grad():
+        alone = f()
+    assert not alone.requires_grad and torch.equal(alone, rows.detach())
