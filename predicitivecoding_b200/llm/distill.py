@@ -81,7 +81,7 @@ class TopLogitDistiller:
 
     loss = alpha * T^2 KL(q || p_T) + (1 - alpha) * cross entropy, q the softmax of the teacher's ``top_k`` logits at
     temperature T, p_T the student's softmax at T over its whole vocabulary.  Both means run over the positions whose
-    target is not ``ignore_index``.  ``embed_scale`` multiplies the student's embedding rows.
+    target is in the vocabulary and not ``ignore_index``.  ``embed_scale`` multiplies the student's embedding rows.
     """
 
     def __init__(self, student: DecoderLM, top_k: int = 32, temperature: float = 2.0, alpha: float = 0.5,
@@ -106,7 +106,8 @@ class TopLogitDistiller:
         m, on_gpu = self.student, tokens.is_cuda
         embed = vocab.embedding if on_gpu else vocab.reference_embedding
         x = m.hidden(tokens, training, embedded=embed(tokens, m.wemb, self.embed_scale))
-        ids = torch.where((targets != self.ignore_index)[..., None], ids, torch.full_like(ids, -1))
+        live = (targets >= 0) & (targets < m.cfg.vocab) & (targets != self.ignore_index)   # as the cross entropy counts
+        ids = torch.where(live[..., None], ids, torch.full_like(ids, -1))
         if on_gpu:
             x, w = x.bfloat16(), m.wout.t().bfloat16().contiguous()
             ce, kd = vocab.cross_entropy, vocab.distill
