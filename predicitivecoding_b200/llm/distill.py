@@ -18,7 +18,7 @@ from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 
-from ..models.decoder_lm import DecoderLM
+from ..models.decoder_lm import DecoderLM, mtp_targets
 from ..ops import vocab
 from ..optim.adam import Adam, clip_global_norm
 from .generation import greedy
@@ -79,9 +79,11 @@ def on_policy_round(model, tok, prompts: Sequence[str], teacher_correct: Callabl
 class TopLogitDistiller:
     """Trains ``student`` on a teacher's top logits.
 
-    loss = alpha * T^2 KL(q || p_T) + (1 - alpha) * cross entropy, q the softmax of the teacher's ``top_k`` logits at
-    temperature T, p_T the student's softmax at T over its whole vocabulary.  Both means run over the positions whose
-    target is in the vocabulary and not ``ignore_index``.  ``embed_scale`` multiplies the student's embedding rows.
+    loss = alpha * T^2 KL(q || p_T) + (1 - alpha) * cross entropy + the student's auxiliary terms, q the softmax of the
+    teacher's ``top_k`` logits at temperature T, p_T the student's softmax at T over its whole vocabulary.  Both means run
+    over the positions whose target is in the vocabulary and not ``ignore_index``.  The auxiliary terms (multi-token
+    head, experts' balance) are those of ``DecoderLM.loss``, which this loss is at alpha 0.  ``embed_scale`` multiplies
+    the student's embedding rows.
     """
 
     def __init__(self, student: DecoderLM, top_k: int = 32, temperature: float = 2.0, alpha: float = 0.5,
@@ -103,21 +105,29 @@ class TopLogitDistiller:
 
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor,
              training: bool = False) -> torch.Tensor:
-        m, on_gpu = self.student, tokens.is_cuda
+        m, c, on_gpu = self.student, self.student.cfg, tokens.is_cuda
         embed = vocab.embedding if on_gpu else vocab.reference_embedding
-        x = m.hidden(tokens, training, embedded=embed(tokens, m.wemb, self.embed_scale))
-        live = (targets >= 0) & (targets < m.cfg.vocab) & (targets != self.ignore_index)   # as the cross entropy counts
+        balance = m.balance_terms()
+        x = m.hidden(tokens, training, aux_losses=balance, embedded=embed(tokens, m.wemb, self.embed_scale))
+        live = (targets >= 0) & (targets < c.vocab) & (targets != self.ignore_index)   # as the cross entropy counts
         ids = torch.where(live[..., None], ids, torch.full_like(ids, -1))
         if on_gpu:
-            x, w = x.bfloat16(), m.wout.t().bfloat16().contiguous()
+            x = x.bfloat16()
+            head = lambda w: w.t().bfloat16().contiguous()
             ce, kd = vocab.cross_entropy, vocab.distill
         else:
-            w, ce, kd = m.wout.t(), vocab.reference_cross_entropy, vocab.reference_distill
+            head, ce, kd = torch.t, vocab.reference_cross_entropy, vocab.reference_distill
+        w = head(m.wout)
         total = x.new_zeros((), dtype=torch.float32)
         if self.alpha < 1.0:
             total = total + (1.0 - self.alpha) * ce(x, w, targets, self.ignore_index)
         if self.alpha > 0.0:
             total = total + self.alpha * kd(x, w, ids, logits, self.temperature)
+        if m.wout_mtp is not None:
+            ahead = mtp_targets(targets, c.mtp_horizon, self.ignore_index)
+            total = total + c.mtp_weight * ce(x, head(m.wout_mtp), ahead, self.ignore_index)
+        if balance:
+            total = total + c.moe_balance_weight * torch.stack(balance).sum()
         return total
 
     def step(self, tokens: torch.Tensor, targets: torch.Tensor, ids: torch.Tensor, logits: torch.Tensor,

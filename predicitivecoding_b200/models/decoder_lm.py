@@ -389,11 +389,15 @@ class DecoderLM(nn.Module):
         """Logits [.., S, V]."""
         return self.hidden(tokens, training, probe) @ self.wout
 
+    def balance_terms(self) -> Optional[list]:
+        """A list for the experts' balance terms of one forward pass; None where the loss has none."""
+        return [] if self.cfg.num_experts > 0 and self.cfg.moe_balance_weight > 0 else None
+
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ignore_index: int = -1,
              training: bool = False) -> torch.Tensor:
         """Masked next-token CE (+ MTP aux head + MoE balance), DecoderLM.cs:320-350."""
         c = self.cfg
-        aux = [] if c.num_experts > 0 and c.moe_balance_weight > 0 else None
+        aux = self.balance_terms()
         main, mtp = self.heads(tokens, training, None, aux)
         loss = cross_entropy_masked(main, targets, ignore_index)
         if mtp is not None:

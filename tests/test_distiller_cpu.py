@@ -33,3 +33,39 @@ def test_both_terms_run_over_the_same_rows(alpha, pad):
     ignored[:, :3] = -1
     got, want = d.loss(tokens, padded, ids, logits), d.loss(tokens, ignored, ids, logits)
     assert float(got.detach()) == float(want.detach())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(mtp_weight=0.3), dict(mtp_weight=0.5, mtp_horizon=3), dict(num_experts=3, moe_top_k=2, moe_balance_weight=0.1),
+    dict(mtp_weight=0.3, num_experts=2, moe_balance_weight=0.2), {},
+])
+def test_without_distillation_the_loss_is_the_students_own(kw):
+    """alpha 0: value and gradients of DecoderLM.loss, with its multi-token head and its experts' balance.  fp32 sums of
+    some hundred terms in another order: 2^-24 sqrt(300) of what they add up, 1e-5 of the largest gradient."""
+    teacher, student = model(1, 24), model(2, **kw)
+    tokens, targets = batch()
+    targets[:, :3] = -1
+    d = TopLogitDistiller(student, top_k=5, alpha=0.0)
+    params = list(student.parameters())
+    grads = lambda loss: torch.autograd.grad(loss, params, allow_unused=True)
+    own, got = student.loss(tokens, targets), d.loss(tokens, targets, *d.ask(teacher, tokens))
+    assert math.isclose(float(got.detach()), float(own.detach()), rel_tol=1e-5)
+    top = max(float(g.abs().max()) for g in grads(student.loss(tokens, targets)) if g is not None)
+    for a, b in zip(grads(got), grads(own)):
+        assert (a is None) == (b is None)
+        assert a is None or float((a - b).abs().max()) <= 1e-5 * top
+
+
+def test_the_students_auxiliary_terms_stand_beside_the_distillation():
+    teacher, student = model(1, 24), model(2, mtp_weight=0.3, num_experts=2, moe_balance_weight=0.2)
+    tokens, targets = batch()
+    top = TopLogitDistiller(student, top_k=5).ask(teacher, tokens)
+    at = lambda alpha: float(TopLogitDistiller(student, top_k=5, alpha=alpha).loss(tokens, targets, *top).detach())
+    assert math.isclose(at(0.25), 0.75 * at(0.0) + 0.25 * at(1.0), rel_tol=1e-5)
+    x = student.hidden(tokens)
+    logp = torch.log_softmax(x @ student.wout / 2.0, -1).gather(-1, top[0].long())
+    q = torch.softmax(top[1] / 2.0, -1)
+    kd = 4.0 * (q * (q.log() - logp)).sum(-1).mean()
+    main = torch.nn.functional.cross_entropy((x @ student.wout).flatten(0, 1), targets.flatten())
+    extra = student.loss(tokens, targets) - main      # the auxiliary terms alone
+    assert math.isclose(at(1.0), float((kd + extra).detach()), rel_tol=1e-4)
