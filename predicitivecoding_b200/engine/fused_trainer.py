@@ -44,6 +44,7 @@ def supports(cfg: DecoderLmConfig, seq: Optional[int] = None) -> bool:
     moe_ok = cfg.num_experts == 0 or moe_ops.supported(cfg.dim, cfg.ff_dim, cfg.num_experts, cfg.moe_top_k)
     return (cfg.use_rms_norm and cfg.use_rope and cfg.block_pattern is None and moe_ok
             and cfg.num_loops == 1 and cfg.mtp_weight == 0 and not cfg.use_plan and cfg.dropout == 0
+            and cfg.embed_scale == 1.0
             and cfg.head_dim in (64, 128) and s % 128 == 0 and cfg.dim % 64 == 0 and cfg.ff_dim % 64 == 0)
 
 
@@ -296,6 +297,8 @@ class FusedDecoderTrainer:
     def _model_to_flat(self, model: DecoderLM) -> torch.Tensor:
         """DecoderLM tensors (reference [in,out] layout) -> flat fp32 arena (cpu)."""
         cfg = self.cfg
+        if model.cfg.embed_scale != cfg.embed_scale:
+            raise ValueError(f"the model scales its embedding by {model.cfg.embed_scale}, the trainer by {cfg.embed_scale}")
         full = torch.zeros(self.arena.total, dtype=torch.float32)
         V = self.arena.views(full)
         V["wemb"][:self.Vr].copy_(model.wemb.detach().float().cpu())

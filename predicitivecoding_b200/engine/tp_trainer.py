@@ -52,6 +52,7 @@ def _interleave(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 def tp_supports(cfg: DecoderLmConfig, batch: int, seq: int, world: int) -> bool:
     return (cfg.use_rms_norm and cfg.use_rope and cfg.ffn == "swiglu" and cfg.num_experts == 0
             and cfg.block_pattern is None and cfg.num_loops == 1 and not cfg.use_plan and cfg.mtp_weight == 0
+            and cfg.embed_scale == 1.0
             and cfg.head_dim in (64, 128) and cfg.num_heads % world == 0 and seq % 128 == 0
             and (batch * seq) % (256 * world) == 0 and cfg.dim % 8 == 0)
 
@@ -179,6 +180,8 @@ class TensorParallelTrainer:
     def _shard_full(self, model: DecoderLM):
         """Full-model tensors in this rank's shard layout (cpu fp32)."""
         cfg, t, Dl, Fl = self.cfg, self.t, self.Dl, self.Fl
+        if model.cfg.embed_scale != cfg.embed_scale:
+            raise ValueError(f"the model scales its embedding by {model.cfg.embed_scale}, the trainer by {cfg.embed_scale}")
         F_ = cfg.ff_dim
         f0, f1 = t * (-(-F_ // self.T)), min(F_, (t + 1) * (-(-F_ // self.T)))
         out = {"wemb": model.wemb.detach().float().cpu(), "wout": model.wout.detach().T.float().cpu(),

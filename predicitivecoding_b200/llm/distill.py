@@ -83,19 +83,28 @@ class TopLogitDistiller:
     teacher's ``top_k`` logits at temperature T, p_T the student's softmax at T over its whole vocabulary.  Both means run
     over the positions whose target is in the vocabulary and not ``ignore_index``.  The auxiliary terms (multi-token
     head, experts' balance) are those of ``DecoderLM.loss``, which this loss is at alpha 0.  ``embed_scale`` multiplies
-    the student's embedding rows.
+    the student's embedding rows; given here it becomes the student's (``DecoderLmConfig.embed_scale``), so that the
+    network which is trained is the one that is evaluated, served and saved.
     """
 
     def __init__(self, student: DecoderLM, top_k: int = 32, temperature: float = 2.0, alpha: float = 0.5,
-                 embed_scale: float = 1.0, ignore_index: int = -1):
+                 embed_scale: Optional[float] = None, ignore_index: int = -1):
         if not 1 <= top_k <= min(vocab.MAX_TOP_K, student.cfg.vocab):
             raise ValueError(f"top_k must be between 1 and {min(vocab.MAX_TOP_K, student.cfg.vocab)}")
         if temperature <= 0:
             raise ValueError("temperature must be positive")
         if not 0.0 <= alpha <= 1.0:
             raise ValueError("alpha must be between 0 and 1")
+        if embed_scale is not None:
+            cfg = student.cfg.with_(embed_scale=float(embed_scale))
+            cfg.validate()
+            student.cfg = cfg
         self.student, self.top_k, self.temperature = student, top_k, float(temperature)
-        self.alpha, self.embed_scale, self.ignore_index = alpha, embed_scale, ignore_index
+        self.alpha, self.ignore_index = alpha, ignore_index
+
+    @property
+    def embed_scale(self) -> float:
+        return self.student.cfg.embed_scale
 
     @torch.no_grad()
     def ask(self, teacher: DecoderLM, tokens: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -108,7 +117,7 @@ class TopLogitDistiller:
         m, c, on_gpu = self.student, self.student.cfg, tokens.is_cuda
         embed = vocab.embedding if on_gpu else vocab.reference_embedding
         balance = m.balance_terms()
-        x = m.hidden(tokens, training, aux_losses=balance, embedded=embed(tokens, m.wemb, self.embed_scale))
+        x = m.hidden(tokens, training, aux_losses=balance, embedded=embed(tokens, m.wemb, c.embed_scale))
         live = (targets >= 0) & (targets < c.vocab) & (targets != self.ignore_index)   # as the cross entropy counts
         ids = torch.where(live[..., None], ids, torch.full_like(ids, -1))
         if on_gpu:

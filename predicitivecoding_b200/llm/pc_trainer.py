@@ -38,6 +38,8 @@ class PcDecoderTrainer:
         c = model.cfg
         if c.num_loops != 1 or c.num_experts != 0 or c.mtp_weight != 0 or c.use_plan or c.block_pattern is not None:
             raise NotImplementedError("PcDecoderTrainer needs a plain dense preset (no loops/MoE/MTP/plan).")
+        if c.embed_scale != 1.0:
+            raise NotImplementedError("PcDecoderTrainer looks embedding rows up unscaled.")
         if not c.use_rope or not c.use_rms_norm:
             raise NotImplementedError("PcDecoderTrainer assumes RMSNorm + RoPE.")
         self.m = model

@@ -68,7 +68,7 @@ class InferenceModel:
         cast = lambda t: None if t is None else t.detach().to(self.device, self.dtype).contiguous()
         self._tc = self.device.type == "cuda" and self.dtype == torch.bfloat16 and ops.available()
         # the plan vector conditions every position identically: fold it into the embedding rows
-        self.wemb = cast(model.wemb + model.plan if cfg.use_plan else model.wemb)
+        self.wemb = cast(model.embedding_table() + model.plan if cfg.use_plan else model.embedding_table())
         self.wout = cast(model.wout)
         self.lnf = (cast(model.lnf_g), cast(model.lnf_b))
         self.blocks = []
@@ -355,5 +355,5 @@ def export_gpt(model: DecoderLM):
     plan = nxt(1, D, "plan").reshape(-1) if c.use_plan else torch.zeros(D)
     if cur[0] != len(ps):
         raise ValueError(f"exporter left {len(ps) - cur[0]} parameter(s) unconsumed (layout drift)")
-    gpt.embedding.copy_(wemb + plan)
+    gpt.embedding.copy_(wemb * c.embed_scale + plan)
     return gpt

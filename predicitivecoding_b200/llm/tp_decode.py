@@ -108,7 +108,7 @@ class TensorParallelDecoder:
         hs = slice(t * Dl, (t + 1) * Dl)
         fs = slice(t * Fl, (t + 1) * Fl)
         with torch.no_grad():
-            self._shard("wemb", model.wemb)
+            self._shard("wemb", model.embedding_table())
             self._shard("lnf", model.lnf_g)
             self._shard("wout", model.wout[:, t * Vl:(t + 1) * Vl])
             for l, blk in enumerate(model.blocks):

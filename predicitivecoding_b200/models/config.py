@@ -3,9 +3,10 @@
 Reference: PredictiveCoding.LLM/Autograd/DecoderLM.cs:31-130 (``DecoderLmConfig``).
 Field names follow the reference's PascalCase in the JSON form
 (:meth:`DecoderLmConfig.to_json` / :meth:`from_json`) so configs written by one
-side load in the other.  Two fields are extensions the reference never trained:
+side load in the other.  Three fields are extensions the reference never trained:
 ``ffn`` ("gelu" = the reference's dense GELU FFN with biases, "swiglu" = gated
-SiLU FFN without biases, used by the GPT-2-small / 1.3B configs) and ``tie_io``
+SiLU FFN without biases, used by the GPT-2-small / 1.3B configs), ``embed_scale``
+(a factor of the looked-up embedding rows) and ``tie_io``
 (kept False: the reference unties the embedding and the output head).
 """
 from __future__ import annotations
@@ -21,7 +22,7 @@ _PASCAL = {
     "loop_exit_tau": "LoopExitTau", "mtp_weight": "MtpWeight", "mtp_horizon": "MtpHorizon",
     "block_pattern": "BlockPattern", "num_experts": "NumExperts", "moe_top_k": "MoeTopK",
     "moe_balance_weight": "MoeBalanceWeight", "use_plan": "UsePlan", "use_rms_norm": "UseRmsNorm",
-    "use_rope": "UseRope", "ffn": "Ffn",
+    "use_rope": "UseRope", "ffn": "Ffn", "embed_scale": "EmbedScale",
 }
 
 
@@ -47,6 +48,7 @@ class DecoderLmConfig:
     use_rms_norm: bool = False
     use_rope: bool = False
     ffn: str = "gelu"
+    embed_scale: float = 1.0
 
     @property
     def head_dim(self) -> int:
@@ -84,6 +86,8 @@ class DecoderLmConfig:
             raise ValueError("UseRmsNorm/UseRope are attention-only (BlockPattern must be null).")
         if self.ffn not in ("gelu", "swiglu"):
             raise ValueError(f"ffn must be 'gelu' or 'swiglu', got {self.ffn!r}.")
+        if not 0.0 < self.embed_scale < float("inf"):
+            raise ValueError(f"embed_scale must be positive and finite, got {self.embed_scale}.")
 
     # ---------------------------------------------------------------- presets
     @staticmethod
@@ -128,8 +132,8 @@ class DecoderLmConfig:
     def to_json(self) -> str:
         d = {}
         for k, v in dataclasses.asdict(self).items():
-            if k == "ffn" and v == "gelu":
-                continue  # the reference has no such field; omit the default
+            if (k, v) in (("ffn", "gelu"), ("embed_scale", 1.0)):
+                continue  # the reference has no such fields; omit the defaults
             d[_PASCAL[k]] = v
         return json.dumps(d)
 

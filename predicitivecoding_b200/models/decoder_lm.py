@@ -334,12 +334,16 @@ class DecoderLM(nn.Module):
         attn_blocks = c.block_pattern.count("A") if c.block_pattern else c.num_blocks
         return self.parameter_count - attn_blocks * (c.num_experts - c.moe_top_k) * per_expert
 
+    def embedding_table(self) -> torch.Tensor:
+        """The rows that tokens look up [V, D], the configured scale included."""
+        return self.wemb if self.cfg.embed_scale == 1.0 else self.wemb * self.cfg.embed_scale
+
     # ------------------------------------------------------------ forward
     def hidden(self, tokens: torch.Tensor, training: bool = False, probe=None,
                aux_losses: Optional[list] = None, base_pos: int = 0,
                embedded: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Embedding -> (looped) block stack -> final norm.  tokens: [B, S] or [S].  ``embedded`` [.., S, D] replaces
-        the lookup of the tokens' rows."""
+        the lookup of the tokens' rows, their scale included."""
         c = self.cfg
         squeeze = tokens.dim() == 1
         if squeeze:
@@ -349,7 +353,11 @@ class DecoderLM(nn.Module):
         if S > c.max_seq:
             raise ValueError(f"Sequence length {S} exceeds MaxSeq {c.max_seq}.")
         self.forward_tokens += B * S
-        x = self.wemb[tokens] if embedded is None else embedded
+        x = embedded
+        if x is None:
+            x = self.wemb[tokens]
+            if c.embed_scale != 1.0:
+                x = x * c.embed_scale
         dev = x.device
         rope = None
         if c.use_rope:

@@ -69,3 +69,58 @@ def test_the_students_auxiliary_terms_stand_beside_the_distillation():
     main = torch.nn.functional.cross_entropy((x @ student.wout).flatten(0, 1), targets.flatten())
     extra = student.loss(tokens, targets) - main      # the auxiliary terms alone
     assert math.isclose(at(1.0), float((kd + extra).detach()), rel_tol=1e-4)
+
+
+def test_a_scaled_embedding_belongs_to_the_model():
+    """The network that is trained with a scale is the one that is evaluated, generated from, served and saved."""
+    cfg = DecoderLmConfig(dim=16, num_blocks=2, ff_dim=24, **SHAPE)
+    teacher, student = DecoderLM(cfg, seed=1), DecoderLM(cfg, seed=2)
+    tokens, targets = batch()
+    before = student.forward(tokens)
+    d = TopLogitDistiller(student, top_k=5, alpha=0.0, embed_scale=4.0)
+    assert d.embed_scale == 4.0 and teacher.cfg.embed_scale == 1.0 and cfg.embed_scale == 1.0
+    got, own = d.loss(tokens, targets, *d.ask(teacher, tokens)), student.loss(tokens, targets)
+    assert math.isclose(float(got.detach()), float(own.detach()), rel_tol=1e-5)
+    logits = student.forward(tokens)
+    assert not torch.allclose(logits, before, atol=1e-4)
+    # the same network with the scale in its rows
+    folded = DecoderLM(cfg, seed=2)
+    with torch.no_grad():
+        folded.wemb *= 4.0
+    assert torch.allclose(folded.forward(tokens), logits, atol=1e-5)
+    assert torch.equal(student.embedding_table(), folded.wemb)
+    # a second distiller keeps the student's scale
+    assert TopLogitDistiller(student, top_k=5).embed_scale == 4.0
+    # served: with a KV cache, and step by step
+    from predicitivecoding_b200.llm.serving import InferenceModel, export_gpt
+    serve = InferenceModel(student, dtype=torch.float32)
+    served = serve.prefill(tokens, serve.new_cache(tokens.shape[0]))
+    assert torch.allclose(served, logits if served.shape == logits.shape else logits[:, -1], atol=1e-4)
+    assert torch.allclose(export_gpt(student).embedding, folded.wemb.detach(), atol=1e-6)
+
+
+def test_a_scaled_embedding_is_saved_with_the_model(tmp_path):
+    from predicitivecoding_b200.llm.facade import PredictiveLlm
+    from predicitivecoding_b200.llm.tokenizer import ByteTokenizer
+    tok = ByteTokenizer()
+    llm = PredictiveLlm(DecoderLmConfig(dim=16, num_blocks=1, ff_dim=24, **{**SHAPE, "vocab": tok.vocab_size}), tok)
+    TopLogitDistiller(llm.model, top_k=5, embed_scale=3.0)
+    llm.save(str(tmp_path / "m"))
+    again = PredictiveLlm.load(str(tmp_path / "m"))
+    tokens = torch.randint(0, tok.vocab_size, (1, 9), generator=torch.Generator().manual_seed(0))
+    assert again.config.embed_scale == 3.0 and torch.equal(again.model.forward(tokens), llm.model.forward(tokens))
+    assert "EmbedScale" not in DecoderLmConfig(dim=16, num_blocks=1, ff_dim=24, **SHAPE).to_json()
+
+
+def test_trainers_without_a_scaled_lookup_refuse_it():
+    from predicitivecoding_b200.engine.fused_trainer import supports
+    from predicitivecoding_b200.engine.tp_trainer import tp_supports
+    from predicitivecoding_b200.llm.pc_trainer import PcDecoderTrainer
+    cfg = DecoderLmConfig(64, 128, 1, 2, 128, 128, use_rms_norm=True, use_rope=True, ffn="swiglu")
+    assert supports(cfg) and tp_supports(cfg, 2, 128, 1)
+    assert not supports(cfg.with_(embed_scale=2.0)) and not tp_supports(cfg.with_(embed_scale=2.0), 2, 128, 1)
+    with pytest.raises(NotImplementedError):
+        PcDecoderTrainer(model(1, embed_scale=2.0))
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            cfg.with_(embed_scale=bad).validate()
