@@ -382,7 +382,7 @@ at::Tensor flat(const at::Tensor& t) { return t.is_contiguous() ? t : t.contiguo
 
 // What a loss of the vocabulary head keeps for its gradients.
 struct HeadState {
-  at::Tensor saved, scalars, x, w;
+  at::Tensor saved, x, w;
   at::Tensor g;   // gradient of the logits, where the forward made it
   pcb::VocabPlan plan;
   std::vector<int64_t> lead;
@@ -478,10 +478,9 @@ std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x,
     loss = at::empty(st.lead, f32);
     a.loss = loss.data_ptr<float>();
   } else {
-    st.scalars = at::empty({2}, f32);
-    a.scalars = st.scalars.data_ptr<float>();
+    loss = at::empty({}, f32);   // the caller's own: nothing reads it again
+    a.total = loss.data_ptr<float>();
     a.loss = part.data_ptr<float>() + pairs;
-    loss = st.scalars.select(0, 0);
   }
   st.plan = pcb::vocab_plan(a.N, a.V, a.D, 0, st.gradient, num_sms());
   if (st.plan.whole) st.g = at::empty({pcb::vocab_g_rows(a.N) * st.plan.piece}, x.options());
@@ -551,7 +550,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
     return {dx, dw};
   }
   if (!dx && !dw) return {dx, dw};
-  for (const at::Tensor& t : {st.saved, st.scalars, st.x, st.w, st.g}) used_here(t);
+  for (const at::Tensor& t : {st.saved, st.x, st.w, st.g}) used_here(t);
   a.x = st.x.data_ptr();
   a.ldx = rows_apart(st.x);
   a.w = st.w.data_ptr();
@@ -563,7 +562,6 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
   a.distill = st.distill;
   a.temperature = (float)st.temperature;
   a.saved = st.saved.data_ptr();
-  a.scalars = st.scalars.data_ptr<float>();
   a.gout = (float)gout;
   if (gout_dev) a.gout_dev = gout_dev->data_ptr<float>();
   a.mean = st.mean;

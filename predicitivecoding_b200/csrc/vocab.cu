@@ -487,14 +487,14 @@ __global__ void __launch_bounds__(few_threads(NR)) few_rows_kernel(FewRowsArgs a
 // 32 rows a block, a warp a row: the row's (max, sum) pairs become one, its target list its loss.  The pairs
 // lie by row, so they are read with a row per lane and change hands through shared memory; the targets, which wait
 // for nothing, are read in the meantime.  The last block to finish adds the losses up, in a fixed order and in 64
-// bits: scalars[0] = their sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).
+// bits: *total = their sum or mean, *inverse = 1 / counted rows (both 0 when there are none).
 constexpr int kLossParts = 32;
 
 __global__ void __launch_bounds__(32 * kLossParts)
     row_loss_kernel(const float2* __restrict__ part, int granules, const int* __restrict__ row,
                     const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lq,
                     const int* __restrict__ len, int N, int K, float c, float factor, float2* __restrict__ norm,
-                    float* loss, int* count, int mean, float* __restrict__ scalars) {
+                    float* loss, int* count, int mean, float* __restrict__ total, float* __restrict__ inverse) {
   __shared__ float sm[kLossParts][33], ss[kLossParts][33];
   __shared__ double sums[kLossParts];
   __shared__ int last;
@@ -559,12 +559,12 @@ __global__ void __launch_bounds__(32 * kLossParts)
     loss[n] = l * factor;
     norm[j] = make_float2(ref, 1.f / tot);
   }
-  if (scalars == nullptr) return;
+  if (total == nullptr) return;
   __syncthreads();
   if (threadIdx.x == 0) last = arrive_last(&count[1], (int)gridDim.x);
   __syncthreads();
   if (!last) return;
-  add_losses<32 * kLossParts>(loss, N, rows, mean, scalars, sums, threadIdx.x, [] { __syncthreads(); });
+  add_losses<32 * kLossParts>(loss, N, rows, mean, total, inverse, sums, threadIdx.x, [] { __syncthreads(); });
 }
 
 // Gradients from their fp32 slabs: the sum in slab order, times the gradient's factor.  The first N rows are dx's, found
@@ -1384,7 +1384,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
   auto finish = [&](const VocabLayout& l, int pairs) {   // row losses from `pairs` (max, sum) pairs a row
     return pdl_launch(row_loss_kernel, dim3((a.N + 31) / 32), dim3(32 * kLossParts), 0, s, (const float2*)part, pairs,
                       (const int*)row, (const float*)z, (const float*)q, (const float*)lq, (const int*)len, a.N, a.K, c,
-                      factor, norm, a.loss, count, mean, a.scalars) == cudaSuccess ? 0 : -3;
+                      factor, norm, a.loss, count, mean, a.total, (float*)(count + 5)) == cudaSuccess ? 0 : -3;
   };
   HeadGemm g{};
   g.N = a.N;
@@ -1412,7 +1412,8 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
     g.q = q;
     g.loss = a.loss;
     g.factor = factor;
-    g.scalars = a.scalars;
+    g.total = a.total;
+    g.inverse = (float*)(count + 5);
     g.mean = mean;
     g.done = count + 1;
     return pcb_head_gemm(HEAD_WHOLE, g, p.xc, l.ldxc, p.in_place ? a.x : nullptr, a.ldx, a.w, a.ldw, dlogits, num_sms, s);
@@ -1448,7 +1449,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   g.dw_f32 = a.dw_f32;
   g.dw_add = a.dw_add;
   g.alpha = a.gout * T;
-  g.scale = a.mean ? a.scalars + 1 : nullptr;
+  g.scale = a.mean ? (const float*)(g.count + 5) : nullptr;
   g.scale2 = a.gout_dev;
   g.slab = a.slab;
   g.ld_slab = a.ld_slab;

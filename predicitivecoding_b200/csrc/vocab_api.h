@@ -27,7 +27,7 @@ struct VocabHeadArgs {
   int K;                // entries per row (1 for cross entropy)
   float temperature;
   float* loss;          // [N] row losses
-  float* scalars;       // [2]: sum or mean of the row losses, 1 / counted rows (nullptr: not wanted)
+  float* total;         // sum or mean of the row losses (nullptr: not wanted)
 };
 
 // Workspaces of the backward.  The vocabulary is taken `piece` columns at a time.
@@ -46,7 +46,8 @@ VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;
-  long long count;   // int [5]: counted rows, finished blocks of the loss kernel, K splits of dw and dx, status of a wait
+  long long count;   // int [6]: counted rows, finished blocks of the loss kernel, K splits of dw and dx, status of a wait;
+                     // float 1 / counted rows, where the losses are summed up
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
   long long norm;    // float2 [N], by packed row: r and 1 / s, the sum of 2^(logit log2(e) / temperature - r)
@@ -70,7 +71,6 @@ struct VocabGradArgs {
   int distill;
   float temperature;
   void* saved;           // buffer of the forward
-  const float* scalars;
   float gout;            // gradient of the loss: gout * *gout_dev (nullptr: 1) / (counted rows, for the mean)
   const float* gout_dev;
   int mean;

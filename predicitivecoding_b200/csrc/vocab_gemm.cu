@@ -610,12 +610,12 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
     if (!ok) break;
   }
   if (lane == 0) bulk_group_wait_all();   // every TMA store has landed
-  if (a.scalars == nullptr) return;
+  if (a.total == nullptr) return;
   bar_sync(5, kEpi);
   if (tid == 0) *last = arrive_last(a.done, (int)gridDim.x);
   bar_sync(5, kEpi);
   if (!*last) return;
-  add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.scalars, sums, tid, [] { bar_sync(5, kEpi); });
+  add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.total, a.inverse, sums, tid, [] { bar_sync(5, kEpi); });
 }
 
 PCB_DEVICE bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -61,7 +61,7 @@ struct HeadGemm {
   // WHOLE
   float* loss;            // [N] by batch row: factor * the divergence in bits
   float factor;
-  float* scalars;         // as row_loss_kernel leaves them (nullptr: not wanted)
+  float *total, *inverse; // as row_loss_kernel leaves them (nullptr: not wanted)
   int mean;
   int* done;              // CTAs that are done, 0 before the launch
   // GRAD, BWD
@@ -136,10 +136,11 @@ __device__ inline bool arrive_last(int* done, int blocks) {
   return before == blocks - 1;
 }
 
-// The last step of a loss: the rows' losses added up by THREADS threads in a fixed order and in 64 bits.  scalars[0] = their
-// sum or mean, scalars[1] = 1 / counted rows (both 0 when there are none).  `sync` joins the threads.
+// The last step of a loss: the rows' losses added up by THREADS threads in a fixed order and in 64 bits.  *total = their sum
+// or mean, *inverse = 1 / counted rows (both 0 when there are none).  `sync` joins the threads.
 template <int THREADS, typename F>
-__device__ inline void add_losses(const float* loss, int N, int rows, int mean, float* scalars, double* sums, int tid, F sync) {
+__device__ inline void add_losses(const float* loss, int N, int rows, int mean, float* total, float* inverse, double* sums,
+                                  int tid, F sync) {
   double t = 0.0;
 #pragma unroll 8
   for (int i = tid; i < N; i += THREADS) t += __ldcg(loss + i);
@@ -152,8 +153,8 @@ __device__ inline void add_losses(const float* loss, int N, int rows, int mean, 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (tid == 0) {
-      scalars[0] = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
-      scalars[1] = rows > 0 ? 1.f / (float)rows : 0.f;
+      *total = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
+      *inverse = rows > 0 ? 1.f / (float)rows : 0.f;
     }
   }
 }

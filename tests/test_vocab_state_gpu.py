@@ -1,0 +1,41 @@
+"""What a loss of the vocabulary head hands back, keeps and needs on the device: a loss that may be changed in place, a
+state that a backward leaves as it was, workspaces within their bound, the launches that are counted, and results that
+say so when a kernel gave up a wait."""
+import pytest
+import torch
+
+from predicitivecoding_b200 import ops
+from predicitivecoding_b200.ops import vocab
+from test_vocab_gpu import head, teacher
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+STATUS = 4          # word of the state's counters
+
+
+def forms(N, V, D, seed=3, **kw):
+    x, w, tgt, g = head(N, V, D, seed)
+    ids, t = teacher(N, V, 6, tgt, g, torch.float32)
+    return x, w, {"ce": lambda x, w, r="mean": vocab.ce_fwd(x, w, tgt, -1, r),
+                  "distill": lambda x, w, r="mean": vocab.distill_fwd(x, w, ids, t, 2.0, r)}, \
+        {"ce": lambda x, w, r="mean": vocab.cross_entropy(x, w, tgt, -1, r),
+         "distill": lambda x, w, r="mean": vocab.distill(x, w, ids, t, 2.0, r)}
+
+
+@pytest.mark.parametrize("N,V", [(3, 900), (300, 900), (300, 200)])
+@pytest.mark.parametrize("kind", ["ce", "distill"])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_a_loss_may_be_changed_in_place(N, V, kind, reduction):
+    x, w, fwd, auto = forms(N, V, 64)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = auto[kind](xg, wg, reduction)
+    whole = float(loss.detach())
+    loss /= 4
+    assert float(loss.detach()) == whole / 4
+    loss.backward()
+    first, state = fwd[kind](x, w, reduction)
+    dx, dw = vocab.head_bwd(state, 0.25)
+    assert torch.equal(xg.grad, dx) and torch.equal(wg.grad, dw)
+    first.zero_()                                  # the gradient does not read it again
+    again = vocab.head_bwd(state, 0.25)
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
