@@ -577,11 +577,15 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
   a.plan = st.plan.whole ? st.plan
                          : pcb::vocab_plan(a.N, a.V, a.D, (int)std::min<int64_t>(piece, 1 << 30), false, num_sms());
   a.ld_slab = (a.D + 3) / 4 * 4;
-  const int64_t gbytes = a.plan.whole ? 0 : (pcb::vocab_g_rows(a.N) * a.plan.piece * 2 + 255) / 256 * 256;
+  // g (a multiple of 256 bytes), the slabs, the splits
+  const int64_t gbytes = a.plan.whole ? 0 : pcb::vocab_g_rows(a.N) * a.plan.piece * 2;
   const bool slabs = dx || a.plan.dw_max > 1;
-  at::Tensor ws = at::empty({gbytes + (slabs ? 4 * a.plan.all_rows * a.ld_slab : 0)}, st.saved.options());
-  a.g = a.plan.whole ? st.g.data_ptr() : ws.data_ptr();
-  if (slabs) a.slab = reinterpret_cast<float*>(static_cast<char*>(ws.data_ptr()) + gbytes);
+  const int64_t sbytes = slabs ? 4 * a.plan.all_rows * a.ld_slab : 0;
+  at::Tensor ws = at::empty({gbytes + sbytes + 8}, st.saved.options());
+  char* base = static_cast<char*>(ws.data_ptr());
+  a.g = a.plan.whole ? st.g.data_ptr() : base;
+  if (slabs) a.slab = reinterpret_cast<float*>(base + gbytes);
+  a.splits = reinterpret_cast<int*>(base + gbytes + sbytes);
   check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", (a.plan.whole ? 1 : 2) * a.plan.pieces + (slabs ? 1 : 0));
   return {dx, dw};
 }

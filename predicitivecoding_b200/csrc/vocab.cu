@@ -1316,10 +1316,10 @@ static int launch_few_rows(const HeadGemm& h, const void* xc, long long ldxc, co
 }
 
 // what the backward's launches, and the forward's where it makes g, know of the gradients' products
-static void plan_products(HeadGemm& g, const VocabPlan& plan, int N, int* count, int num_sms) {
+static void plan_products(HeadGemm& g, const VocabPlan& plan, int N, int* splits, int num_sms) {
   g.g_low = (N + 255) / 256 * 256;
   g.g_rows = (int)vocab_g_rows(N);
-  g.plan = count + 2;
+  g.plan = splits;
   g.dw_max = plan.dw_max;
   g.slab_rows = plan.slab_rows;
   g.bwd_pairs = num_sms / 2;
@@ -1408,7 +1408,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
     return rc ? rc : finish(l, (a.V + 127) / 128);
   }
   if (plan.whole) {
-    plan_products(g, plan, a.N, count, num_sms);
+    plan_products(g, plan, a.N, count + 2, num_sms);
     g.q = q;
     g.loss = a.loss;
     g.factor = factor;
@@ -1442,7 +1442,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
     g.start = (const unsigned short*)at(sv, l.start);
   }
   g.norm = (const float2*)at(sv, l.norm);
-  plan_products(g, a.plan, a.N, (int*)at(sv, l.count), num_sms);
+  plan_products(g, a.plan, a.N, a.plan.whole ? (int*)at(sv, l.count) + 2 : a.splits, num_sms);
   g.want_dw = a.dw != nullptr;
   g.want_dx = a.dx != nullptr;
   g.lddw = a.lddw;

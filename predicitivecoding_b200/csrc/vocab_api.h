@@ -46,8 +46,8 @@ VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;
-  long long count;   // int [6]: counted rows, finished blocks of the loss kernel, K splits of dw and dx, status of a wait;
-                     // float 1 / counted rows, where the losses are summed up
+  long long count;   // int [6]: counted rows, finished blocks of the loss kernel, K splits of dw and dx (where the forward
+                     // makes g), status of a wait; float 1 / counted rows, where the losses are summed up
   long long row;     // int [N]: batch place of each packed row
   long long pos;     // int [N]: packed place of each row, -1 where it is not counted
   long long norm;    // float2 [N], by packed row: r and 1 / s, the sum of 2^(logit log2(e) / temperature - r)
@@ -83,6 +83,8 @@ struct VocabGradArgs {
   int dw_add;
   VocabPlan plan;
   void* g;               // bf16, vocab_g_rows(N) * piece: workspace, or as the forward left it
+  int* splits;           // int [2], K splits of dw and dx: workspace (not used where the forward made g).  The backward writes
+                         // nothing into `saved` but a status, so two of one state may run at the same time
   float* slab;           // workspace: fp32 [all_rows, ld_slab]
   long long ld_slab;
 };

@@ -13,6 +13,12 @@ DEV = "cuda"
 STATUS = 4          # word of the state's counters
 
 
+def counters(state):
+    """The state's int32 words: counted rows, blocks done, K splits of dw and dx, status of a wait."""
+    at = state.N * ((state.D + 7) // 8 * 8) * 2
+    return state.saved.view(torch.int32)[(at + 255) // 256 * 64:][:8]
+
+
 def forms(N, V, D, seed=3, **kw):
     x, w, tgt, g = head(N, V, D, seed)
     ids, t = teacher(N, V, 6, tgt, g, torch.float32)
@@ -39,3 +45,27 @@ def test_a_loss_may_be_changed_in_place(N, V, kind, reduction):
     first.zero_()                                  # the gradient does not read it again
     again = vocab.head_bwd(state, 0.25)
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+
+
+@pytest.mark.parametrize("N,V,D", [(3, 5000, 64), (40, 5000, 64), (300, 5000, 64), (200, 2000, 1024), (300, 300, 64)])
+@pytest.mark.parametrize("kind", ["ce", "distill"])
+def test_a_backward_leaves_the_state_as_it_was(N, V, D, kind):
+    """Two backwards of one state may run at the same time, in pieces of different sizes."""
+    x, w, fwd, _ = forms(N, V, D)
+    _, state = fwd[kind](x, w)
+    if V > 512:
+        counters(state)[2:4] = -7                  # the splits are each backward's own
+    before = state.saved.clone()
+    pieces = (0, 256, 1024, 2560)
+    want = [vocab.head_bwd(state, piece=p) for p in pieces]
+    assert torch.equal(state.saved, before)
+    side = [torch.cuda.Stream() for _ in pieces]
+    got = []
+    for s, p in zip(side, pieces):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(vocab.head_bwd(state, piece=p))
+    for s in side:
+        torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
