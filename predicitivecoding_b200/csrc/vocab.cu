@@ -1244,14 +1244,15 @@ VocabLayout vocab_layout(int N, int V, int D, int K, bool distill) {
   return l;
 }
 
-long long vocab_g_rows(int N) { return (N + 255LL) / 256 * 256 + kTwoTermRows; }
+// Rows of g: the counted ones up to the next tile; behind the one tile that a second term is made for, that term.
+long long vocab_g_rows(int N) { return std::max((N + 255LL) / 256 * 256, 2LL * kTwoTermRows); }
 
 static bool few_rows(int N, int D) { return N <= kFewRows && D <= kFewColumns; }
 
 VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num_sms) {
   VocabPlan r{};
   const long long all = (V + 255LL) / 256 * 256;
-  long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2LL * N) / 256 * 256;
+  long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2 * vocab_g_rows(N)) / 256 * 256;
   p = std::max(256LL, std::min(p, all));
   r.pieces = (int)((all + p - 1) / p);
   p = (all / 256 + r.pieces - 1) / r.pieces * 256;   // pieces of one size
@@ -1317,7 +1318,7 @@ static int launch_few_rows(const HeadGemm& h, const void* xc, long long ldxc, co
 
 // what the backward's launches, and the forward's where it makes g, know of the gradients' products
 static void plan_products(HeadGemm& g, const VocabPlan& plan, int N, int* splits, int num_sms) {
-  g.g_low = (N + 255) / 256 * 256;
+  g.g_low = kTwoTermRows;
   g.g_rows = (int)vocab_g_rows(N);
   g.plan = splits;
   g.dw_max = plan.dw_max;

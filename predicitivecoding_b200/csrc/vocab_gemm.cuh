@@ -69,7 +69,7 @@ struct HeadGemm {
   // g: panels of 64 columns, each [g_rows, 64], so that every box that is stored or loaded (32 or 64 rows of a panel) is
   // one run of memory, whichever of its two dimensions the product contracts
   int g_rows;
-  int g_low;              // row of a panel where the second terms begin (a multiple of 256, at least N)
+  int g_low;              // row of a panel where the second terms begin: behind the one tile of rows that has them
   // BWD.  The K splits of the two products depend on the number of counted rows: GRAD of the first
   // piece of the vocabulary works them out and leaves them in plan[0] (dw) and plan[1] (dx).
   int* plan;

@@ -11,10 +11,15 @@ Shapes: tokens and targets [...] int32 or int64, w [V, D] (nn.Linear layout, the
     head_bwd     the gradients of either loss
 
 The losses take bf16 x and w, multiply on the tensor cores and hold the logits, the softmax statistics and every sum
-in fp32; the logits themselves are never stored.  ``head_bwd`` makes them again, ``piece`` columns of the vocabulary
-at a time, which costs 8 N V D operations for a step instead of 6 and needs N * piece * 2 bytes (256 MiB by default)
-instead of N * V * 2.  A vocabulary of up to 512 whose N * V * 2 bytes stay within that bound is the exception: its loss
-is taken together with the gradient of its logits, which the state then keeps.  softmax - target is rounded to bf16 once, as an operand of the two gradient products.
+in fp32; the logits themselves are not stored.  ``head_bwd`` makes them again, ``piece`` columns of the vocabulary
+at a time, and keeps the gradient of a piece of them, g, for the two products that read it: 8 N V D operations for a
+step instead of 6.  Its workspaces are g, R * piece * 2 bytes with R = N rounded up to a multiple of 256 and at least
+512 (``piece`` is by default as large as 256 MiB allow, which may be all of V), and fp32 slabs, (R + 4096) * D * 4 bytes
+for dx and up to 19 MiB more where dw has few tiles.  The state keeps N * D * 2 bytes for packed rows.  A vocabulary of up to
+512 whose g stays within the bound is the exception: its loss is taken together with g, which the state then keeps.
+
+softmax - target is an operand of the two gradient products in bf16: rounded once for more than 256 counted rows, as
+two bf16 terms (2^-14 of it left out) up to there, whatever the type of the results.
 
 Rows that are not counted - a target outside [0, V) or equal to ``ignore_index``, a teacher's list without entries -
 have loss 0 and gradient 0, are not read and cost no products; the mean is over the counted rows, and 0 when there
@@ -97,7 +102,7 @@ def head_bwd(state: HeadState, gout: Union[float, torch.Tensor] = 1.0, dx: Optio
              piece: int = 0) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx [..., D], dw [V, D]) of a mean or summed loss times ``gout`` (a number, or an fp32 CUDA tensor with one
     value).  They are bf16, or go into ``dx`` / ``dw`` (bf16 or fp32; ``accumulate`` adds to ``dw``).  ``piece``: columns of
-    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of workspace take; a vocabulary of up
+    the vocabulary at a time (rounded up to a multiple of 256; 0: as many as 256 MiB of g take; a vocabulary of up
     to 512 may be taken whole).  x and w must
     still hold what the loss read."""
     if isinstance(gout, torch.Tensor):

@@ -69,3 +69,17 @@ def test_a_backward_leaves_the_state_as_it_was(N, V, D, kind):
         torch.cuda.current_stream().wait_stream(s)
     for a, b in zip(got, want):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("N,V", [(1, 300000), (200, 300000), (300, 262144), (257, 270001)])
+def test_the_workspace_of_g_is_bounded(N, V):
+    """256 MiB of g by default, however many rows its panels are padded to."""
+    x, w, tgt, _ = head(N, V, 16, 4)
+    _, state = vocab.ce_fwd(x, w, tgt)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    dw = vocab.head_bwd(state, need_dx=False)[1]
+    torch.cuda.synchronize()
+    extra = torch.cuda.max_memory_allocated() - held - dw.numel() * 2
+    assert extra <= (256 << 20) + (1 << 20)
