@@ -586,7 +586,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
   a.g = a.plan.whole ? st.g.data_ptr() : base;
   if (slabs) a.slab = reinterpret_cast<float*>(base + gbytes);
   a.splits = reinterpret_cast<int*>(base + gbytes + sbytes);
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", (a.plan.whole ? 1 : 2) * a.plan.pieces + (slabs ? 1 : 0));
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", (a.plan.whole ? 1 : 2) * a.plan.pieces + 1);
   return {dx, dw};
 }
 

@@ -503,6 +503,7 @@ __global__ void __launch_bounds__(32 * kLossParts)
   const int j = blockIdx.x * 32 + w;   // this warp's packed row
   const int place = j < N ? row[j] : 0;   // asked for together with the count: a row behind it holds anything
   const int rows = min(count[0], N);
+  const bool spoilt = count[4] != 0;   // a wait ran out: the pairs and the logits at the targets may be anything
   const bool live = j < rows;
   const int n = live ? place : 0;
   // the first two targets of a lane: weight, its logarithm, logit
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(32 * kLossParts)
   }
   l = warp_sum(l);
   if (live && lane == 0) {
-    loss[n] = l * factor;
+    loss[n] = spoilt ? NAN : l * factor;
     norm[j] = make_float2(ref, 1.f / tot);
   }
   if (total == nullptr) return;
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(32 * kLossParts)
   if (threadIdx.x == 0) last = arrive_last(&count[1], (int)gridDim.x);
   __syncthreads();
   if (!last) return;
-  add_losses<32 * kLossParts>(loss, N, rows, mean, total, inverse, sums, threadIdx.x, [] { __syncthreads(); });
+  add_losses<32 * kLossParts>(loss, N, rows, mean, count + 4, total, inverse, sums, threadIdx.x, [] { __syncthreads(); });
 }
 
 // Gradients from their fp32 slabs: the sum in slab order, times the gradient's factor.  The first N rows are dx's, found
@@ -577,19 +578,36 @@ struct FinishArgs {
   int slab_rows;         // of dx, dw's behind them
   const int* count;
   const int* plan;       // K splits of dw and dx
+  const int* status;     // of the waits of all launches before
   const int* pos;
   void *dx, *dw;
   long long ld_slab, lddx, lddw;
   int dx_f32, dw_f32, dw_add;
   int N, V, D;           // N = 0 where dx is not wanted, V = 0 where dw cannot be in slabs
+  int dw_rows;           // 0 where dw is not wanted
   float alpha;
   const float* scale;
   const float* scale2;
 };
 
+// [rows, D] of NaN, by all threads of the grid
+PCB_DEVICE void spoil(void* p, int f32, long long ld, int rows, int D) {
+  const long long step = (long long)gridDim.x * gridDim.y * kThreads;
+  for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x; i < (long long)rows * D; i += step) {
+    const long long r = i / D, at = r * ld + (i - r * D);
+    if (f32) reinterpret_cast<float*>(p)[at] = NAN;
+    else reinterpret_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(NAN);
+  }
+}
+
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a) {
   pdl_begin();
+  if (*a.status != 0) {   // some launch gave up a wait: what the products wrote, dw itself too, may be anything
+    if (a.N > 0) spoil(a.dx, a.dx_f32, a.lddx, a.N, a.D);
+    spoil(a.dw, a.dw_f32, a.lddw, a.dw_rows, a.D);
+    return;
+  }
   int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (n >= a.N + a.V) return;
   const bool w = n >= a.N;
@@ -1473,6 +1491,7 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   f.slab_rows = a.plan.slab_rows;
   f.count = g.count;
   f.plan = g.plan;
+  f.status = g.err;
   f.pos = (const int*)at(sv, l.pos);
   f.dx = a.dx;
   f.dw = a.dw;
@@ -1484,15 +1503,16 @@ int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   f.dw_add = a.dw_add;
   f.N = a.dx != nullptr ? a.N : 0;
   f.V = a.dw != nullptr && a.plan.dw_max > 1 ? a.V : 0;
+  f.dw_rows = a.dw != nullptr ? a.V : 0;
   f.D = a.D;
   f.alpha = g.alpha;
   f.scale = g.scale;
   f.scale2 = g.scale2;
-  if (f.N + f.V == 0) return 0;
   const bool v4 = a.D % 4 == 0 && (f.N == 0 || (a.lddx % 4 == 0 && al(a.dx, a.dx_f32 ? 16 : 8))) &&
                   (f.V == 0 || (a.lddw % 4 == 0 && al(a.dw, a.dw_f32 ? 16 : 8)));
   const int vecs = v4 ? a.D / 4 : a.D;
-  const dim3 grid((f.N + f.V + 7) / 8, (vecs + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
+  // with nothing to gather the launch is there for the status alone
+  const dim3 grid(std::max((f.N + f.V + 7) / 8, 1), (vecs + 32 * kFinishVecs - 1) / (32 * kFinishVecs));
   if (grid.y > 65535) return -1;
   return pdl_launch(v4 ? finish_kernel<4> : finish_kernel<1>, grid, dim3(kThreads), 0, s, f) == cudaSuccess ? 0 : -3;
 }

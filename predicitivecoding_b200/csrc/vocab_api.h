@@ -42,7 +42,8 @@ struct VocabPlan {
 // `gradient`: for a forward that a backward follows
 VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num_sms);
 
-// Where the forward keeps what the backward reads: byte offsets into one buffer.
+// Where the forward keeps what the backward reads: byte offsets into one buffer.  A kernel that gives up a wait records it
+// in the status and leaves its outputs unfinished; the losses and the gradients are then NaN.
 struct VocabLayout {
   long long xc;      // [N, ldxc] bf16: the counted rows of x, packed; zero rows up to the next multiple of 64
   long long ldxc;

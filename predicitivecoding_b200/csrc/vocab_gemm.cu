@@ -480,6 +480,7 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
   const int mine = q * 32 + lane;
   Tile tile;
   RowTargets ahead;
+  bool all_ok = true;
   auto row_of = [&](const Tile& t) { return t.mb * 2 * kBM + (int)rank * kBM + q * 32; };
   if (tile_at<HEAD_WHOLE>(a, sh, pair, pairs, 0, tile)) {
     ahead.ask_row<HEAD_WHOLE>(a, row_of(tile) + lane, half * 128, sh.rows);
@@ -607,15 +608,17 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
     if (half) losses[mine] = l;
     bar_sync(1 + q, 64);
     if (!half && live) a.loss[place] = (l + losses[mine]) * a.factor;
+    all_ok = ok;
     if (!ok) break;
   }
   if (lane == 0) bulk_group_wait_all();   // every TMA store has landed
   if (a.total == nullptr) return;
+  if (!all_ok) record_error(a.err, kErrTimeoutTmemFull);   // known to the last block, whichever role gave up first
   bar_sync(5, kEpi);
   if (tid == 0) *last = arrive_last(a.done, (int)gridDim.x);
   bar_sync(5, kEpi);
   if (!*last) return;
-  add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.total, a.inverse, sums, tid, [] { bar_sync(5, kEpi); });
+  add_losses<kEpi>(a.loss, a.N, sh.rows, a.mean, a.err, a.total, a.inverse, sums, tid, [] { bar_sync(5, kEpi); });
 }
 
 PCB_DEVICE bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

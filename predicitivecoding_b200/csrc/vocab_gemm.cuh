@@ -1,6 +1,7 @@
 // Products of the vocabulary head (csrc/vocab_gemm.cu): what one launch reads and writes.
 #pragma once
 #include <atomic>
+#include <cmath>
 
 #include <cuda_runtime.h>
 
@@ -137,10 +138,11 @@ __device__ inline bool arrive_last(int* done, int blocks) {
 }
 
 // The last step of a loss: the rows' losses added up by THREADS threads in a fixed order and in 64 bits.  *total = their sum
-// or mean, *inverse = 1 / counted rows (both 0 when there are none).  `sync` joins the threads.
+// or mean, *inverse = 1 / counted rows (both 0 when there are none); *total = NaN behind a wait that ran out.  `sync`
+// joins the threads.
 template <int THREADS, typename F>
-__device__ inline void add_losses(const float* loss, int N, int rows, int mean, float* total, float* inverse, double* sums,
-                                  int tid, F sync) {
+__device__ inline void add_losses(const float* loss, int N, int rows, int mean, const int* status, float* total, float* inverse,
+                                  double* sums, int tid, F sync) {
   double t = 0.0;
 #pragma unroll 8
   for (int i = tid; i < N; i += THREADS) t += __ldcg(loss + i);
@@ -153,7 +155,7 @@ __device__ inline void add_losses(const float* loss, int N, int rows, int mean, 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (tid == 0) {
-      *total = (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
+      *total = __ldcg(status) != 0 ? NAN : (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
       *inverse = rows > 0 ? 1.f / (float)rows : 0.f;
     }
   }

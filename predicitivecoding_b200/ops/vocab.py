@@ -28,6 +28,9 @@ are none.  A teacher's entry is absent when its id is outside [0, V) or its logi
 The ids of a row's list are meant to differ; entries that repeat an id count as they stand in the loss, and together
 in the gradient.  All results are the same from run to run: no sum depends on the order in which atomics arrive.
 x and w are read again by ``head_bwd`` and must not change in between.
+A kernel that gives up a wait (which none does unless the device is in trouble) records it in the state: the loss and
+the gradients made from it are NaN then, and ``state.status()``, which synchronises, returns the wait's code instead
+of 0.  Several backwards of one state may run at the same time.
 Kernels: csrc/vocab.cu, csrc/vocab_gemm.cu.
 """
 from __future__ import annotations

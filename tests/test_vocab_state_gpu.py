@@ -83,3 +83,31 @@ def test_the_workspace_of_g_is_bounded(N, V):
     torch.cuda.synchronize()
     extra = torch.cuda.max_memory_allocated() - held - dw.numel() * 2
     assert extra <= (256 << 20) + (1 << 20)
+
+
+@pytest.mark.parametrize("N,V,D", [(3, 700, 64), (40, 700, 64), (300, 5000, 64), (200, 2000, 1024), (300, 300, 64),
+                                   (700, 30000, 264)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_gradients_behind_a_wait_that_ran_out_are_nan(N, V, D, f32):
+    """A kernel that gives up a wait records it in the state and leaves its outputs unfinished: the gradients are NaN
+    then, whichever launch writes them, so nobody trains on them."""
+    x, w, fwd, _ = forms(N, V, D)
+    _, state = fwd["ce"](x, w)
+    assert state.status() == 0
+    counters(state)[STATUS] = 2
+    assert state.status() == 2
+    dt = torch.float32 if f32 else torch.bfloat16
+    new = lambda *s: torch.zeros(*s, device=DEV, dtype=dt)
+    nan = lambda t: bool(torch.isnan(t.float()).all())
+    for piece in (0, 512):
+        dx, dw = vocab.head_bwd(state, dx=new(N, D), dw=new(V, D), piece=piece)
+        assert nan(dx) and nan(dw)
+        assert nan(vocab.head_bwd(state, dx=new(N, D), need_dw=False, piece=piece)[0])
+        assert nan(vocab.head_bwd(state, dw=new(V, D), need_dx=False, piece=piece)[1])
+        assert nan(vocab.head_bwd(state, dw=new(V, D), accumulate=True, piece=piece)[1])
+    apart = new(N, D + 16)[:, 8:8 + D]
+    rows = new(V, D + 5)[:, 3:3 + D]
+    vocab.head_bwd(state, dx=apart, dw=rows)
+    assert nan(apart) and nan(rows)
+    counters(state)[STATUS] = 0
+    assert not bool(torch.isnan(vocab.head_bwd(state)[1].float()).any())
