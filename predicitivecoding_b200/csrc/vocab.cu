@@ -590,8 +590,8 @@ struct FinishArgs {
   const float* scale2;
 };
 
-// [rows, D] of NaN, by all threads of the grid
-PCB_DEVICE void spoil(void* p, int f32, long long ld, int rows, int D) {
+// [rows, D] of NaN, by all threads of the grid; not a part of the code that every launch fetches
+__device__ __noinline__ void spoil(void* p, int f32, long long ld, int rows, int D) {
   const long long step = (long long)gridDim.x * gridDim.y * kThreads;
   for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x; i < (long long)rows * D; i += step) {
     const long long r = i / D, at = r * ld + (i - r * D);
@@ -603,18 +603,16 @@ PCB_DEVICE void spoil(void* p, int f32, long long ld, int rows, int D) {
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) finish_kernel(FinishArgs a) {
   pdl_begin();
-  if (*a.status != 0) {   // some launch gave up a wait: what the products wrote, dw itself too, may be anything
+  int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const bool in = n < a.N + a.V, w = n >= a.N;
+  if (w) n -= a.N;
+  const int status = *a.status, slabs = a.plan[w ? 0 : 1], j = w ? n : a.pos[n];   // asked for together
+  if (__builtin_expect(status != 0, 0)) {   // some launch gave up a wait: what the products wrote, dw itself too, may be anything
     if (a.N > 0) spoil(a.dx, a.dx_f32, a.lddx, a.N, a.D);
     spoil(a.dw, a.dw_f32, a.lddw, a.dw_rows, a.D);
     return;
   }
-  int n = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (n >= a.N + a.V) return;
-  const bool w = n >= a.N;
-  if (w) n -= a.N;
-  const int slabs = a.plan[w ? 0 : 1];
-  if (w && slabs == 1) return;   // written by the product itself
-  const int j = w ? n : a.pos[n];
+  if (!in || (w && slabs == 1)) return;   // slabs == 1: written by the product itself
   float f = a.alpha;
   if (a.scale != nullptr) f *= *a.scale;
   if (a.scale2 != nullptr) f *= *a.scale2;

@@ -143,6 +143,7 @@ __device__ inline bool arrive_last(int* done, int blocks) {
 template <int THREADS, typename F>
 __device__ inline void add_losses(const float* loss, int N, int rows, int mean, const int* status, float* total, float* inverse,
                                   double* sums, int tid, F sync) {
+  const int spoilt = tid == 0 ? __ldcg(status) : 0;
   double t = 0.0;
 #pragma unroll 8
   for (int i = tid; i < N; i += THREADS) t += __ldcg(loss + i);
@@ -155,7 +156,7 @@ __device__ inline void add_losses(const float* loss, int N, int rows, int mean, 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (tid == 0) {
-      *total = __ldcg(status) != 0 ? NAN : (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
+      *total = spoilt != 0 ? NAN : (float)(mean ? (rows > 0 ? t / rows : 0.0) : t);
       *inverse = rows > 0 ? 1.f / (float)rows : 0.f;
     }
   }
