@@ -496,8 +496,9 @@ PCB_DEVICE void whole_rows(const HeadGemm& a, const Shape& sh, uint8_t* smem, ui
 #pragma unroll 1
     for (int nb = 0; nb < sh.num_n; ++nb) {
       const int acc = (u + nb) & 1, col0 = nb * 256 + half * 128;
-      // behind a wait that ran out the barriers below are still met, and both threads of a row leave together
-      ok = mbar_wait(&tfull[acc], ((u + nb) >> 1) & 1, a.err, kErrTimeoutTmemFull, abort_flag) && ok;
+      // behind a wait that ran out the barriers below are still met, and both threads of a row leave together; the lanes of
+      // a warp are together again before its loads from TMEM
+      ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], ((u + nb) >> 1) & 1, a.err, kErrTimeoutTmemFull, abort_flag)) && ok;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + half * 128;
 #pragma unroll 1
@@ -842,7 +843,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i == 1) ahead.ask_entries(a);
         if (i == 2) ahead.template ask_ids<MODE>(a);
       };
-      if (!mbar_wait(&tfull[acc], acc_phase, a.err, kErrTimeoutTmemFull, abort_flag)) break;
+      // the warp leaves together: what follows is warp-wide
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.err, kErrTimeoutTmemFull, abort_flag))) break;
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if (MODE == HEAD_STAT) {
@@ -1051,10 +1053,15 @@ __global__ void __launch_bounds__(kScoreThreads, 2)
     umma_commit(done);
   }
   __syncwarp();
-  // all lanes leave together, before the warp-wide loads; a wait that ran out has recorded its error
-  __all_sync(0xffffffffu, mbar_wait(done, 0, a.err, kErrTimeoutTmemFull, abort_flag));
+  // the product ends with `done` even where a wait for an operand ran out in front of it
+  const bool ok = mbar_wait(done, 0, a.err, kErrTimeoutTmemFull, abort_flag) && !*abort_flag;
   tc_fence_after();
-  __syncthreads();   // every warp is past the wait: no copy or product uses the ring
+  if (!__syncthreads_and(ok)) {   // the status says so, and the row losses are NaN
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, 256);
+    return;
+  }
+  // every warp is past the wait: no copy or product uses the ring
   float* logits = reinterpret_cast<float*>(smem);   // [NB][LD]
 #pragma unroll 1
   for (int b = 0; b < NB; b += 32) {
