@@ -442,6 +442,16 @@ PCB_DEVICE void store_box64(const CUtensorMap* map, uint8_t* stg, int& box_at, c
   }
 }
 
+// Behind a wait that ran out, copies into this block's shared memory and matrix instructions that read it or write TMEM may
+// still be on their way, and the barriers that they would have completed may lie in the other CTA.  A thread that sees
+// the abort stays 2 ms, a thousand times as long as any of them takes, before it meets the block's last barrier, so none
+// of them finds the memory in other hands.
+constexpr long long kSettleCycles = 4000000;
+PCB_DEVICE void settle() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < kSettleCycles) __nanosleep(1000);
+}
+
 PCB_DEVICE void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // whether `p` holds for all of them
 PCB_DEVICE bool bar_and(int id, int threads, bool p) {
@@ -940,6 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (MODE != HEAD_STAT && lane == 0) bulk_group_wait_all();   // every TMA store has landed
   }
+  if (*abort_flag) settle();
   __syncwarp();
   tc_fence_before();
   cluster_sync_all();   // both CTAs done with TMEM and with each other's barriers
@@ -1057,6 +1068,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2)
   const bool ok = mbar_wait(done, 0, a.err, kErrTimeoutTmemFull, abort_flag) && !*abort_flag;
   tc_fence_after();
   if (!__syncthreads_and(ok)) {   // the status says so, and the row losses are NaN
+    settle();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem, 256);
     return;
