@@ -486,7 +486,7 @@ std::pair<at::Tensor, HeadState> head_fwd(const char* what, const at::Tensor& x,
   if (st.plan.whole) st.g = at::empty({pcb::vocab_g_rows(a.N) * st.plan.piece}, x.options());
   check(pcb_vocab_fwd(a, st.plan, st.saved.data_ptr(), part.data_ptr(), st.g.defined() ? st.g.data_ptr() : nullptr,
                       st.mean ? 1 : 0, num_sms(), cur_stream()),
-        what, (st.distill ? 2 : 1) + (st.plan.whole ? 1 : 2));
+        what, pcb_vocab_fwd_launches(st.plan, a.N, st.distill));
   return {loss, st};
 }
 
@@ -586,7 +586,7 @@ std::pair<c10::optional<at::Tensor>, c10::optional<at::Tensor>> vocab_head_bwd(
   a.g = a.plan.whole ? st.g.data_ptr() : base;
   if (slabs) a.slab = reinterpret_cast<float*>(base + gbytes);
   a.splits = reinterpret_cast<int*>(base + gbytes + sbytes);
-  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", (a.plan.whole ? 1 : 2) * a.plan.pieces + 1);
+  check(pcb_vocab_bwd(a, num_sms(), cur_stream()), "head_bwd", pcb_vocab_bwd_launches(a.plan));
   return {dx, dw};
 }
 

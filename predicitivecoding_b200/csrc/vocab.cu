@@ -1440,6 +1440,14 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
   return finish(l, l.granules);
 }
 
+// the lists' sort, a long batch's count, the packing; the product, which makes the row losses too where it is whole
+int pcb_vocab_fwd_launches(const VocabPlan& plan, int N, bool distill) {
+  return (distill ? 1 : 0) + (N > kSelfCountRows ? 1 : 0) + 1 + (plan.whole ? 1 : 2);
+}
+
+// for each piece g, unless the forward made it, and the products; the gather
+int pcb_vocab_bwd_launches(const VocabPlan& plan) { return (plan.whole ? 1 : 2) * plan.pieces + 1; }
+
 int pcb_vocab_bwd(const VocabGradArgs& a, int num_sms, cudaStream_t s) {
   const VocabLayout l = vocab_layout(a.N, a.V, a.D, a.K, a.distill != 0);
   void* sv = a.saved;

@@ -97,6 +97,9 @@ int pcb_vocab_pad_rows(const void* src, long long ld, void* dst, long long ldd, 
 // `part`: [granules, N] float2 workspace; `g`: bf16 [vocab_g_rows(N) * piece] where plan.whole
 int pcb_vocab_fwd(const pcb::VocabHeadArgs& a, const pcb::VocabPlan& plan, void* saved, void* part, void* g, int mean,
                   int num_sms, cudaStream_t s);
+// kernels that these launch
+int pcb_vocab_fwd_launches(const pcb::VocabPlan& plan, int N, bool distill);
+int pcb_vocab_bwd_launches(const pcb::VocabPlan& plan);
 int pcb_vocab_bwd(const pcb::VocabGradArgs& a, int num_sms, cudaStream_t s);
 
 // x[n] = scale * w[tok[n]]; rows of tokens outside [0, V) are zero

@@ -19,7 +19,7 @@ def counters(state):
     return state.saved.view(torch.int32)[(at + 255) // 256 * 64:][:8]
 
 
-def forms(N, V, D, seed=3, **kw):
+def forms(N, V, D, seed=3):
     x, w, tgt, g = head(N, V, D, seed)
     ids, t = teacher(N, V, 6, tgt, g, torch.float32)
     return x, w, {"ce": lambda x, w, r="mean": vocab.ce_fwd(x, w, tgt, -1, r),
@@ -83,6 +83,32 @@ def test_the_workspace_of_g_is_bounded(N, V):
     torch.cuda.synchronize()
     extra = torch.cuda.max_memory_allocated() - held - dw.numel() * 2
     assert extra <= (256 << 20) + (1 << 20)
+
+
+def launches(f):
+    before = ops.launch_count()
+    f()
+    return ops.launch_count() - before
+
+
+def test_launches_are_counted():
+    """Lists are sorted (1), long batches counted (1), rows packed (1), logits (1), row losses (1); loss and g of whole
+    vocabularies come of one launch; rows of w that no vector fits are copied (1).  A backward: g and both
+    products for each piece, and the gather."""
+    for N, long in ((8192, 0), (8193, 1)):
+        for V, whole in ((512, 1), (700, 0)):
+            x, w, fwd, _ = forms(N, V, 16)
+            apart = torch.zeros(V, 21, device=DEV, dtype=torch.bfloat16)[:, 2:18].copy_(w)
+            for kind, lists in (("ce", 0), ("distill", 1)):
+                made = lists + long + 1 + (1 if whole else 2)
+                assert launches(lambda: fwd[kind](x, w)) == made
+                assert launches(lambda: fwd[kind](x, apart)) == made + 1
+                assert launches(lambda: fwd[kind](x, w, "none")) == lists + long + 3
+                state = fwd[kind](x, w)[1]
+                assert launches(lambda: vocab.head_bwd(state)) == (1 if whole else 2) + 1
+                if not whole:
+                    assert launches(lambda: vocab.head_bwd(state, piece=256)) == 2 * 3 + 1
+                    assert launches(lambda: vocab.head_bwd(state, need_dx=False)) == 3
 
 
 @pytest.mark.parametrize("N,V,D", [(3, 700, 64), (40, 700, 64), (300, 5000, 64), (200, 2000, 1024), (300, 300, 64),
