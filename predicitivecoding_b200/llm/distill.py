@@ -76,6 +76,20 @@ def on_policy_round(model, tok, prompts: Sequence[str], teacher_correct: Callabl
     return step(model, tok, data, optimizer, lr, clip_norm)
 
 
+class _Operands(torch.autograd.Function):
+    """``t`` as ``n`` operands in bf16, all of one memory, whose gradients are added in fp32."""
+
+    @staticmethod
+    def forward(ctx, t, n):
+        ctx.set_materialize_grads(False)
+        b = t.bfloat16().contiguous()
+        return tuple(b.view_as(b) for _ in range(n))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return sum(g.float() for g in grads if g is not None), None
+
+
 class TopLogitDistiller:
     """Trains ``student`` on a teacher's top logits.
 
@@ -85,6 +99,10 @@ class TopLogitDistiller:
     head, experts' balance) are those of ``DecoderLM.loss``, which this loss is at alpha 0.  ``embed_scale`` multiplies
     the student's embedding rows; given here it becomes the student's (``DecoderLmConfig.embed_scale``), so that the
     network which is trained is the one that is evaluated, served and saved.
+
+    On a GPU the heads' products take the hidden rows and the output matrix in bf16, as the operators do, and each loss
+    hands their gradients back in bf16; these are added, and reach the parameters, in the parameters' type.  On the CPU
+    everything is in the model's type.
     """
 
     def __init__(self, student: DecoderLM, top_k: int = 32, temperature: float = 2.0, alpha: float = 0.5,
@@ -116,25 +134,24 @@ class TopLogitDistiller:
              training: bool = False) -> torch.Tensor:
         m, c, on_gpu = self.student, self.student.cfg, tokens.is_cuda
         embed = vocab.embedding if on_gpu else vocab.reference_embedding
+        ce, kd = (vocab.cross_entropy, vocab.distill) if on_gpu else (vocab.reference_cross_entropy, vocab.reference_distill)
         balance = m.balance_terms()
-        x = m.hidden(tokens, training, aux_losses=balance, embedded=embed(tokens, m.wemb, c.embed_scale))
+        hidden = m.hidden(tokens, training, aux_losses=balance, embedded=embed(tokens, m.wemb, c.embed_scale))
         live = (targets >= 0) & (targets < c.vocab) & (targets != self.ignore_index)   # as the cross entropy counts
         ids = torch.where(live[..., None], ids, torch.full_like(ids, -1))
-        if on_gpu:
-            x = x.bfloat16()
-            head = lambda w: w.t().bfloat16().contiguous()
-            ce, kd = vocab.cross_entropy, vocab.distill
-        else:
-            head, ce, kd = torch.t, vocab.reference_cross_entropy, vocab.reference_distill
-        w = head(m.wout)
-        total = x.new_zeros((), dtype=torch.float32)
+        mixed = (self.alpha < 1.0) + (self.alpha > 0.0)
+        second = m.wout_mtp is not None
+        operands = _Operands.apply if on_gpu else lambda t, n: (t,) * n
+        x, w = list(operands(hidden, mixed + second)), list(operands(m.wout.t(), mixed))
+        total = hidden.new_zeros((), dtype=torch.float32)
         if self.alpha < 1.0:
-            total = total + (1.0 - self.alpha) * ce(x, w, targets, self.ignore_index)
+            total = total + (1.0 - self.alpha) * ce(x.pop(), w.pop(), targets, self.ignore_index)
         if self.alpha > 0.0:
-            total = total + self.alpha * kd(x, w, ids, logits, self.temperature)
-        if m.wout_mtp is not None:
+            total = total + self.alpha * kd(x.pop(), w.pop(), ids, logits, self.temperature)
+        if second:
+            w, = operands(m.wout_mtp.t(), 1)
             ahead = mtp_targets(targets, c.mtp_horizon, self.ignore_index)
-            total = total + c.mtp_weight * ce(x, head(m.wout_mtp), ahead, self.ignore_index)
+            total = total + c.mtp_weight * ce(x.pop(), w, ahead, self.ignore_index)
         if balance:
             total = total + c.moe_balance_weight * torch.stack(balance).sum()
         return total

@@ -124,3 +124,15 @@ def test_trainers_without_a_scaled_lookup_refuse_it():
     for bad in (0.0, -1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError):
             cfg.with_(embed_scale=bad).validate()
+
+
+def test_gradients_of_shared_operands_are_added_in_fp32():
+    from predicitivecoding_b200.llm.distill import _Operands
+    t = torch.tensor([[1.0, -3.0], [0.5, 2.0]], requires_grad=True)
+    a, b, unused = _Operands.apply(t.t(), 3)
+    assert a.dtype == torch.bfloat16 and a.is_contiguous() and a.data_ptr() == b.data_ptr() == unused.data_ptr()
+    assert torch.equal(a.float(), t.t())
+    big = torch.tensor([[1.0, 2.0], [3.0, 4.0]])
+    small = big * 2.0 ** -10                         # lost in a sum of 8 bits
+    ((a.float() * big).sum() + (b.float() * small).sum()).backward()
+    assert torch.equal(t.grad, (big + small).t())

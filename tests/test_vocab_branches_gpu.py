@@ -107,3 +107,17 @@ def test_top_logit_distiller_with_a_second_head_on_the_device():
     assert abs(float(got.detach()) - float(want.detach())) <= 1.3 * 2 * 2 * U * size + 1e-4
     for a, b in zip(torch.autograd.grad(got, params()), grads):
         assert float((a.cpu() - b).norm() / b.norm()) <= 8 * U
+
+
+def test_the_distillers_two_heads_are_added_without_another_rounding():
+    """With weights of 1/2 (exact) the gradient of the output matrix is half of the two terms' own, added in fp32."""
+    from predicitivecoding_b200.llm.distill import TopLogitDistiller
+    from predicitivecoding_b200.models.config import DecoderLmConfig
+    from predicitivecoding_b200.models.decoder_lm import DecoderLM
+    cfg = DecoderLmConfig(vocab=900, dim=64, num_blocks=1, num_heads=4, ff_dim=96, max_seq=32, use_rms_norm=True, use_rope=True)
+    student, teacher_ = DecoderLM(cfg, seed=2).to(DEV), DecoderLM(cfg, seed=1).to(DEV)
+    rows = torch.randint(0, 900, (3, 33), generator=torch.Generator().manual_seed(1)).to(DEV)
+    x, y = rows[:, :-1], rows[:, 1:]
+    top = TopLogitDistiller(student, top_k=7).ask(teacher_, x)
+    grad = lambda alpha: torch.autograd.grad(TopLogitDistiller(student, top_k=7, alpha=alpha).loss(x, y, *top), student.wout)[0]
+    assert torch.equal(grad(0.5), 0.5 * grad(0.0) + 0.5 * grad(1.0))
