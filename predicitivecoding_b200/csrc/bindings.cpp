@@ -506,8 +506,9 @@ std::pair<at::Tensor, HeadState> vocab_distill_fwd(const at::Tensor& x, const at
             "distill_fwd: ids and logits must be [*x.shape[:-1], K]");
   PCB_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= pcb::kVocabMaxEntries, "distill_fwd: between 1 and ",
             pcb::kVocabMaxEntries, " entries per row");
-  PCB_CHECK(temperature > 0 && temperature < std::numeric_limits<float>::infinity(),
-            "distill_fwd: temperature must be positive and finite");
+  const float t32 = (float)temperature;   // what the kernels take
+  PCB_CHECK(t32 >= std::numeric_limits<float>::min() && t32 < std::numeric_limits<float>::infinity(),
+            "distill_fwd: temperature must be positive and finite in 32 bits");
   return head_fwd("distill_fwd", x, w, nullptr, -1, &ids, &logits, temperature, reduction, gradient);
 }
 

@@ -109,8 +109,8 @@ class TopLogitDistiller:
                  embed_scale: Optional[float] = None, ignore_index: int = -1):
         if not 1 <= top_k <= min(vocab.MAX_TOP_K, student.cfg.vocab):
             raise ValueError(f"top_k must be between 1 and {min(vocab.MAX_TOP_K, student.cfg.vocab)}")
-        if temperature <= 0:
-            raise ValueError("temperature must be positive")
+        if not 2.0 ** -126 <= temperature < 2.0 ** 127:   # a positive fp32 number, as the operators take it
+            raise ValueError("temperature must be positive and finite")
         if not 0.0 <= alpha <= 1.0:
             raise ValueError("alpha must be between 0 and 1")
         if embed_scale is not None:

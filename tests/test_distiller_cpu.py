@@ -136,3 +136,9 @@ def test_gradients_of_shared_operands_are_added_in_fp32():
     small = big * 2.0 ** -10                         # lost in a sum of 8 bits
     ((a.float() * big).sum() + (b.float() * small).sum()).backward()
     assert torch.equal(t.grad, (big + small).t())
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("inf"), float("nan"), 1e-60, 1e60])
+def test_what_is_no_temperature_is_refused(temperature):
+    with pytest.raises(ValueError):
+        TopLogitDistiller(model(2), top_k=5, temperature=temperature)

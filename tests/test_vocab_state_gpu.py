@@ -137,3 +137,11 @@ def test_gradients_behind_a_wait_that_ran_out_are_nan(N, V, D, f32):
     assert nan(apart) and nan(rows)
     counters(state)[STATUS] = 0
     assert not bool(torch.isnan(vocab.head_bwd(state)[1].float()).any())
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("inf"), float("nan"), 1e-60, 1e60])
+def test_what_is_no_temperature_in_32_bits_is_refused(temperature):
+    x, w, tgt, g = head(8, 40, 16, 15)
+    ids, t = teacher(8, 40, 4, tgt, g, torch.float32)
+    with pytest.raises(ValueError):
+        vocab.distill_fwd(x, w, ids, t, temperature)
