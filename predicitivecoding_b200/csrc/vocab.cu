@@ -8,7 +8,7 @@
 // The logits [N, V] are never kept.  The forward's product (csrc/vocab_gemm.cu) reduces each row's 128 columns to (max,
 // sum) and picks the logits at the targets; the backward makes the logits again, a piece of the vocabulary at a
 // time, and turns them into bf16 p - q, which two more products read: dw of the piece is finished there, dx is
-// accumulated over the pieces in fp32.  8 N V D operations instead of 6, for N * piece * 2 bytes of workspace.
+// accumulated over the pieces in fp32.  8 N V D operations instead of 6, for workspaces that do not grow with N * V.
 // (A vocabulary of up to 512 columns is taken whole where a gradient follows: its loss and p - q come of one product.)
 // Rows without a target (masked prompts, padding) are taken out first: the counted rows are packed in order,
 // the products run over their number, known on the device only, and what stands in the other rows (NaN too) is
@@ -121,7 +121,10 @@ struct PackArgs {
   float* loss;
 };
 constexpr int kCountRows = kThreads;
-constexpr int kSelfCountRows = 8192;   // longer batches are counted by a launch of their own
+// Longer batches are counted by a launch of their own.  Losses of N x 64 against 700, half of the rows counted, each
+// block counting for itself and a launch: 13.5 and 18.0 us at 2048 rows, 18.0 and 18.9 at 4096, 23.1 and 20.5 at 8192,
+// 30.8 and 27.7 at 16384, 54.7 and 39.9 at 32768.
+constexpr int kSelfCountRows = 8192;
 
 PCB_DEVICE bool counted(const PackArgs& a, int n) {
   if (a.len != nullptr) return a.len[n] > 0;
@@ -224,16 +227,16 @@ __global__ void pad_rows_kernel(const __nv_bfloat16* __restrict__ src, long long
 // holds R entries; their ranks are counted together, four other entries at a time.  The table of first entries lies by
 // row, so a block collects it for its rows in shared memory and stores 16 bytes of a column at a time (2048 rows, K
 // 64, V 32000: 12.0 us with a store per entry from 4 rows a block, 14.1 with 32 rows a block, 10.1 as it is).
-constexpr int sort_rows(int R) { return 8; }
+constexpr int kSortRows = 8;
 constexpr int kStartPass = 256;   // columns of the table at a time
 
 template <int R>
-__global__ void __launch_bounds__(32 * sort_rows(R))
+__global__ void __launch_bounds__(32 * kSortRows)
     sort_targets_kernel(const void* __restrict__ ids, int ids64, long long ld_ids, const void* __restrict__ logits,
                         int bf16, long long ld_logits, int N, int V, int K, float c, int* __restrict__ out_ids,
                         float* __restrict__ out_q, float* __restrict__ out_lq, int* __restrict__ out_len,
                         unsigned short* __restrict__ start, int granules) {
-  constexpr int kRows = sort_rows(R);
+  constexpr int kRows = kSortRows;
   __shared__ __align__(16) int s_id[kRows][32 * R];
   __shared__ int s_sorted[kRows][32 * R];
   __shared__ unsigned short s_start[kStartPass][kRows];
@@ -1093,7 +1096,8 @@ __global__ void __launch_bounds__(kThreads)
 // rows without a token.  Sorting against this, tokens that fall off as 1 / rank: 32 tokens into 5003 x 101 8.0 -> 2.9 us,
 // 512 10.3 -> 5.5, 1024 11.4 -> 6.8; 1024 that are all the same 10.7 -> 11.3.  A large matrix's zeros are in the
 // way of the rows: into 32000 x 768 fp32 512 tokens take 20.9 -> 19.7 us, 21.3 -> 21.9 all the same, but 1024 22.1 ->
-// 23.5 and 22.3 -> 31.6.
+// 23.5 and 22.3 -> 31.6.  A warp takes up to 16 places alone: 1024 tokens in runs of 12 into 5003 x 101 take 6.0 us, 9.3 with
+// up to 8; in runs of 24 8.4, 6.2 with up to 32, and all else (1 / rank: 7.1) the same.
 constexpr int kFewTokens = 1024;
 constexpr long long kFewZeros = 32 << 20;   // more zeros than this: half as many tokens
 constexpr int kFewTogether = 16;
@@ -1268,6 +1272,8 @@ static bool few_rows(int N, int D) { return N <= kFewRows && D <= kFewColumns; }
 VocabPlan vocab_plan(int N, int V, int D, int want_piece, bool gradient, int num_sms) {
   VocabPlan r{};
   const long long all = (V + 255LL) / 256 * 256;
+  // 256 MiB of g: the backward of 16384 x 768 x 32000 takes 1868 us (128 MiB: 1970, 64: 2648, 512: 1830, 1024, which is one
+  // piece: 1756)
   long long p = want_piece > 0 ? (want_piece + 255LL) / 256 * 256 : (256LL << 20) / (2 * vocab_g_rows(N)) / 256 * 256;
   p = std::max(256LL, std::min(p, all));
   r.pieces = (int)((all + p - 1) / p);
@@ -1357,7 +1363,7 @@ int pcb_vocab_fwd(const VocabHeadArgs& a, const VocabPlan& plan, void* saved, vo
   const float c = 1.4426950408889634f / T, factor = 0.6931471805599453f * T * T;
   if (distill) {
     auto sort = [&](auto r) {
-      constexpr int R = decltype(r)::value, rows = sort_rows(R);
+      constexpr int R = decltype(r)::value, rows = kSortRows;
       return pdl_launch(sort_targets_kernel<R>, dim3((a.N + rows - 1) / rows), dim3(32 * rows), 0, s, a.ids, a.ids64, a.ld_ids, a.logits, a.logits_bf16, a.ld_logits, a.N, a.V,
                         a.K, c, ids, q, lq, len, start, l.granules);
     };

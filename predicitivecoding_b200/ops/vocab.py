@@ -27,7 +27,8 @@ are none.  A teacher's entry is absent when its id is outside [0, V) or its logi
 
 The ids of a row's list are meant to differ; entries that repeat an id count as they stand in the loss, and together
 in the gradient.  All results are the same from run to run: no sum depends on the order in which atomics arrive.
-x and w are read again by ``head_bwd`` and must not change in between.
+x and w are read again by ``head_bwd`` and must not change in between; the state keeps them, next to its own buffers, for as
+long as it lives (the autograd forms: as long as the graph does, outside the hooks of saved tensors).
 A kernel that gives up a wait (which none does unless the device is in trouble) records it in the state: the loss and
 the gradients made from it are NaN then, and ``state.status()``, which synchronises, returns the wait's code instead
 of 0.  Several backwards of one state may run at the same time.
@@ -57,8 +58,9 @@ def embed_fwd(tok: torch.Tensor, w: torch.Tensor, scale: float = 1.0, out: Optio
 def embed_bwd(tok: torch.Tensor, dx: torch.Tensor, vocab: int, scale: float = 1.0, out: Optional[torch.Tensor] = None,
               dtype: torch.dtype = torch.float32, accumulate: bool = False) -> torch.Tensor:
     """Gradient of :func:`embed_fwd` by w: [vocab, D] of ``dtype``, or into ``out`` (added to it with
-    ``accumulate``, as for a matrix that the output head shares).  dx [..., D] fp32 or bf16.  The tokens are sorted
-    and each row's sum is taken in fp32 in ascending order of place, then rounded once."""
+    ``accumulate``, as for a matrix that the output head shares).  dx [..., D] fp32 or bf16.  Each row's sum is taken
+    in fp32 over its tokens in ascending order of place, in parts of a fixed size where they are many, then rounded once.
+    Batches above 1024 tokens (512 into a large matrix) are sorted; their workspace is N * D bytes and some per token."""
     return ext().vocab_embed_bwd(tok, dx, vocab, scale, out, dtype, accumulate)
 
 
